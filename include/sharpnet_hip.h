@@ -363,6 +363,147 @@ int snhip_rnn_backward_weights(void* handle, const snhip_rnn_desc* desc, int bat
                                const float* hx, const float* y, float* weight_gradients, void* workspace,
                                size_t workspace_bytes, void* reserve, size_t reserve_bytes);
 
+/* ---- word embedding --------------------------------------------------------- */
+/* Types of operands that are not always fp32. */
+#define SNHIP_TYPE_F32 0
+#define SNHIP_TYPE_BF16 1
+#define SNHIP_TYPE_I32 2
+#define SNHIP_TYPE_I64 3
+
+/* y[t] = scale * table[id[t]] and its gradient, table_gradient[v] = scale * sum of dy[t] over the tokens t with id[t] = v:
+ * the reference's WordEmbeddingForwardPropagation / WordEmbeddingBackwardPropagation kernels
+ * (Prod/GPU/Kernels/SinglePrecision.cu:617,650).  table is vocabulary x dim, y and dy are tokens x dim, both row-major
+ * with the given row pitches.  Ids may be 32- or 64-bit integers or floats (the reference's form; rounded toward zero).
+ * An id outside [0, vocabulary), or NaN, is no token: its row of y is zeros and it adds nothing to the gradient.
+ * A row dy[t] of such a token is not read, nor is that of padding_index. */
+typedef struct snhip_embedding_desc {
+    int struct_size;
+    int id_type;     /* SNHIP_TYPE_F32, _I32 or _I64 */
+    int table_type;  /* SNHIP_TYPE_F32 or _BF16 (the gradient is always fp32) */
+    int output_type; /* of y and dy: SNHIP_TYPE_F32 or _BF16 */
+    long long tokens;
+    int vocabulary, dim;
+    long long ld_table, ld_output; /* row pitches in elements, 0 = dim; ld_table is also the gradient's */
+    int padding_index;             /* the tokens with this id get their row but add nothing to the gradient; -1: none */
+    float scale;
+} snhip_embedding_desc;
+int snhip_sizeof_embedding_desc(void);
+int snhip_embedding_forward(void* handle, const snhip_embedding_desc* desc, const void* ids, const void* table, void* y);
+/* Bytes of device memory that snhip_embedding_backward needs for a descriptor (the sorted order and partial sums). */
+int snhip_embedding_backward_workspace_size(const snhip_embedding_desc* desc, size_t* bytes);
+/* Writes every row of table_gradient (zeros where no token has the id), or adds to it with accumulate != 0.  workspace is
+ * scratch for this call (16-byte aligned; less than the size above is refused with status 7): the caller's own, so that
+ * two calls on two streams or in two captured graphs only meet if they are given the same one.  The order of the sums
+ * depends on the ids alone: bits repeat from run to run. */
+int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, const void* ids, const void* dy,
+                             float* table_gradient, int accumulate, void* workspace, size_t workspace_bytes);
+
+/* ---- norms before and after a block ------------------------------------------ */
+/* The join between two blocks of a network in one pass over the rows (every part but x optional):
+ *     u = x + residual_scale * act(gate) * N_post(y)      y: the block's output, x: the residual stream
+ *     h = N_pre(u)                                        what the next block reads (u as it is stored)
+ * with N(z) = (z - mean) * rstd * weight + bias (SNHIP_NORM_LAYER) or z * rstd * weight + bias (SNHIP_NORM_RMS),
+ * rstd = 1 / sqrt(mean of (z - mean)^2 + epsilon) with mean = 0 for RMS, over the `dim` elements of a row: the reference's
+ * StandardizeRowsInPlaceBroadcastGammasBetas / RMSStandardizeRowsInPlaceBroadcastGammas and the LayerNormalizationBackward
+ * / RMSNormalizationBackward kernels (Prod/GPU/Kernels/SinglePrecision.cu:82,108,158-236).
+ * Without y the call is the norm alone (u is not written and may be NULL); with pre_norm = SNHIP_NORM_NONE there is no h.
+ * gate: NULL; one fp32 vector of dim elements (gate_rows = 0); or rows of block_type, row r / gate_rows for row r.
+ * weights and biases are fp32 vectors of dim elements, NULL for ones and zeros; post_weight / post_bias belong to
+ * post_norm and are ignored without it.
+ * statistics: (mean, rstd) per row as the backward call wants them, NULL to skip; sums are taken in fp32 over the row in
+ * registers, the variance around the mean.
+ * Backward, from dh and du (the gradients that reach h and u; either may be NULL = zeros, not both):
+ *     t = du + dN_pre(dh);  dx = t;  dy = dN_post(residual_scale * act(gate) * t)
+ * and the gradients of gate, weights and biases (each NULL to skip) summed over the rows in a fixed order: bits repeat.
+ * x / dx, y / dy, u / du, h / dh and gate / d_gate share their row pitch (0: dim).  u may be x, h may be y, dx may be du and
+ * dy may be dh, if their types and pitches are equal; other overlaps are not allowed.
+ * dim is at most 8192 (status 15 beyond), stream_type must not be bf16 with an fp32 block_type (status 15). */
+#define SNHIP_NORM_NONE 0
+#define SNHIP_NORM_RMS 1
+#define SNHIP_NORM_LAYER 2
+typedef struct snhip_block_norm_desc {
+    int struct_size;
+    int stream_type; /* of x, u, dx, du: SNHIP_TYPE_F32 or _BF16 */
+    int block_type;  /* of y, h, dy, dh and a gate in rows */
+    int pre_norm, post_norm;
+    int gate_activation; /* SNHIP_ACT_NONE, _SIGMOID or _TANH */
+    int dim, gate_rows;
+    long long rows;
+    long long ld_x, ld_y, ld_u, ld_h, ld_gate;
+    float epsilon, residual_scale;
+    const float* pre_weight;
+    const float* pre_bias;
+    const float* post_weight;
+    const float* post_bias;
+    const void* gate;
+    const void* x;
+    const void* y;
+    void* u; /* written by the forward call, read by the backward call */
+    void* h;
+    float* pre_statistics; /* [rows][2]; written by the forward call, read by the backward call */
+    float* post_statistics;
+    /* the backward call alone */
+    const void* du;
+    const void* dh;
+    void* dx;
+    void* dy;
+    void* d_gate; /* fp32 for a vector, block_type for rows */
+    float* d_pre_weight;
+    float* d_pre_bias;
+    float* d_post_weight;
+    float* d_post_bias;
+    int accumulate; /* != 0: d_pre_weight ... d_post_bias and the gradient of a gate vector are added to */
+} snhip_block_norm_desc;
+int snhip_sizeof_block_norm_desc(void);
+int snhip_block_norm_forward(void* handle, const snhip_block_norm_desc* desc);
+/* Bytes of device memory that snhip_block_norm_backward needs for a descriptor (partial column sums); 0 is possible. */
+int snhip_block_norm_backward_workspace_size(const snhip_block_norm_desc* desc, size_t* bytes);
+/* workspace: the caller's own scratch for this call, 16-byte aligned (see snhip_embedding_backward). */
+int snhip_block_norm_backward(void* handle, const snhip_block_norm_desc* desc, void* workspace, size_t workspace_bytes);
+
+/* ---- AdamW over many tensors at once -------------------------------------------- */
+/* One launch updates every element of every tensor of a plan (the reference's UpdateAdamOptimizer kernel,
+ * Prod/GPU/Kernels/SinglePrecision.cu:19, one launch per tensor, with decoupled weight decay):
+ *     g = gradient_scale * gradient;  m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g g
+ *     p' = p (1 - learning_rate weight_decay) - learning_rate / (1 - beta1^step) * m' / (sqrt(v') / sqrt(1 - beta2^step) + epsilon)
+ * in fp32, each product and sum of m' and v' rounded by itself, and writes a bf16 copy of p' for the bf16-stored products
+ * where a tensor has one.
+ * state_bits = 32: moment1 and moment2 are fp32.  state_bits = 8: blocks of 256 consecutive elements of a tensor (the last
+ * one shorter) keep m in e4m3 and v in e5m2 with a power of two per block and moment, 2^(scale - 127): scale1 / scale2 hold
+ * one byte a block, max(e - 7, 1) for m and max(e - 14, 1) for v, where e is the biased exponent of the block's largest
+ * finite magnitude.  m' and v' are rounded up or down at random (unbiased: with 2 or 3 bits after the point the 0.1 % a step
+ * that v moves by would never show under rounding to nearest) with 16 bits each of Philox4x32-10, key = seed, counter =
+ * {element / 4 low word, high word, tensor, step}, word element % 4, low half for m, high half for v.  A positive v' is
+ * never stored as zero; a moment that is not finite is stored as NaN.  Zeroed states (all bytes 0) are zero moments. */
+typedef struct snhip_adamw_tensor {
+    float* parameter;
+    const void* gradient;
+    void* moment1;
+    void* moment2;
+    unsigned char* scale1; /* state_bits = 8: (count + 255) / 256 bytes; ignored else */
+    unsigned char* scale2;
+    void* bf16_copy; /* or NULL */
+    long long count;
+    int gradient_type; /* SNHIP_TYPE_F32 or _BF16 */
+    float weight_decay;
+} snhip_adamw_tensor;
+typedef struct snhip_adamw_step_desc {
+    int struct_size;
+    int step; /* 1 for the first */
+    double learning_rate, beta1, beta2, epsilon;
+    float gradient_scale;
+    unsigned long long seed;
+} snhip_adamw_step_desc;
+int snhip_sizeof_adamw_tensor(void);
+int snhip_sizeof_adamw_step_desc(void);
+/* Lays out the table of the tensors in device memory (synchronises, allocates: not under stream capture).  The addresses
+ * must stay valid until the plan is destroyed.  Tensors whose parameters, states or copies overlap are refused (status 7). */
+int snhip_adamw_create(void* handle, const snhip_adamw_tensor* tensors, int count, int state_bits, void** plan);
+/* The plan's last step must have finished on the device. */
+int snhip_adamw_destroy(void* plan);
+/* May be captured into a graph: a replay repeats the step with the scalars of the capture. */
+int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* step);
+
 /* ---- bf16-input / fp32-accumulate variant (no reference counterpart) ------ */
 /* Operands stay fp32 in device memory; they are rounded to bf16 (nearest even)
  * on their way into LDS and multiplied with v_mfma_f32_32x32x16_bf16, products

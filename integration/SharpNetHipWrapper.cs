@@ -168,6 +168,60 @@ namespace SharpNet.GPU
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_gemm_ex(IntPtr handle, ref GemmDesc desc);
         [DllImport(DLL_NAME)] public static extern int snhip_sizeof_gemm_desc();
 
+        // word embedding, norms around a block, AdamW over all tensors: the descriptors of include/sharpnet_hip.h, field for
+        // field (check them once against the snhip_sizeof_* functions)
+        [StructLayout(LayoutKind.Sequential)]
+        public struct EmbeddingDesc
+        {
+            public int struct_size, id_type, table_type, output_type;   // 0 float (the reference's ids), 1 bf16, 2 int, 3 long
+            public long tokens;
+            public int vocabulary, dim;
+            public long ld_table, ld_output;    // 0: dim
+            public int padding_index;           // -1: none
+            public float scale;
+        }
+        [DllImport(DLL_NAME)] public static extern int snhip_sizeof_embedding_desc();
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_embedding_forward(IntPtr handle, ref EmbeddingDesc desc, IntPtr ids, IntPtr table, IntPtr y);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_embedding_backward_workspace_size(ref EmbeddingDesc desc, out size_t bytes);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_embedding_backward(IntPtr handle, ref EmbeddingDesc desc, IntPtr ids, IntPtr dy,
+            IntPtr tableGradient, int accumulate, IntPtr workspace, size_t workspaceBytes);
+        [StructLayout(LayoutKind.Sequential)]
+        public struct BlockNormDesc
+        {
+            public int struct_size, stream_type, block_type, pre_norm, post_norm, gate_activation, dim, gate_rows;
+            public long rows, ld_x, ld_y, ld_u, ld_h, ld_gate;
+            public float epsilon, residual_scale;
+            public IntPtr pre_weight, pre_bias, post_weight, post_bias, gate, x, y, u, h, pre_statistics, post_statistics;
+            public IntPtr du, dh, dx, dy, d_gate, d_pre_weight, d_pre_bias, d_post_weight, d_post_bias;
+            public int accumulate;
+        }
+        [DllImport(DLL_NAME)] public static extern int snhip_sizeof_block_norm_desc();
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_block_norm_forward(IntPtr handle, ref BlockNormDesc desc);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_block_norm_backward_workspace_size(ref BlockNormDesc desc, out size_t bytes);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_block_norm_backward(IntPtr handle, ref BlockNormDesc desc, IntPtr workspace, size_t workspaceBytes);
+        [StructLayout(LayoutKind.Sequential)]
+        public struct AdamwTensor
+        {
+            public IntPtr parameter, gradient, moment1, moment2, scale1, scale2, bf16_copy;
+            public long count;
+            public int gradient_type;
+            public float weight_decay;
+        }
+        [StructLayout(LayoutKind.Sequential)]
+        public struct AdamwStepDesc
+        {
+            public int struct_size, step;
+            public double learning_rate, beta1, beta2, epsilon;
+            public float gradient_scale;
+            public ulong seed;
+        }
+        [DllImport(DLL_NAME)] public static extern int snhip_sizeof_adamw_tensor();
+        [DllImport(DLL_NAME)] public static extern int snhip_sizeof_adamw_step_desc();
+        // tensors: the address of a pinned AdamwTensor[]
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_adamw_create(IntPtr handle, IntPtr tensors, int count, int stateBits, out IntPtr plan);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_adamw_destroy(IntPtr plan);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_adamw_step(IntPtr handle, IntPtr plan, ref AdamwStepDesc step);
+
         // device memory / stream (replace the nvcuda P/Invokes used by GPUTensor)
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_malloc(out IntPtr dptr, UIntPtr bytes);
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_free(IntPtr dptr);

@@ -18,11 +18,18 @@ LIB_PATH = os.path.join(HERE, LIB_NAME)
 MAIN_SOURCE = os.path.join(CSRC, "sharpnet_hip.hip")       # C ABI, dispatch, small kernels
 KERNEL_SOURCE = os.path.join(CSRC, "gemm_kernels.hip")     # GEMM kernels, compiled once per group of kernel_list.hpp
 KERNEL_GROUPS = 10                                         # SNHIP_NUM_KERNEL_GROUPS
-SOURCES = [MAIN_SOURCE, KERNEL_SOURCE]
-HEADERS = [os.path.join(CSRC, n) for n in ("sgemm_mfma.hpp", "bgemm_mfma.hpp", "rowops.hpp", "kernel_list.hpp", "attention_mfma.hpp", "rnn_cells.hpp", "rnn_layers.hpp", "sgemm_ksplit.hpp", "sgemm_stream.hpp", "bgemm_dtl.hpp")] + \
+TRAINING_SOURCE = os.path.join(CSRC, "training_ops.hip")   # entry points of the training operators, embedding and AdamW kernels
+NORM_SOURCE = os.path.join(CSRC, "block_norm.hip")         # block norm kernels, compiled once per combination of types
+NORM_TYPES = 3
+SOURCES = [MAIN_SOURCE, KERNEL_SOURCE, TRAINING_SOURCE, NORM_SOURCE]
+HEADERS = [os.path.join(CSRC, n) for n in ("sgemm_mfma.hpp", "bgemm_mfma.hpp", "rowops.hpp", "kernel_list.hpp", "attention_mfma.hpp", "rnn_cells.hpp", "rnn_layers.hpp", "sgemm_ksplit.hpp", "sgemm_stream.hpp", "bgemm_dtl.hpp", "handle.hpp", "philox.hpp")] + \
           [os.path.join(REPO, "include", "sharpnet_hip.h")]
 # what gemm_kernels.hip includes; the other headers belong to the translation unit with the C ABI
 KERNEL_HEADERS = [os.path.join(CSRC, n) for n in ("sgemm_mfma.hpp", "bgemm_mfma.hpp", "kernel_list.hpp")]
+TRAINING_HEADERS = [os.path.join(CSRC, n) for n in ("embedding.hpp", "adamw.hpp", "philox.hpp", "column_parts.hpp", "block_norm.hpp",
+                                                      "block_norm_launch.hpp", "handle.hpp", "vec_types.hpp")] + \
+                   [os.path.join(REPO, "include", "sharpnet_hip.h")]
+NORM_HEADERS = [os.path.join(CSRC, n) for n in ("block_norm.hpp", "block_norm_launch.hpp", "vec_types.hpp")]
 OBJ_DIR = os.path.join(HERE, "_obj")
 
 HIPCC_FLAGS = [
@@ -49,7 +56,7 @@ def is_stale():
     if not os.path.exists(LIB_PATH):
         return True
     built = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(p) > built for p in SOURCES + HEADERS)
+    return any(os.path.getmtime(p) > built for p in SOURCES + HEADERS + TRAINING_HEADERS)
 
 
 def _run(cmd, verbose):
@@ -67,7 +74,7 @@ def build_library(force=False, verbose=True, jobs=None):
     """Compile the HIP sources into libsharpnet_hip.so.  Returns the library path.
 
     The GEMM kernels are split into KERNEL_GROUPS translation units that are compiled side by side
-    (``jobs`` at a time, default min(8, cpu count)); one more unit holds the C ABI.  Everything is linked into
+    (``jobs`` at a time, default min(8, cpu count)); one more unit holds the C ABI, others the operators around the layers.  Everything is linked into
     one shared library.
     """
     if not force and not is_stale():
@@ -76,7 +83,11 @@ def build_library(force=False, verbose=True, jobs=None):
     hipcc = find_hipcc()
     os.makedirs(OBJ_DIR, exist_ok=True)
     inc = ["-I", os.path.join(REPO, "include")]
-    units = [([hipcc] + HIPCC_FLAGS + inc + ["-c", MAIN_SOURCE, "-o", os.path.join(OBJ_DIR, "sharpnet_hip.o")])]
+    units = [([hipcc] + HIPCC_FLAGS + inc + ["-c", MAIN_SOURCE, "-o", os.path.join(OBJ_DIR, "sharpnet_hip.o")]),
+             ([hipcc] + HIPCC_FLAGS + inc + ["-c", TRAINING_SOURCE, "-o", os.path.join(OBJ_DIR, "training_ops.o")])]
+    for t in range(NORM_TYPES):
+        units.append([hipcc] + HIPCC_FLAGS + inc + ["-DSNHIP_NORM_TYPES=%d" % t, "-c", NORM_SOURCE, "-o",
+                                                    os.path.join(OBJ_DIR, "block_norm_%d.o" % t)])
     for g in range(KERNEL_GROUPS):
         units.append([hipcc] + HIPCC_FLAGS + inc + ["-DSNHIP_KERNEL_GROUP=%d" % g, "-c", KERNEL_SOURCE, "-o",
                                                     os.path.join(OBJ_DIR, "gemm_kernels_%d.o" % g)])
@@ -86,7 +97,7 @@ def build_library(force=False, verbose=True, jobs=None):
         # rebuild only the objects that are older than their own source or a header they include
         def fresh(unit):
             obj, src = unit[-1], unit[-3]
-            deps = HEADERS if src == MAIN_SOURCE else KERNEL_HEADERS
+            deps = {MAIN_SOURCE: HEADERS, TRAINING_SOURCE: TRAINING_HEADERS, NORM_SOURCE: NORM_HEADERS}.get(src, KERNEL_HEADERS)
             return os.path.exists(obj) and all(os.path.getmtime(p) <= os.path.getmtime(obj) for p in [src] + deps)
         units = [u for u in units if not fresh(u)]
     with ThreadPoolExecutor(max_workers=jobs) as pool:

@@ -1,0 +1,89 @@
+// The block norm kernels for one combination of storage types, SNHIP_NORM_TYPES = 0, 1 or 2 (block_norm_launch.hpp).
+#include "block_norm_launch.hpp"
+
+#ifndef SNHIP_NORM_TYPES
+#error "compile with -DSNHIP_NORM_TYPES=0..2"
+#endif
+
+namespace snhip {
+
+#if SNHIP_NORM_TYPES == 0
+typedef float Stream;
+typedef float Block;
+#define SNHIP_FORWARD block_norm_forward_0
+#define SNHIP_BACKWARD block_norm_backward_0
+#elif SNHIP_NORM_TYPES == 1
+typedef float Stream;
+typedef __bf16 Block;
+#define SNHIP_FORWARD block_norm_forward_1
+#define SNHIP_BACKWARD block_norm_backward_1
+#else
+typedef __bf16 Stream;
+typedef __bf16 Block;
+#define SNHIP_FORWARD block_norm_forward_2
+#define SNHIP_BACKWARD block_norm_backward_2
+#endif
+
+namespace {
+
+template <int TPR, int N>
+void forward(const BlockNormParams& p, hipStream_t stream) {
+    constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
+    hipLaunchKernelGGL((block_norm_forward_kernel<Stream, Block, TPR, N>), dim3((unsigned)((p.rows + GROUPS - 1) / GROUPS)),
+                       dim3(NT), 0, stream, p);
+}
+
+template <int TPR, int N, int MODE, bool BIAS, bool GATE>
+void backward(const BlockNormParams& p, hipStream_t stream) {
+    constexpr int NT = TPR > 256 ? TPR : 256;
+    hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE>), dim3((unsigned)p.chunks), dim3(NT),
+                       0, stream, p);
+}
+
+template <int TPR, int N>
+void backward_kind(const BlockNormParams& p, BlockNormKind k, hipStream_t stream) {
+    if (k.mode == 0)
+        k.bias ? backward<TPR, N, 0, true, false>(p, stream) : backward<TPR, N, 0, false, false>(p, stream);
+    else if (k.mode == 1 && k.gate)
+        k.bias ? backward<TPR, N, 1, true, true>(p, stream) : backward<TPR, N, 1, false, true>(p, stream);
+    else if (k.mode == 1)
+        k.bias ? backward<TPR, N, 1, true, false>(p, stream) : backward<TPR, N, 1, false, false>(p, stream);
+    else if (k.gate)
+        k.bias ? backward<TPR, N, 2, true, true>(p, stream) : backward<TPR, N, 2, false, true>(p, stream);
+    else
+        k.bias ? backward<TPR, N, 2, true, false>(p, stream) : backward<TPR, N, 2, false, false>(p, stream);
+}
+
+}  // namespace
+
+// A row of up to 1024 elements is one wavefront's (no barrier), a longer one a workgroup's; with few rows to go round a row
+// is spread over as many threads as it has pieces of four.
+void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
+    const int units = (p.dim + 3) / 4;
+    if (units <= 16) return forward<16, 1>(p, stream);
+    if (units <= 64) return forward<64, 1>(p, stream);
+    if (p.rows <= 512) {
+        if (units <= 256) return forward<256, 1>(p, stream);
+        if (units <= 1024) return forward<1024, 1>(p, stream);
+        return forward<1024, 2>(p, stream);
+    }
+    if (units <= 128) return forward<64, 2>(p, stream);
+    if (units <= 256) return forward<64, 4>(p, stream);
+    if (units <= 512) return forward<256, 2>(p, stream);
+    if (units <= 1024) return forward<256, 4>(p, stream);
+    forward<256, 8>(p, stream);
+}
+
+// (the groups of threads per workgroup: block_norm_backward_groups)
+void SNHIP_BACKWARD(const BlockNormParams& p, BlockNormKind kind, hipStream_t stream) {
+    const int units = (p.dim + 3) / 4;
+    if (units <= 16) return backward_kind<16, 1>(p, kind, stream);
+    if (units <= 64) return backward_kind<64, 1>(p, kind, stream);
+    if (units <= 128) return backward_kind<64, 2>(p, kind, stream);
+    if (units <= 256) return backward_kind<256, 1>(p, kind, stream);
+    if (units <= 512) return backward_kind<256, 2>(p, kind, stream);
+    if (units <= 1024) return backward_kind<512, 2>(p, kind, stream);
+    backward_kind<1024, 2>(p, kind, stream);
+}
+
+}  // namespace snhip

@@ -12,6 +12,7 @@
 #include <new>
 
 #include "attention_mfma.hpp"
+#include "handle.hpp"
 #include "kernel_list.hpp"
 #include "rowops.hpp"
 #include "bgemm_dtl.hpp"
@@ -52,27 +53,6 @@ hipError_t static_scratch_address(int dev, void** out) {
 }
 
 constexpr int kVersion = 100;  // 0.1.0
-
-struct Handle {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    float* ws = nullptr;      // split-K partial sums
-    size_t ws_bytes = 0;
-    int* counters = nullptr;  // split-K arrival counters, zero whenever no GEMM is in flight
-    size_t n_counters = 0;
-    int splitk_mode = 0;      // 0: automatic, 1: always reduce in a second kernel, 2: always reduce in the GEMM kernel
-    int num_cu = 256;
-    int math_mode = 0;  // 0: fp32 MFMA, 1: bf16-input MFMA for every GEMM on this handle
-    int force_cfg = -1;
-    int force_splitk = 0;
-    int last_cfg = -1;
-    int last_splitk = 0;
-    int rnn_step_mode = 0;  // 0: recurrent forward steps as one launch when the shape allows, 1: always GEMM + cell kernel
-    unsigned long long rnn_dropout_seed = 0;   // the reference seeds cuDNN's dropout states with 0 (GPUWrapper.cs:472)
-    unsigned long long rnn_dropout_calls = 0;  // training-mode forward calls that drew masks so far
-    float* static_scratch = nullptr;  // this device's copy of `scratch` (kStaticScratchBytes), never freed
-    char last_error[192] = {0};       // text of the last refusal that has more to say than its status code
-};
 
 // Upper bound for the split-K workspace; larger requests fall back to fewer splits.
 constexpr size_t kMaxWorkspaceBytes = size_t(1) << 30;
@@ -311,25 +291,6 @@ const Attn16Entry* find_attn16(const Attn16Entry (&table)[N], int keys, int hd) 
         if (c.keys == keys && c.hd == hd) return &c;
     return nullptr;
 }
-
-int hip_to_status(hipError_t e) {
-    switch (e) {
-        case hipSuccess:
-            return SNHIP_STATUS_SUCCESS;
-        case hipErrorOutOfMemory:
-            return SNHIP_STATUS_ALLOC_FAILED;
-        case hipErrorInvalidValue:
-        case hipErrorInvalidDevicePointer:
-            return SNHIP_STATUS_INVALID_VALUE;
-        case hipErrorNotInitialized:
-        case hipErrorNoDevice:
-            return SNHIP_STATUS_NOT_INITIALIZED;
-        default:
-            return SNHIP_STATUS_EXECUTION_FAILED;
-    }
-}
-
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 hipError_t rnn_prepare_kernels();  // rnn_layers.hpp: LDS opt-in of the recurrent step kernels
 

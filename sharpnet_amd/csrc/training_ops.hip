@@ -1,0 +1,511 @@
+// C ABI of the operators around the Dense, attention and recurrent layers in a training step: argument checks, choice of
+// launch shape, launches.  Declarations are in include/sharpnet_hip.h.
+#include "../../include/sharpnet_hip.h"
+
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <memory>
+#include <new>
+#include <vector>
+
+#include "adamw.hpp"
+#include "block_norm_launch.hpp"
+#include "column_parts.hpp"
+#include "embedding.hpp"
+#include "handle.hpp"
+
+using namespace snhip;
+
+namespace {
+
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+bool is_storage_type(int type) { return type == SNHIP_TYPE_F32 || type == SNHIP_TYPE_BF16; }
+size_t type_bytes(int type) { return type == SNHIP_TYPE_BF16 ? 2 : type == SNHIP_TYPE_I64 ? 8 : 4; }
+size_t up256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+// ---- word embedding ------------------------------------------------------------------------------------------
+
+int embedding_check_desc(const snhip_embedding_desc* d) {
+    if (d == nullptr || d->struct_size != (int)sizeof(snhip_embedding_desc)) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->id_type != SNHIP_TYPE_F32 && d->id_type != SNHIP_TYPE_I32 && d->id_type != SNHIP_TYPE_I64)
+        return SNHIP_STATUS_INVALID_VALUE;
+    if (!is_storage_type(d->table_type) || !is_storage_type(d->output_type)) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->tokens < 0 || d->vocabulary < 0 || d->dim < 0 || d->padding_index < -1) return SNHIP_STATUS_INVALID_VALUE;
+    if ((d->ld_table != 0 && d->ld_table < d->dim) || (d->ld_output != 0 && d->ld_output < d->dim))
+        return SNHIP_STATUS_INVALID_VALUE;
+    // token numbers and the places in the sorted order are 32-bit integers
+    if (d->tokens > 0x7fff0000LL || d->vocabulary > 0x7fff0000) return SNHIP_STATUS_NOT_SUPPORTED;
+    return SNHIP_STATUS_SUCCESS;
+}
+
+EmbeddingParams embedding_params(const snhip_embedding_desc* d, const void* ids, const void* in, void* out, bool backward) {
+    EmbeddingParams p{};
+    p.ids = ids, p.in = in, p.out = out;
+    p.tokens = d->tokens, p.vocabulary = d->vocabulary, p.dim = d->dim, p.scale = d->scale;
+    const long long ldt = d->ld_table != 0 ? d->ld_table : d->dim, ldo = d->ld_output != 0 ? d->ld_output : d->dim;
+    p.ld_in = backward ? ldo : ldt, p.ld_out = backward ? ldt : ldo;
+    p.padding = backward && d->padding_index < d->vocabulary ? d->padding_index : -1;
+    const int in_type = backward ? d->output_type : d->table_type, out_type = backward ? SNHIP_TYPE_F32 : d->output_type;
+    p.whole = d->dim % 4 == 0 && ldt % 4 == 0 && ldo % 4 == 0 && aligned(in, 4 * type_bytes(in_type)) &&
+              aligned(out, 4 * type_bytes(out_type));
+    const int units = ceil_div(d->dim, 4);
+    p.lanes_log2 = 3;
+    while (p.lanes_log2 < 8 && (1 << p.lanes_log2) < units) ++p.lanes_log2;
+    return p;
+}
+
+struct EmbeddingPlan {
+    int bins, chunk;
+    long long chunks;
+    size_t order, sorted, offsets, partial, bytes;  // places in the workspace
+};
+EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
+    EmbeddingPlan e{};
+    e.bins = ceil_div(d->vocabulary, 256);
+    if (e.bins < 1) e.bins = 1;
+    if (e.bins > 512) e.bins = 512;
+    e.chunk = d->tokens >= 16384 ? 32 : 8;
+    e.chunks = (d->tokens + e.chunk - 1) / e.chunk;
+    e.order = 0;
+    e.sorted = e.order + up256((size_t)d->tokens * 4);
+    e.offsets = e.sorted + up256((size_t)d->tokens * 4);
+    e.partial = e.offsets + up256(((size_t)d->vocabulary + 1) * 4);
+    e.bytes = e.partial + up256((size_t)e.chunks * 2 * (size_t)d->dim * 4);
+    return e;
+}
+
+template <typename ID, typename TIN, typename TOUT>
+void embedding_forward_launch(const EmbeddingParams& p, hipStream_t stream) {
+    constexpr int ROWS = 4;
+    const int groups = 256 >> p.lanes_log2;
+    const long long blocks = (p.tokens + (long long)groups * ROWS - 1) / ((long long)groups * ROWS);
+    hipLaunchKernelGGL((embedding_forward_kernel<ID, TIN, TOUT, ROWS>),
+                       dim3((unsigned)blocks, (unsigned)ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2)), dim3(256), 0, stream, p);
+}
+template <typename ID>
+void embedding_forward_types(const EmbeddingParams& p, int table_type, int output_type, hipStream_t stream) {
+    const bool tb = table_type == SNHIP_TYPE_BF16, ob = output_type == SNHIP_TYPE_BF16;
+    if (tb && ob)
+        embedding_forward_launch<ID, __bf16, __bf16>(p, stream);
+    else if (tb)
+        embedding_forward_launch<ID, __bf16, float>(p, stream);
+    else if (ob)
+        embedding_forward_launch<ID, float, __bf16>(p, stream);
+    else
+        embedding_forward_launch<ID, float, float>(p, stream);
+}
+
+// ---- block norm ----------------------------------------------------------------------------------------------
+
+int block_norm_check_desc(const snhip_block_norm_desc* d, bool backward) {
+    if (d == nullptr || d->struct_size != (int)sizeof(snhip_block_norm_desc)) return SNHIP_STATUS_INVALID_VALUE;
+    if (!is_storage_type(d->stream_type) || !is_storage_type(d->block_type)) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->pre_norm < SNHIP_NORM_NONE || d->pre_norm > SNHIP_NORM_LAYER || d->post_norm < SNHIP_NORM_NONE ||
+        d->post_norm > SNHIP_NORM_LAYER)
+        return SNHIP_STATUS_INVALID_VALUE;
+    if (d->gate_activation != SNHIP_ACT_NONE && d->gate_activation != SNHIP_ACT_SIGMOID && d->gate_activation != SNHIP_ACT_TANH)
+        return SNHIP_STATUS_NOT_SUPPORTED;
+    if (d->rows < 0 || d->dim < 0 || d->gate_rows < 0) return SNHIP_STATUS_INVALID_VALUE;
+    const long long lds[] = {d->ld_x, d->ld_y, d->ld_u, d->ld_h, d->ld_gate};
+    for (long long ld : lds)
+        if (ld != 0 && ld < d->dim) return SNHIP_STATUS_INVALID_VALUE;
+    if (!(d->epsilon >= 0.0f) || !(d->epsilon < INFINITY)) return SNHIP_STATUS_INVALID_VALUE;
+    // a gate or a norm behind the block without a block; nothing to compute
+    if (d->y == nullptr && (d->gate != nullptr || d->post_norm != SNHIP_NORM_NONE || d->pre_norm == SNHIP_NORM_NONE))
+        return SNHIP_STATUS_INVALID_VALUE;
+    if (d->dim > kBlockNormMaxDim || d->rows > 0x7fffffffLL) return SNHIP_STATUS_NOT_SUPPORTED;
+    if (d->stream_type == SNHIP_TYPE_BF16 && d->block_type == SNHIP_TYPE_F32) return SNHIP_STATUS_NOT_SUPPORTED;
+    const size_t sb = type_bytes(d->stream_type), bb = type_bytes(d->block_type), gb = d->gate_rows == 0 ? 4 : bb;
+    const void* streams[] = {d->x, d->u, d->du, d->dx};
+    const void* blocks[] = {d->y, d->h, d->dh, d->dy};
+    const void* floats[] = {d->pre_weight, d->pre_bias, d->post_weight, d->post_bias, d->pre_statistics, d->post_statistics,
+                            d->d_pre_weight, d->d_pre_bias, d->d_post_weight, d->d_post_bias};
+    for (const void* p : streams)
+        if (!aligned(p, sb)) return SNHIP_STATUS_INVALID_VALUE;
+    for (const void* p : blocks)
+        if (!aligned(p, bb)) return SNHIP_STATUS_INVALID_VALUE;
+    for (const void* p : floats)
+        if (!aligned(p, 4)) return SNHIP_STATUS_INVALID_VALUE;
+    if (!aligned(d->gate, gb) || !aligned(d->d_gate, gb)) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->rows == 0 || d->dim == 0) return SNHIP_STATUS_SUCCESS;
+    if (!backward) {
+        if (d->x == nullptr || (d->y != nullptr && d->u == nullptr) || (d->pre_norm != SNHIP_NORM_NONE && d->h == nullptr))
+            return SNHIP_STATUS_INVALID_VALUE;
+        return SNHIP_STATUS_SUCCESS;
+    }
+    if (d->dx == nullptr || (d->y != nullptr && d->dy == nullptr) || (d->du == nullptr && d->dh == nullptr))
+        return SNHIP_STATUS_INVALID_VALUE;
+    if (d->pre_norm == SNHIP_NORM_NONE && d->dh != nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->dh != nullptr && (d->u == nullptr || d->pre_statistics == nullptr)) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->post_norm != SNHIP_NORM_NONE && d->post_statistics == nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->gate == nullptr && d->d_gate != nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    return SNHIP_STATUS_SUCCESS;
+}
+
+struct BlockNormPlan {
+    int slots[5];       // pre weight, pre bias, post weight, post bias, gate: their vector of partial sums, or -1
+    int vectors;
+    bool flush;
+    long long groups, rows_per_group;
+    int groups_per_chunk, chunks_per_group, rows_per_chunk, chunks;
+    size_t bytes;
+};
+// How the rows are cut into chunks, one workgroup each.  kBlockNormChunks of them keep every compute unit busy; each more
+// costs its column sums' way to memory and back.
+constexpr long long kBlockNormChunks = 1024;
+BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
+    BlockNormPlan b{};
+    const bool gate_rows = d->gate != nullptr && d->gate_rows > 0;
+    b.rows_per_group = gate_rows && d->gate_rows < d->rows ? d->gate_rows : d->rows;
+    if (b.rows_per_group < 1) b.rows_per_group = 1;
+    b.groups = (d->rows + b.rows_per_group - 1) / b.rows_per_group;
+    const int at_once = block_norm_backward_groups(d->dim);
+    long long c = (d->rows + kBlockNormChunks - 1) / kBlockNormChunks;
+    if (c < at_once) c = at_once;
+    b.flush = gate_rows && b.rows_per_group <= c;
+    if (b.flush) {
+        b.groups_per_chunk = (int)((c / b.rows_per_group + at_once - 1) / at_once * at_once);
+        b.chunks = (int)((b.groups + b.groups_per_chunk - 1) / b.groups_per_chunk);
+    } else if (d->rows > 0) {
+        b.chunks_per_group = (int)((b.rows_per_group + c - 1) / c);
+        b.rows_per_chunk = (int)((b.rows_per_group + b.chunks_per_group - 1) / b.chunks_per_group);
+        b.chunks = (int)(b.groups * b.chunks_per_group);
+    }
+    const bool wanted[5] = {d->d_pre_weight != nullptr && d->dh != nullptr, d->d_pre_bias != nullptr && d->dh != nullptr,
+                            d->d_post_weight != nullptr && d->post_norm != SNHIP_NORM_NONE,
+                            d->d_post_bias != nullptr && d->post_norm != SNHIP_NORM_NONE, d->d_gate != nullptr && !b.flush};
+    for (int k = 0; k < 5; ++k) b.slots[k] = wanted[k] ? b.vectors++ : -1;
+    b.bytes = up256((size_t)b.vectors * (size_t)b.chunks * (size_t)d->dim * 4);
+    return b;
+}
+
+BlockNormParams block_norm_params(const snhip_block_norm_desc* d) {
+    BlockNormParams p{};
+    p.x = d->x, p.y = d->y, p.gate = d->gate, p.u = d->u, p.h = d->h;
+    p.pre_w = d->pre_weight, p.pre_b = d->pre_bias, p.post_w = d->post_weight, p.post_b = d->post_bias;
+    p.pre_s = d->pre_statistics, p.post_s = d->post_statistics;
+    p.du = d->du, p.dh = d->dh, p.dx = d->dx, p.dy = d->dy, p.d_gate = d->d_gate;
+    p.rows = d->rows, p.dim = d->dim, p.gate_rows = d->gate_rows;
+    p.ld_x = d->ld_x ? d->ld_x : d->dim, p.ld_y = d->ld_y ? d->ld_y : d->dim, p.ld_u = d->ld_u ? d->ld_u : d->dim;
+    p.ld_h = d->ld_h ? d->ld_h : d->dim, p.ld_gate = d->ld_gate ? d->ld_gate : d->dim;
+    p.pre = d->pre_norm, p.post = d->post_norm, p.act = d->gate_activation;
+    p.eps = d->epsilon, p.scale = d->residual_scale, p.inv_dim = 1.0f / (float)(d->dim > 0 ? d->dim : 1);
+    const size_t sb = 4 * type_bytes(d->stream_type), bb = 4 * type_bytes(d->block_type), gb = d->gate_rows == 0 ? 16 : bb;
+    p.whole = p.dim % 4 == 0 && p.ld_x % 4 == 0 && p.ld_y % 4 == 0 && p.ld_u % 4 == 0 && p.ld_h % 4 == 0 && p.ld_gate % 4 == 0 &&
+              aligned(d->x, sb) && aligned(d->u, sb) && aligned(d->du, sb) && aligned(d->dx, sb) && aligned(d->y, bb) &&
+              aligned(d->h, bb) && aligned(d->dh, bb) && aligned(d->dy, bb) && aligned(d->gate, gb) && aligned(d->d_gate, gb) &&
+              aligned(d->pre_weight, 16) && aligned(d->pre_bias, 16) && aligned(d->post_weight, 16) && aligned(d->post_bias, 16);
+    return p;
+}
+
+// 0: both fp32, 1: fp32 stream and bf16 block, 2: both bf16
+int block_norm_types(const snhip_block_norm_desc* d) {
+    return d->stream_type == SNHIP_TYPE_BF16 ? 2 : d->block_type == SNHIP_TYPE_BF16 ? 1 : 0;
+}
+
+// ---- AdamW ------------------------------------------------------------------------------------------------------
+
+struct AdamwPlan {
+    int device = 0, state_bits = 32;
+    long long chunks = 0;
+    void* table = nullptr;  // entries, then the owner of each chunk
+    const int* owner = nullptr;
+};
+
+struct Range {
+    uintptr_t begin, end;
+    bool written;
+};
+// whether a written range meets any other one
+bool overlapping(std::vector<Range>& ranges) {
+    std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+    uintptr_t end = 0, written_end = 0;
+    for (const Range& r : ranges) {
+        if (r.begin < (r.written ? end : written_end)) return true;
+        end = std::max(end, r.end);
+        if (r.written) written_end = std::max(written_end, r.end);
+    }
+    return false;
+}
+
+int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int state_bits, void** plan) {
+    std::vector<AdamwEntry> entries((size_t)count);
+    std::vector<Range> ranges;
+    long long chunks = 0;
+    const size_t sb = state_bits == 32 ? 4 : 1;
+    for (int k = 0; k < count; ++k) {
+        const snhip_adamw_tensor& t = tensors[k];
+        if (t.count < 0 || !is_storage_type(t.gradient_type) || !isfinite(t.weight_decay)) return SNHIP_STATUS_INVALID_VALUE;
+        AdamwEntry& e = entries[(size_t)k];
+        e = AdamwEntry{t.parameter, t.gradient, t.moment1, t.moment2, t.scale1, t.scale2, static_cast<__bf16*>(t.bf16_copy),
+                       t.count, chunks, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16, 0};
+        if (t.count == 0) continue;
+        const size_t gb = type_bytes(t.gradient_type);
+        if (t.parameter == nullptr || t.gradient == nullptr || t.moment1 == nullptr || t.moment2 == nullptr ||
+            (state_bits == 8 && (t.scale1 == nullptr || t.scale2 == nullptr)))
+            return SNHIP_STATUS_INVALID_VALUE;
+        if (!aligned(t.parameter, 4) || !aligned(t.gradient, gb) || !aligned(t.moment1, sb) || !aligned(t.moment2, sb) ||
+            !aligned(t.bf16_copy, 2))
+            return SNHIP_STATUS_INVALID_VALUE;
+        e.whole = aligned(t.parameter, 16) && aligned(t.gradient, 4 * gb) && aligned(t.moment1, 4 * sb) &&
+                  aligned(t.moment2, 4 * sb) && aligned(t.bf16_copy, 8);
+        const size_t n = (size_t)t.count, blocks = (n + kAdamwBlock - 1) / kAdamwBlock;
+        auto add = [&ranges](const void* p, size_t bytes, bool written) {
+            const uintptr_t b = reinterpret_cast<uintptr_t>(p);
+            if (p != nullptr) ranges.push_back(Range{b, b + bytes, written});
+        };
+        add(t.parameter, 4 * n, true);
+        add(t.moment1, sb * n, true);
+        add(t.moment2, sb * n, true);
+        add(t.bf16_copy, 2 * n, true);
+        if (state_bits == 8) add(t.scale1, blocks, true), add(t.scale2, blocks, true);
+        add(t.gradient, gb * n, false);
+        chunks += (t.count + kAdamwChunk - 1) / kAdamwChunk;
+    }
+    if (chunks > 0x7fffffffLL) return SNHIP_STATUS_NOT_SUPPORTED;
+    if (overlapping(ranges)) return SNHIP_STATUS_INVALID_VALUE;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    std::vector<int> owner((size_t)chunks);
+    for (int k = 0; k < count; ++k) {
+        const long long n = (entries[(size_t)k].count + kAdamwChunk - 1) / kAdamwChunk;
+        std::fill_n(owner.begin() + entries[(size_t)k].first_chunk, n, k);
+    }
+    std::unique_ptr<AdamwPlan> a(new AdamwPlan);
+    a->device = h->device, a->state_bits = state_bits, a->chunks = chunks;
+    if (chunks > 0) {
+        const size_t entry_bytes = up256(entries.size() * sizeof(AdamwEntry));
+        hipError_t e = hipMalloc(&a->table, entry_bytes + owner.size() * sizeof(int));
+        if (e == hipSuccess) e = hipMemcpy(a->table, entries.data(), entries.size() * sizeof(AdamwEntry), hipMemcpyHostToDevice);
+        if (e == hipSuccess)
+            e = hipMemcpy(static_cast<char*>(a->table) + entry_bytes, owner.data(), owner.size() * sizeof(int), hipMemcpyHostToDevice);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            if (a->table != nullptr) (void)hipFree(a->table);
+            return hip_to_status(e);
+        }
+        a->owner = reinterpret_cast<const int*>(static_cast<char*>(a->table) + entry_bytes);
+    }
+    *plan = a.release();
+    return SNHIP_STATUS_SUCCESS;
+}
+
+}  // namespace
+
+extern "C" {
+
+int snhip_sizeof_embedding_desc(void) { return (int)sizeof(snhip_embedding_desc); }
+
+int snhip_embedding_forward(void* handle, const snhip_embedding_desc* desc, const void* ids, const void* table, void* y) {
+    const int st = embedding_check_desc(desc);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (desc->tokens == 0 || desc->dim == 0) return SNHIP_STATUS_SUCCESS;
+    if (ids == nullptr || y == nullptr || (table == nullptr && desc->vocabulary > 0)) return SNHIP_STATUS_INVALID_VALUE;
+    if (!aligned(ids, type_bytes(desc->id_type)) || !aligned(table, type_bytes(desc->table_type)) ||
+        !aligned(y, type_bytes(desc->output_type)))
+        return SNHIP_STATUS_INVALID_VALUE;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    const EmbeddingParams p = embedding_params(desc, ids, table, y, false);
+    if (ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2) > 65535) return SNHIP_STATUS_NOT_SUPPORTED;
+    if (desc->id_type == SNHIP_TYPE_F32)
+        embedding_forward_types<float>(p, desc->table_type, desc->output_type, h->stream);
+    else if (desc->id_type == SNHIP_TYPE_I32)
+        embedding_forward_types<int>(p, desc->table_type, desc->output_type, h->stream);
+    else
+        embedding_forward_types<long long>(p, desc->table_type, desc->output_type, h->stream);
+    return hip_to_status(hipGetLastError());
+}
+
+int snhip_embedding_backward_workspace_size(const snhip_embedding_desc* desc, size_t* bytes) {
+    const int st = embedding_check_desc(desc);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    if (bytes == nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    *bytes = embedding_plan(desc).bytes;
+    return SNHIP_STATUS_SUCCESS;
+}
+
+int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, const void* ids, const void* dy,
+                             float* table_gradient, int accumulate, void* workspace, size_t workspace_bytes) {
+    const int st = embedding_check_desc(desc);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (desc->vocabulary == 0 || desc->dim == 0 || (desc->tokens == 0 && accumulate)) return SNHIP_STATUS_SUCCESS;
+    if (table_gradient == nullptr || (desc->tokens > 0 && (ids == nullptr || dy == nullptr))) return SNHIP_STATUS_INVALID_VALUE;
+    if (!aligned(ids, type_bytes(desc->id_type)) || !aligned(dy, type_bytes(desc->output_type)) || !aligned(table_gradient, 4))
+        return SNHIP_STATUS_INVALID_VALUE;
+    const EmbeddingPlan e = embedding_plan(desc);
+    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < e.bytes) return SNHIP_STATUS_INVALID_VALUE;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    EmbeddingParams p = embedding_params(desc, ids, dy, table_gradient, true);
+    const int col_blocks = ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2);
+    if (col_blocks > 65535) return SNHIP_STATUS_NOT_SUPPORTED;
+    p.accumulate = accumulate != 0;
+    p.bins = e.bins, p.chunk = e.chunk;
+    char* ws = static_cast<char*>(workspace);
+    p.order = reinterpret_cast<int*>(ws + e.order), p.sorted = reinterpret_cast<int*>(ws + e.sorted);
+    p.offsets = reinterpret_cast<int*>(ws + e.offsets), p.partial = reinterpret_cast<float*>(ws + e.partial);
+    const int groups = 256 >> p.lanes_log2;
+    p.chunk_blocks = (e.chunks + groups - 1) / groups;
+    const dim3 sort_grid((unsigned)ceil_div(p.vocabulary, p.bins));
+    const size_t lds = (size_t)16 * p.bins * sizeof(int);
+    if (desc->id_type == SNHIP_TYPE_F32)
+        hipLaunchKernelGGL(embedding_sort_kernel<float>, sort_grid, dim3(1024), lds, h->stream, p);
+    else if (desc->id_type == SNHIP_TYPE_I32)
+        hipLaunchKernelGGL(embedding_sort_kernel<int>, sort_grid, dim3(1024), lds, h->stream, p);
+    else
+        hipLaunchKernelGGL(embedding_sort_kernel<long long>, sort_grid, dim3(1024), lds, h->stream, p);
+    const long long clear_blocks = p.accumulate ? 0 : ((long long)p.vocabulary + 8 * groups - 1) / (8 * groups);
+    const dim3 grid((unsigned)(p.chunk_blocks + clear_blocks), (unsigned)col_blocks);
+    if (desc->output_type == SNHIP_TYPE_BF16)
+        hipLaunchKernelGGL(embedding_grad_kernel<__bf16>, grid, dim3(256), 0, h->stream, p);
+    else
+        hipLaunchKernelGGL(embedding_grad_kernel<float>, grid, dim3(256), 0, h->stream, p);
+    if (e.chunks > 1)
+        hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)p.chunk_blocks, (unsigned)col_blocks), dim3(256), 0, h->stream, p);
+    return hip_to_status(hipGetLastError());
+}
+
+int snhip_sizeof_block_norm_desc(void) { return (int)sizeof(snhip_block_norm_desc); }
+
+int snhip_block_norm_forward(void* handle, const snhip_block_norm_desc* desc) {
+    const int st = block_norm_check_desc(desc, false);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (desc->rows == 0 || desc->dim == 0) return SNHIP_STATUS_SUCCESS;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    const BlockNormParams p = block_norm_params(desc);
+    switch (block_norm_types(desc)) {
+        case 0: block_norm_forward_0(p, h->stream); break;
+        case 1: block_norm_forward_1(p, h->stream); break;
+        default: block_norm_forward_2(p, h->stream); break;
+    }
+    return hip_to_status(hipGetLastError());
+}
+
+int snhip_block_norm_backward_workspace_size(const snhip_block_norm_desc* desc, size_t* bytes) {
+    const int st = block_norm_check_desc(desc, true);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    if (bytes == nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    *bytes = block_norm_plan(desc).bytes;
+    return SNHIP_STATUS_SUCCESS;
+}
+
+int snhip_block_norm_backward(void* handle, const snhip_block_norm_desc* desc, void* workspace, size_t workspace_bytes) {
+    const int st = block_norm_check_desc(desc, true);
+    if (st != SNHIP_STATUS_SUCCESS) return st;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (desc->dim == 0) return SNHIP_STATUS_SUCCESS;
+    const BlockNormPlan b = block_norm_plan(desc);
+    if (b.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < b.bytes))
+        return SNHIP_STATUS_INVALID_VALUE;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    BlockNormParams p = block_norm_params(desc);
+    p.partial = static_cast<float*>(workspace);
+    p.gate_groups = b.groups, p.rows_per_group = b.rows_per_group, p.flush = b.flush;
+    p.groups_per_chunk = b.groups_per_chunk, p.chunks_per_group = b.chunks_per_group, p.rows_per_chunk = b.rows_per_chunk;
+    p.chunks = b.chunks;
+    for (int k = 0; k < 5; ++k) p.slot[k] = b.slots[k];
+    if (desc->rows > 0) {
+        const BlockNormKind kind{desc->y == nullptr ? 0 : desc->post_norm == SNHIP_NORM_NONE ? 1 : 2,
+                                 b.slots[1] >= 0 || b.slots[3] >= 0, desc->gate != nullptr};
+        switch (block_norm_types(desc)) {
+            case 0: block_norm_backward_0(p, kind, h->stream); break;
+            case 1: block_norm_backward_1(p, kind, h->stream); break;
+            default: block_norm_backward_2(p, kind, h->stream); break;
+        }
+    }
+    // the sums over the chunks; wanted gradients without a source (no dh, no rows) are zeros
+    ColumnJobs j{};
+    j.partial = p.partial, j.chunks = b.chunks, j.dim = p.dim, j.chunks_per_group = b.chunks_per_group;
+    j.accumulate = desc->accumulate != 0, j.accumulate_gate = desc->accumulate != 0 && desc->gate_rows == 0;
+    j.slot[4] = b.slots[4];
+    j.gate_out = desc->d_gate, j.ld_gate = p.ld_gate;
+    j.gate_bf16 = desc->gate_rows > 0 && desc->block_type == SNHIP_TYPE_BF16;
+    float* outs[4] = {desc->d_pre_weight, desc->d_pre_bias, desc->d_post_weight, desc->d_post_bias};
+    for (int k = 0; k < 4; ++k) {
+        if (outs[k] == nullptr) continue;
+        if (b.slots[k] >= 0)
+            j.out[j.vectors] = outs[k], j.slot[j.vectors] = b.slots[k], ++j.vectors;
+        else if (!j.accumulate)
+            hipLaunchKernelGGL(clear_vector_kernel, dim3((unsigned)ceil_div(p.dim, 256)), dim3(256), 0, h->stream, outs[k], p.dim);
+    }
+    // (a gate vector without rows has one group and no chunks: its gradient is cleared like the others)
+    const long long gate_jobs = b.slots[4] < 0 ? 0 : desc->gate_rows == 0 ? 1 : b.groups;
+    if (j.vectors + gate_jobs > 0)
+        hipLaunchKernelGGL(column_parts_kernel, dim3((unsigned)ceil_div(p.dim, 64), (unsigned)(j.vectors + gate_jobs)), dim3(1024), 0,
+                           h->stream, j);
+    return hip_to_status(hipGetLastError());
+}
+
+int snhip_sizeof_adamw_tensor(void) { return (int)sizeof(snhip_adamw_tensor); }
+int snhip_sizeof_adamw_step_desc(void) { return (int)sizeof(snhip_adamw_step_desc); }
+
+int snhip_adamw_create(void* handle, const snhip_adamw_tensor* tensors, int count, int state_bits, void** plan) {
+    if (plan == nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    *plan = nullptr;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (count < 0 || (count > 0 && tensors == nullptr)) return SNHIP_STATUS_INVALID_VALUE;
+    if (state_bits != 8 && state_bits != 32) return SNHIP_STATUS_NOT_SUPPORTED;
+    try {
+        return adamw_build(h, tensors, count, state_bits, plan);
+    } catch (const std::bad_alloc&) {
+        return SNHIP_STATUS_ALLOC_FAILED;
+    } catch (...) {
+        return SNHIP_STATUS_INTERNAL_ERROR;
+    }
+}
+
+int snhip_adamw_destroy(void* plan) {
+    if (plan == nullptr) return SNHIP_STATUS_SUCCESS;
+    AdamwPlan* a = static_cast<AdamwPlan*>(plan);
+    hipError_t e = hipSuccess;
+    if (a->table != nullptr) {
+        DeviceScope scope(a->device);
+        e = scope.ok() ? hipFree(a->table) : hipErrorNoDevice;
+    }
+    delete a;
+    return hip_to_status(e);
+}
+
+int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
+    if (d == nullptr || d->struct_size != (int)sizeof(snhip_adamw_step_desc)) return SNHIP_STATUS_INVALID_VALUE;
+    Handle* h = static_cast<Handle*>(handle);
+    if (h == nullptr || plan == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    const AdamwPlan* a = static_cast<const AdamwPlan*>(plan);
+    if (a->device != h->device) return SNHIP_STATUS_INVALID_VALUE;
+    if (d->step < 1 || !isfinite(d->learning_rate) || !(d->beta1 >= 0.0 && d->beta1 < 1.0) || !(d->beta2 >= 0.0 && d->beta2 < 1.0) ||
+        !(d->epsilon >= 0.0) || !isfinite(d->epsilon) || !isfinite(d->gradient_scale))
+        return SNHIP_STATUS_INVALID_VALUE;
+    if (a->chunks == 0) return SNHIP_STATUS_SUCCESS;
+    DeviceScope scope(h->device);
+    if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
+    AdamwScalars s{};
+    s.beta1 = (float)d->beta1, s.rest1 = (float)(1.0 - d->beta1);
+    s.beta2 = (float)d->beta2, s.rest2 = (float)(1.0 - d->beta2);
+    s.rate = (float)d->learning_rate;
+    s.step_size = (float)(d->learning_rate / (1.0 - pow(d->beta1, d->step)));
+    s.root_scale = (float)(1.0 / sqrt(1.0 - pow(d->beta2, d->step)));
+    s.eps = (float)d->epsilon, s.grad_scale = d->gradient_scale;
+    s.key0 = (unsigned int)d->seed, s.key1 = (unsigned int)(d->seed >> 32), s.step = (unsigned int)d->step;
+    const AdamwEntry* entries = static_cast<const AdamwEntry*>(a->table);
+    if (a->state_bits == 32)
+        hipLaunchKernelGGL(adamw32_kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
+    else
+        hipLaunchKernelGGL(adamw8_kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
+    return hip_to_status(hipGetLastError());
+}
+
+}  // extern "C"

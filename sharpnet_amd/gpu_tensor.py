@@ -161,10 +161,25 @@ def _prod(xs):
     return p
 
 
-class GPUTensor:
-    """float32 tensor in device memory (row-major, dense), 1 to 4 dimensions."""
+# element types: numpy type of the host copy (bfloat16 travels as float32 values) and bytes in device memory
+ELEMENT_TYPES = {"float32": (np.float32, 4), "bfloat16": (np.float32, 2), "int32": (np.int32, 4), "int64": (np.int64, 8),
+                 "uint8": (np.uint8, 1)}
 
-    def __init__(self, shape, data=None, gpu_wrapper=None, _pointer=None, _owner=None):
+
+def _bf16_bits(x):
+    """float32 values as bfloat16 bits, rounded to nearest even (NaN stays NaN)."""
+    bits = np.ascontiguousarray(x, dtype=np.float32).view(np.uint32)
+    rounded = ((bits + (0x7FFF + ((bits >> 16) & 1))) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), np.uint16(0x7FC0), rounded)
+
+
+class GPUTensor:
+    """Tensor in device memory (row-major, dense), 1 to 4 dimensions; float32 unless said otherwise, as everything the
+    GEMM path computes with is (the counterpart of the reference's GPUTensor<T>)."""
+
+    def __init__(self, shape, data=None, gpu_wrapper=None, _pointer=None, _owner=None, element_type="float32"):
+        self.Type = element_type
+        self.ElementBytes = ELEMENT_TYPES[element_type][1]
         shape = [int(s) for s in shape]
         assert 1 <= len(shape) <= 4 and min(shape) >= 0  # Tensor.cs:29-31
         self.Shape = shape
@@ -179,10 +194,20 @@ class GPUTensor:
         else:
             self.IsOwnerOfMemory = True
             self._owner = None
-            self._nbytes = max(self.Count * 4, 8)  # capacity is at least 8 bytes (GpuTensor.cs:38)
+            self._nbytes = max((self.Count * self.ElementBytes + 3) // 4 * 4, 8)  # capacity is at least 8 bytes (GpuTensor.cs:38)
             self.Pointer = self.Wrapper.allocate(self._nbytes)
             if data is not None:
                 self.InitializeFromHostMemory(data)
+
+    @classmethod
+    def FromPointer(cls, shape, pointer, element_type="float32", gpu_wrapper=None, owner=None):
+        """Non-owning tensor on device memory that something else allocated (GpuTensor.cs:52-63).  The memory must stay
+        valid for as long as the tensor is used; ``owner`` is kept alive with it."""
+        if pointer is None or int(pointer) % ELEMENT_TYPES[element_type][1]:
+            raise ValueError("the address of a %s tensor must be a multiple of %d bytes" % (element_type, ELEMENT_TYPES[element_type][1]))
+        t = cls(shape, None, gpu_wrapper, _pointer=int(pointer), element_type=element_type)
+        t._keeps = owner
+        return t
 
     # -- shape helpers (Tensor.cs:18-21,1521-1526) ---------------------------
     @property
@@ -212,8 +237,8 @@ class GPUTensor:
         """Non-owning view at element offset startIndex (GpuTensor.cs:616)."""
         self.AssertIsNotDisposed()
         assert startIndex >= 0 and startIndex + _prod(sliceShape) <= self.Count
-        return GPUTensor(sliceShape, gpu_wrapper=self.Wrapper, _pointer=self.Pointer + 4 * startIndex,
-                         _owner=self._owner or self)
+        return GPUTensor(sliceShape, gpu_wrapper=self.Wrapper, _pointer=self.Pointer + self.ElementBytes * startIndex,
+                         _owner=self._owner or self, element_type=self.Type)
 
     def RowSlice(self, startRowIndex, nbRows):
         assert len(self.Shape) >= 2 and 0 <= startRowIndex and startRowIndex + nbRows <= self.Shape[0]
@@ -228,7 +253,8 @@ class GPUTensor:
             known = _prod(s for s in newShape if s != -1)
             newShape[newShape.index(-1)] = self.Count // known if known else 0
         assert _prod(newShape) == self.Count
-        return GPUTensor(newShape, gpu_wrapper=self.Wrapper, _pointer=self.Pointer, _owner=self._owner or self)
+        return GPUTensor(newShape, gpu_wrapper=self.Wrapper, _pointer=self.Pointer, _owner=self._owner or self,
+                         element_type=self.Type)
 
     def As2DTensor(self, flattenInputTensorOnLastDimension):
         # Tensor.cs:1645-1654
@@ -241,7 +267,9 @@ class GPUTensor:
     # -- copies ---------------------------------------------------------------
     def InitializeFromHostMemory(self, data):
         self.AssertIsNotDisposed()
-        host = np.ascontiguousarray(np.asarray(data, dtype=np.float32).reshape(-1))
+        host = np.ascontiguousarray(np.asarray(data, dtype=ELEMENT_TYPES[self.Type][0]).reshape(-1))
+        if self.Type == "bfloat16":
+            host = _bf16_bits(host)
         assert host.size == self.Count, "host data has %d elements, tensor has %d" % (host.size, self.Count)
         if host.size:
             check_status(self._lib.snhip_memcpy_htod_async(self.Wrapper.handle, self.Pointer,
@@ -250,12 +278,14 @@ class GPUTensor:
             self.Wrapper.synchronize()
 
     def ContentAsFloatArray(self):
-        """Synchronous D2H copy (GpuTensor.cs:1668)."""
+        """Synchronous D2H copy (GpuTensor.cs:1668); bfloat16 comes back as float32, the integer types as they are."""
         self.AssertIsNotDisposed()
-        host = np.empty(self.Count, dtype=np.float32)
+        host = np.empty(self.Count, dtype=np.uint16 if self.Type == "bfloat16" else ELEMENT_TYPES[self.Type][0])
         if host.size:
             check_status(self._lib.snhip_memcpy_dtoh(self.Wrapper.handle, host.ctypes.data, self.Pointer,
                                                      host.nbytes), "snhip_memcpy_dtoh")
+        if self.Type == "bfloat16":
+            return (host.astype(np.uint32) << 16).view(np.float32)
         return host
 
     def ToNumpy(self):
@@ -264,20 +294,29 @@ class GPUTensor:
     def CopyTo(self, other):
         self.AssertIsNotDisposed()
         other.AssertIsNotDisposed()
-        assert other.Count == self.Count
+        assert other.Count == self.Count and other.Type == self.Type
         check_status(self._lib.snhip_memcpy_dtod_async(self.Wrapper.handle, other.Pointer, self.Pointer,
-                                                       self.Count * 4), "snhip_memcpy_dtod_async")
+                                                       self.Count * self.ElementBytes), "snhip_memcpy_dtod_async")
 
     def ZeroMemory(self):
-        self.SetValue(0.0)
+        if self.Type == "float32":
+            self.SetValue(0.0)
+            return
+        self.AssertIsNotDisposed()
+        nbytes = self._nbytes if self.IsOwnerOfMemory else self.Count * self.ElementBytes
+        if nbytes % 4 or self.Pointer % 4:
+            raise ValueError("only whole 32-bit words can be cleared")
+        check_status(self._lib.snhip_memset32(self.Wrapper.handle, self.Pointer, 0, nbytes // 4), "snhip_memset32")
 
     def SetValue(self, value):
         self.AssertIsNotDisposed()
+        if self.Type != "float32":
+            raise ValueError("SetValue takes a float32 tensor")
         bits = int(np.float32(value).view(np.uint32))
         check_status(self._lib.snhip_memset32(self.Wrapper.handle, self.Pointer, bits, self.Count), "snhip_memset32")
 
     def Clone(self):
-        c = GPUTensor(self.Shape, gpu_wrapper=self.Wrapper)
+        c = GPUTensor(self.Shape, gpu_wrapper=self.Wrapper, element_type=self.Type)
         self.CopyTo(c)
         return c
 

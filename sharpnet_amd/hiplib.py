@@ -133,6 +133,70 @@ class RnnDesc(ctypes.Structure):
             setattr(self, k, float(v) if k == "dropout" else int(v))
 
 
+class EmbeddingDesc(ctypes.Structure):
+    """snhip_embedding_desc of include/sharpnet_hip.h (field for field)."""
+    _fields_ = [("struct_size", _i), ("id_type", _i), ("table_type", _i), ("output_type", _i), ("tokens", _ll),
+                ("vocabulary", _i), ("dim", _i), ("ld_table", _ll), ("ld_output", _ll), ("padding_index", _i),
+                ("scale", _f)]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(EmbeddingDesc)
+        self.padding_index, self.scale = -1, 1.0
+        for k, v in kw.items():
+            if k not in dict(self._fields_):
+                raise TypeError("snhip_embedding_desc has no field %r" % k)
+            setattr(self, k, v)
+
+
+class BlockNormDesc(ctypes.Structure):
+    """snhip_block_norm_desc of include/sharpnet_hip.h (field for field)."""
+    _fields_ = [("struct_size", _i), ("stream_type", _i), ("block_type", _i), ("pre_norm", _i), ("post_norm", _i),
+                ("gate_activation", _i), ("dim", _i), ("gate_rows", _i), ("rows", _ll), ("ld_x", _ll), ("ld_y", _ll),
+                ("ld_u", _ll), ("ld_h", _ll), ("ld_gate", _ll), ("epsilon", _f), ("residual_scale", _f),
+                ("pre_weight", _vp), ("pre_bias", _vp), ("post_weight", _vp), ("post_bias", _vp), ("gate", _vp), ("x", _vp),
+                ("y", _vp), ("u", _vp), ("h", _vp), ("pre_statistics", _vp), ("post_statistics", _vp), ("du", _vp),
+                ("dh", _vp), ("dx", _vp), ("dy", _vp), ("d_gate", _vp), ("d_pre_weight", _vp), ("d_pre_bias", _vp),
+                ("d_post_weight", _vp), ("d_post_bias", _vp), ("accumulate", _i)]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(BlockNormDesc)
+        self.epsilon, self.residual_scale = 1e-5, 1.0
+        for k, v in kw.items():
+            if k not in dict(self._fields_):
+                raise TypeError("snhip_block_norm_desc has no field %r" % k)
+            setattr(self, k, v)
+
+
+class AdamwTensor(ctypes.Structure):
+    """snhip_adamw_tensor of include/sharpnet_hip.h (field for field)."""
+    _fields_ = [("parameter", _vp), ("gradient", _vp), ("moment1", _vp), ("moment2", _vp), ("scale1", _vp), ("scale2", _vp),
+                ("bf16_copy", _vp), ("count", _ll), ("gradient_type", _i), ("weight_decay", _f)]
+
+
+class AdamwStepDesc(ctypes.Structure):
+    """snhip_adamw_step_desc of include/sharpnet_hip.h (field for field)."""
+    _fields_ = [("struct_size", _i), ("step", _i), ("learning_rate", ctypes.c_double), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("epsilon", ctypes.c_double), ("gradient_scale", _f), ("seed", ctypes.c_ulonglong)]
+
+    def __init__(self, **kw):
+        super().__init__()
+        self.struct_size = ctypes.sizeof(AdamwStepDesc)
+        self.step, self.beta1, self.beta2, self.epsilon, self.gradient_scale = 1, 0.9, 0.999, 1e-8, 1.0
+        for k, v in kw.items():
+            if k not in dict(self._fields_):
+                raise TypeError("snhip_adamw_step_desc has no field %r" % k)
+            setattr(self, k, v)
+
+
+# SNHIP_NORM_*
+NORM_NONE, NORM_RMS, NORM_LAYER = range(3)
+
+# SNHIP_TYPE_* by the names of the element types
+TYPE_F32, TYPE_BF16, TYPE_I32, TYPE_I64 = range(4)
+TYPES = {"float32": TYPE_F32, "bfloat16": TYPE_BF16, "int32": TYPE_I32, "int64": TYPE_I64}
+
 # SNHIP_ACT_* and the reference's cudnnActivationMode_t names for them (Prod/GPU/CudnnWrapper.cs:267-281)
 ACT_NONE, ACT_RELU, ACT_LEAKY_RELU, ACT_SIGMOID, ACT_TANH = range(5)
 ACTIVATIONS = {
@@ -196,6 +260,19 @@ SIGNATURES = {
     "snhip_rnn_backward_data": [_vp, ctypes.POINTER(RnnDesc), _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                 _vp, _sz, _vp, _sz],
     "snhip_rnn_backward_weights": [_vp, ctypes.POINTER(RnnDesc), _i, _i, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _sz],
+    "snhip_sizeof_embedding_desc": [],
+    "snhip_embedding_forward": [_vp, ctypes.POINTER(EmbeddingDesc), _vp, _vp, _vp],
+    "snhip_embedding_backward_workspace_size": [ctypes.POINTER(EmbeddingDesc), ctypes.POINTER(_sz)],
+    "snhip_embedding_backward": [_vp, ctypes.POINTER(EmbeddingDesc), _vp, _vp, _vp, _i, _vp, _sz],
+    "snhip_sizeof_block_norm_desc": [],
+    "snhip_block_norm_forward": [_vp, ctypes.POINTER(BlockNormDesc)],
+    "snhip_block_norm_backward_workspace_size": [ctypes.POINTER(BlockNormDesc), ctypes.POINTER(_sz)],
+    "snhip_block_norm_backward": [_vp, ctypes.POINTER(BlockNormDesc), _vp, _sz],
+    "snhip_sizeof_adamw_tensor": [],
+    "snhip_sizeof_adamw_step_desc": [],
+    "snhip_adamw_create": [_vp, ctypes.POINTER(AdamwTensor), _i, _i, _vpp],
+    "snhip_adamw_destroy": [_vp],
+    "snhip_adamw_step": [_vp, _vp, ctypes.POINTER(AdamwStepDesc)],
     "snhip_dense_forward": [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _f],
     "snhip_dense_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _f],
     "snhip_dense_backward_ex": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _f, _vp, _f],

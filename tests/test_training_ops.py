@@ -1,0 +1,331 @@
+"""Word embedding, block norm and AdamW without a GPU: descriptor layouts, refusals (all before any device work), and the
+plain forms that the GPU tests compare with: their gradients against differences, their 8-bit formats against torch's,
+their random words against the published vectors."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from sharpnet_amd import hiplib
+from tests import training_reference as ref
+
+S = hiplib.CublasStatus
+OK_SO_FAR = S.CUBLAS_STATUS_NOT_INITIALIZED   # the arguments were taken; there is no device to go on with
+BAD, UNSUPPORTED = S.CUBLAS_STATUS_INVALID_VALUE, S.CUBLAS_STATUS_NOT_SUPPORTED
+
+
+@pytest.fixture
+def lib():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("checks what happens on a machine without a GPU")
+    return hiplib.load_library()
+
+
+@pytest.fixture
+def handle():
+    """Something that is not NULL; its device cannot be made current here, so no call gets past its argument checks."""
+    return ctypes.addressof(_HANDLE)
+
+
+_HANDLE = ctypes.create_string_buffer(4096)
+A = 0x10000000          # an address like any other (aligned, never touched)
+
+
+def test_descriptor_layouts(lib):
+    assert lib.snhip_sizeof_embedding_desc() == ctypes.sizeof(hiplib.EmbeddingDesc)
+    assert lib.snhip_sizeof_block_norm_desc() == ctypes.sizeof(hiplib.BlockNormDesc)
+    assert lib.snhip_sizeof_adamw_tensor() == ctypes.sizeof(hiplib.AdamwTensor)
+    assert lib.snhip_sizeof_adamw_step_desc() == ctypes.sizeof(hiplib.AdamwStepDesc)
+    for cls in (hiplib.EmbeddingDesc, hiplib.BlockNormDesc, hiplib.AdamwStepDesc):
+        with pytest.raises(TypeError):
+            cls(no_such_field=1)
+
+
+EMBEDDING = dict(id_type=hiplib.TYPE_I32, table_type=hiplib.TYPE_F32, output_type=hiplib.TYPE_BF16, tokens=10, vocabulary=7, dim=6)
+
+
+@pytest.mark.parametrize("change,status", [
+    ({}, OK_SO_FAR), ({"ld_table": 6, "ld_output": 9}, OK_SO_FAR), ({"padding_index": 100}, OK_SO_FAR),
+    ({"struct_size": 4}, BAD), ({"id_type": hiplib.TYPE_BF16}, BAD), ({"id_type": 9}, BAD), ({"table_type": hiplib.TYPE_I32}, BAD),
+    ({"output_type": -1}, BAD), ({"tokens": -1}, BAD), ({"vocabulary": -1}, BAD), ({"dim": -1}, BAD), ({"ld_table": 5}, BAD),
+    ({"ld_output": 5}, BAD), ({"padding_index": -2}, BAD), ({"tokens": 2 ** 31}, UNSUPPORTED)])
+def test_embedding_descriptor_checks(lib, handle, change, status):
+    d = hiplib.EmbeddingDesc(**{**EMBEDDING, **change})
+    n = ctypes.c_size_t()
+    assert lib.snhip_embedding_forward(handle, ctypes.byref(d), A, A, A) == status
+    assert lib.snhip_embedding_backward(handle, ctypes.byref(d), A, A, A, 0, A, 1 << 40) == status
+    assert lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(n)) == (0 if status == OK_SO_FAR else status)
+
+
+def test_embedding_pointer_checks(lib, handle):
+    d = hiplib.EmbeddingDesc(**EMBEDDING)
+    r, n = ctypes.byref(d), ctypes.c_size_t()
+    assert lib.snhip_embedding_forward(None, r, A, A, A) == S.CUBLAS_STATUS_NOT_INITIALIZED
+    assert lib.snhip_embedding_forward(handle, None, A, A, A) == BAD
+    for args in ((None, A, A), (A, None, A), (A, A, None), (A + 2, A, A), (A, A + 2, A), (A, A, A + 1)):
+        assert lib.snhip_embedding_forward(handle, r, *args) == BAD, args
+    assert lib.snhip_embedding_backward_workspace_size(r, None) == BAD
+    assert lib.snhip_embedding_backward_workspace_size(r, ctypes.byref(n)) == 0
+    full = n.value
+    for args in ((None, A, A, 0, A, full), (A, None, A, 0, A, full), (A, A, None, 0, A, full), (A, A, A, 0, None, full),
+                 (A, A, A, 0, A + 4, full), (A, A, A, 0, A, full - 1), (A, A + 1, A, 0, A, full), (A, A, A + 2, 0, A, full)):
+        assert lib.snhip_embedding_backward(handle, r, *args) == BAD, args
+    assert lib.snhip_embedding_backward(handle, r, A, A, A, 0, A, full) == OK_SO_FAR
+    d.tokens = 0      # nothing to look up, nothing to add
+    assert lib.snhip_embedding_forward(handle, r, None, None, None) == 0
+    assert lib.snhip_embedding_backward(handle, r, None, None, None, 1, None, 0) == 0
+    assert lib.snhip_embedding_backward(handle, r, None, None, None, 0, A, full) == BAD   # the gradient has to be cleared
+    d.id_type, d.tokens = hiplib.TYPE_I64, 4
+    assert lib.snhip_embedding_forward(handle, r, A + 4, A, A) == BAD
+
+
+NORM = dict(stream_type=hiplib.TYPE_F32, block_type=hiplib.TYPE_BF16, pre_norm=hiplib.NORM_LAYER, post_norm=hiplib.NORM_RMS,
+            gate_activation=hiplib.ACT_SIGMOID, dim=12, gate_rows=3, rows=10, x=A, y=A, u=A, h=A, gate=A, pre_statistics=A,
+            post_statistics=A, du=A, dh=A, dx=A, dy=A)
+
+
+@pytest.mark.parametrize("change,forward,backward", [
+    ({}, OK_SO_FAR, OK_SO_FAR), ({"gate_rows": 0}, OK_SO_FAR, OK_SO_FAR), ({"dim": 8192}, OK_SO_FAR, OK_SO_FAR),
+    ({"struct_size": 8}, BAD, BAD), ({"stream_type": hiplib.TYPE_I32}, BAD, BAD), ({"block_type": 7}, BAD, BAD),
+    ({"pre_norm": 3}, BAD, BAD), ({"post_norm": -1}, BAD, BAD), ({"gate_activation": hiplib.ACT_RELU}, UNSUPPORTED, UNSUPPORTED),
+    ({"rows": -1}, BAD, BAD), ({"dim": -4}, BAD, BAD), ({"gate_rows": -1}, BAD, BAD), ({"ld_x": 11}, BAD, BAD), ({"ld_gate": 1}, BAD, BAD),
+    ({"epsilon": -1.0}, BAD, BAD), ({"epsilon": float("nan")}, BAD, BAD), ({"epsilon": float("inf")}, BAD, BAD),
+    ({"dim": 8193}, UNSUPPORTED, UNSUPPORTED), ({"rows": 2 ** 31}, UNSUPPORTED, UNSUPPORTED),
+    ({"stream_type": hiplib.TYPE_BF16, "block_type": hiplib.TYPE_F32}, UNSUPPORTED, UNSUPPORTED),
+    ({"y": None}, BAD, BAD), ({"y": None, "gate": None}, BAD, BAD), ({"y": None, "gate": None, "post_norm": 0}, OK_SO_FAR, OK_SO_FAR),
+    ({"y": None, "gate": None, "post_norm": 0, "pre_norm": 0}, BAD, BAD),
+    ({"x": None}, BAD, OK_SO_FAR), ({"u": None}, BAD, BAD), ({"h": None}, BAD, OK_SO_FAR), ({"dx": None}, OK_SO_FAR, BAD),
+    ({"dy": None}, OK_SO_FAR, BAD), ({"dh": None}, OK_SO_FAR, OK_SO_FAR), ({"du": None}, OK_SO_FAR, OK_SO_FAR),
+    ({"du": None, "dh": None}, OK_SO_FAR, BAD), ({"pre_norm": 0}, OK_SO_FAR, BAD), ({"pre_norm": 0, "dh": None}, OK_SO_FAR, OK_SO_FAR),
+    ({"pre_statistics": None}, OK_SO_FAR, BAD), ({"post_statistics": None}, OK_SO_FAR, BAD),
+    ({"gate": None, "d_gate": A}, OK_SO_FAR, BAD), ({"x": A + 2}, BAD, BAD), ({"y": A + 1}, BAD, BAD), ({"gate": A + 1}, BAD, BAD),
+    ({"gate": A + 2, "gate_rows": 0}, BAD, BAD), ({"pre_weight": A + 2}, BAD, BAD), ({"d_post_bias": A + 1}, BAD, BAD)])
+def test_block_norm_checks(lib, handle, change, forward, backward):
+    d = hiplib.BlockNormDesc(**{**NORM, **change})
+    assert lib.snhip_block_norm_forward(handle, ctypes.byref(d)) == forward
+    n = ctypes.c_size_t()
+    assert lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(n)) == (0 if backward == OK_SO_FAR else backward)
+    assert lib.snhip_block_norm_backward(handle, ctypes.byref(d), A, 1 << 40) == backward
+
+
+def test_block_norm_workspace_and_handle_checks(lib, handle):
+    d = hiplib.BlockNormDesc(**{**NORM, "d_pre_weight": A, "d_gate": A, "gate_rows": 0})
+    r, n = ctypes.byref(d), ctypes.c_size_t()
+    assert lib.snhip_block_norm_forward(None, r) == lib.snhip_block_norm_backward(None, r, A, 1 << 40) == S.CUBLAS_STATUS_NOT_INITIALIZED
+    assert lib.snhip_block_norm_forward(handle, None) == lib.snhip_block_norm_backward(handle, None, A, 1 << 40) == BAD
+    assert lib.snhip_block_norm_backward_workspace_size(r, None) == BAD
+    assert lib.snhip_block_norm_backward_workspace_size(r, ctypes.byref(n)) == 0 and n.value > 0
+    for ws, size in ((None, n.value), (A + 8, n.value), (A, n.value - 1)):
+        assert lib.snhip_block_norm_backward(handle, r, ws, size) == BAD
+    assert lib.snhip_block_norm_backward(handle, r, A, n.value) == OK_SO_FAR
+    d.d_pre_weight = d.d_gate = None      # nothing to sum up: no scratch memory
+    assert lib.snhip_block_norm_backward_workspace_size(r, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.snhip_block_norm_backward(handle, r, None, 0) == OK_SO_FAR
+    d.rows = 0
+    assert lib.snhip_block_norm_forward(handle, r) == 0
+
+
+def adamw_tensors(*changes):
+    made = (hiplib.AdamwTensor * len(changes))()
+    for k, (t, change) in enumerate(zip(made, changes)):
+        base = A + (k << 20)
+        fields = dict(parameter=base, gradient=base + 0x10000, moment1=base + 0x20000, moment2=base + 0x30000, scale1=base + 0x40000,
+                      scale2=base + 0x50000, bf16_copy=base + 0x60000, count=1000, gradient_type=hiplib.TYPE_F32, weight_decay=0.1)
+        for f, v in {**fields, **change}.items():
+            setattr(t, f, v)
+    return made
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("change,status", [
+    ({}, OK_SO_FAR), ({"bf16_copy": None}, OK_SO_FAR), ({"count": 0, "parameter": None}, 0), ({"count": -1}, BAD),
+    ({"parameter": None}, BAD), ({"gradient": None}, BAD), ({"moment1": None}, BAD), ({"moment2": None}, BAD),
+    ({"parameter": A + 2}, BAD), ({"gradient": A + 0x10001}, BAD), ({"bf16_copy": A + 0x60001}, BAD), ({"gradient_type": hiplib.TYPE_I32}, BAD),
+    ({"weight_decay": float("nan")}, BAD), ({"moment2": A + 0x20000}, BAD), ({"bf16_copy": A + 2000}, BAD), ({"gradient": A}, BAD),
+    ({"gradient": A + 3996}, BAD), ({"gradient": A + 4000}, OK_SO_FAR)])
+def test_adamw_plan_checks(lib, handle, bits, change, status):
+    plan = ctypes.c_void_p(1)
+    assert lib.snhip_adamw_create(handle, adamw_tensors(change), 1, bits, ctypes.byref(plan)) == \
+        (status if status != 0 else OK_SO_FAR)
+    assert not plan.value
+
+
+def test_adamw_scales_several_tensors_and_arguments(lib, handle):
+    plan = ctypes.c_void_p()
+    create = lambda t, n, bits: lib.snhip_adamw_create(handle, t, n, bits, ctypes.byref(plan))  # noqa: E731
+    assert create(adamw_tensors({"scale1": None}), 1, 8) == BAD and create(adamw_tensors({"scale1": None}), 1, 32) == OK_SO_FAR
+    assert create(adamw_tensors({"scale2": A + 0x40003}), 1, 8) == BAD      # four blocks: bytes 0 to 3 are scale1's
+    assert create(adamw_tensors({"scale2": A + 0x40004}), 1, 8) == OK_SO_FAR
+    assert create(adamw_tensors({}, {}), 2, 8) == OK_SO_FAR
+    assert create(adamw_tensors({}, {"parameter": A}), 2, 32) == BAD        # the same tensor twice
+    assert create(adamw_tensors({}, {"parameter": A + 4000}), 2, 32) == OK_SO_FAR
+    assert create(adamw_tensors({}, {"gradient": A + 0x10000}), 2, 32) == OK_SO_FAR   # gradients are only read
+    assert create(adamw_tensors({}), 1, 16) == UNSUPPORTED
+    assert create(None, 1, 32) == BAD and create(adamw_tensors({}), -1, 32) == BAD
+    assert lib.snhip_adamw_create(handle, None, 0, 32, None) == BAD
+    assert lib.snhip_adamw_create(None, None, 0, 32, ctypes.byref(plan)) == S.CUBLAS_STATUS_NOT_INITIALIZED
+    assert lib.snhip_adamw_destroy(None) == 0
+
+
+@pytest.mark.parametrize("change", [{"struct_size": 8}, {"step": 0}, {"step": -3}, {"learning_rate": float("nan")}, {"beta1": 1.0}, {"beta1": -0.1},
+                                    {"beta2": 1.0}, {"beta2": float("nan")}, {"epsilon": -1e-8}, {"epsilon": float("inf")},
+                                    {"gradient_scale": float("inf")}])
+def test_adamw_step_checks(lib, handle, change):
+    plan = ctypes.create_string_buffer(256)      # a plan of no chunks on device 0
+    d = hiplib.AdamwStepDesc(learning_rate=1e-3)
+    assert lib.snhip_adamw_step(handle, ctypes.addressof(plan), ctypes.byref(d)) == 0
+    assert lib.snhip_adamw_step(handle, None, ctypes.byref(d)) == lib.snhip_adamw_step(None, ctypes.addressof(plan), ctypes.byref(d)) == \
+        S.CUBLAS_STATUS_NOT_INITIALIZED
+    for k, v in change.items():
+        setattr(d, k, v)
+    assert lib.snhip_adamw_step(handle, ctypes.addressof(plan), ctypes.byref(d)) == BAD
+    assert lib.snhip_adamw_step(handle, ctypes.addressof(plan), None) == BAD
+
+
+class Stub:
+    """Shape and type of a tensor, for the host side's checks."""
+
+    def __init__(self, shape, type_="float32"):
+        self.Shape, self.Type, self.Pointer = list(shape), type_, A
+        self.Count = int(np.prod(shape))
+        self.lib = self._lib = self.Wrapper = self
+
+    def AssertIsNotDisposed(self):
+        pass
+
+
+def test_host_sides_refuse_what_does_not_fit():
+    from sharpnet_amd import GPUTensor, embedding, normalization, optimizer
+    e = embedding.WordEmbedding(7, 6)
+    ids, y, table = Stub((10,), "int32"), Stub((10, 6)), Stub((7, 6))
+    for args in ((Stub((9, 6)), ids, table), (Stub((10, 5)), ids, table), (y, ids, Stub((6, 6))), (y, Stub((10,), "uint8"), table),
+                 (Stub((10, 6), "int32"), ids, table), (y, ids, Stub((7, 6), "int64"))):
+        with pytest.raises(ValueError):
+            e.ForwardPropagation(*args)
+    with pytest.raises(ValueError):
+        e.BackwardPropagation(Stub((7, 6), "bfloat16"), ids, y)
+    with pytest.raises(ValueError):
+        embedding.WordEmbedding(-1, 6)
+    with pytest.raises(ValueError):
+        normalization.BlockNorm(8, "batch")
+    with pytest.raises(hiplib.SharpNetHipError):
+        normalization.BlockNorm(8, gateActivation="CUDNN_ACTIVATION_RELU")
+    n = normalization.BlockNorm(8, "layer", "rms")
+    x, h, y = Stub((5, 8)), Stub((5, 8)), Stub((5, 8))
+    for kw in (dict(y=Stub((4, 8))), dict(y=Stub((5, 8), "bfloat16")), dict(u=Stub((5, 8), "bfloat16")), dict(preWeight=Stub((7,))),
+               dict(preWeight=Stub((8,), "bfloat16")), dict(preStatistics=Stub((5,))), dict(gate=Stub((8,)), gateRows=2),
+               dict(gate=Stub((3, 8)), gateRows=0), dict(gate=Stub((8,)), gateRows=-1)):
+        with pytest.raises(ValueError):
+            n.ForwardPropagation(x, h, **{**dict(y=y, u=Stub((5, 8))), **kw})
+    with pytest.raises(ValueError):
+        n.BackwardPropagation(x, x, h, y=y, dy=y, gate=Stub((8,)), dGate=Stub((8, 1)))
+    p, g = Stub((3, 4)), Stub((3, 4))
+    good = [[Stub((3, 4)), Stub((3, 4))]]
+    for kw in (dict(parameters=[Stub((3, 4), "bfloat16")]), dict(gradients=[Stub((3, 5))]), dict(gradients=[]), dict(copies=[Stub((3, 4))]),
+               dict(stateBits=16), dict(stateBits=8), dict(states=[[Stub((3, 4))]]), dict(weightDecay=[0.1, 0.2])):
+        with pytest.raises(ValueError):
+            optimizer.AdamW(**{**dict(parameters=[p], gradients=[g], states=good), **kw})
+    with pytest.raises(ValueError):
+        GPUTensor.FromPointer([4], A + 2, "float32", gpu_wrapper=p)
+    t = GPUTensor.FromPointer([4], A + 2, "bfloat16", gpu_wrapper=p, owner=ids)
+    assert t.ElementBytes == 2 and t.Slice(1, [2]).Pointer == A + 4 and t.Slice(1, [2]).Type == "bfloat16" and not t.IsOwnerOfMemory
+
+
+# ---- the plain forms ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("pre,post,gate_rows,activation", [
+    ("layer", "layer", 0, "sigmoid"), ("rms", "rms", 2, "tanh"), ("layer", None, 1, None), (None, "layer", 3, "sigmoid"),
+    ("rms", "layer", None, None), ("layer", None, None, None)])
+def test_plain_block_norm_gradients_against_differences(pre, post, gate_rows, activation):
+    """Central differences in 64 bits with steps of 1e-5: off by the third derivative times 1e-10 and by rounding of
+    1e-16 / 1e-5, both far below 1e-7."""
+    rng = np.random.default_rng(0)
+    rows, dim, eps, scale = 5, 7, 1e-3, np.float32(0.7)
+    x = rng.normal(0, 1, (rows, dim))
+    y = rng.normal(0, 1, (rows, dim)) if post or gate_rows is not None else None
+    gate = None if gate_rows is None else rng.normal(0, 1, dim if gate_rows == 0 else (-(-rows // gate_rows), dim))
+    weights = {}
+    for which, kind in (("pre", pre), ("post", post)):
+        if kind:
+            weights[which + "_weight"], weights[which + "_bias"] = rng.normal(1, 0.3, dim), rng.normal(0, 0.3, dim)
+    gu, gh = rng.normal(0, 1, (rows, dim)), rng.normal(0, 1, (rows, dim))
+
+    def outputs():
+        return ref.block_norm_forward(x, y, gate, gate_rows or 0, pre, post, weights, scale, eps, activation, "float32", "float32")
+
+    def loss():
+        o = outputs()
+        return ((o["u"][0] * gu).sum() if "u" in o else 0.0) + ((o["h"][0] * gh).sum() if pre else 0.0)
+
+    u = outputs()["u"][0] if y is not None else x
+    stats = {}
+    if pre:
+        stats["pre"] = np.concatenate(ref.statistics(u, pre, eps), 1)
+    if post:
+        stats["post"] = np.concatenate(ref.statistics(y, post, eps), 1)
+    got = ref.block_norm_backward(u, gh if pre else None, gu if y is not None else None, y, gate, gate_rows or 0, pre, post, weights, stats,
+                                  scale, activation, "float32", "float32")
+    inputs = {"dx": x, "dy": y, "d_gate": gate, **{"d_" + k: v for k, v in weights.items()}}
+    for name, a in inputs.items():
+        if a is None:
+            continue
+        flat, want = a.reshape(-1), got[name][0].reshape(-1)
+        for i in range(flat.size):
+            old = flat[i]
+            flat[i] = old + 1e-5
+            up = loss()
+            flat[i] = old - 1e-5
+            down = loss()
+            flat[i] = old
+            assert abs((up - down) / 2e-5 - want[i]) < 1e-7 * (1 + abs(want[i])), (name, i)
+
+
+def test_plain_embedding_gradient_is_the_transpose_of_the_lookup():
+    rng = np.random.default_rng(1)
+    ids = np.array([3, -1, 0, 3, 9, 4, 3], np.int64)
+    W, dy = rng.normal(0, 1, (5, 4)), rng.normal(0, 1, (7, 4))
+    g, _ = ref.embedding_backward(ids, dy, 5, 0.5)
+    assert abs((ref.embedding_forward(ids, W, 0.5) * dy).sum() - (g * W).sum()) < 1e-12
+    assert np.array_equal(ref.valid_ids(np.array([0.9, -0.9, 4.99, 5.0, np.nan, -1.0, np.inf], np.float32), 5), [0, 0, 4, -1, -1, -1, -1])
+
+
+def test_plain_8_bit_formats_are_torchs():
+    import torch
+    codes = torch.arange(256, dtype=torch.int32).to(torch.uint8)
+    for table, type_ in ((ref.E4M3, torch.float8_e4m3fn), (ref.E5M2, torch.float8_e5m2)):
+        want = codes.view(type_).float().numpy()
+        assert np.array_equal(table, want, equal_nan=True)
+
+
+def test_plain_random_words_are_the_published_ones():
+    """The known answers that the generator's authors publish for philox4x32-10."""
+    f = 0xFFFFFFFF
+    for counter, key, want in (((0, 0, 0, 0), (0, 0), (0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8)),
+                               ((f, f, f, f), (f, f), (0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD)),
+                               ((0x243F6A88, 0x85A308D3, 0x13198A2E, 0x03707344), (0xA4093822, 0x299F31D0),
+                                (0xD16CFE09, 0x94FDCCEB, 0x5001E420, 0x24126EA1))):
+        assert tuple(int(x) for x in ref.philox(counter, key)) == want
+
+
+def test_plain_8_bit_storage_rounds_to_a_neighbour_and_keeps_the_mean():
+    rng = np.random.default_rng(2)
+    x = (rng.normal(0, 1, 2048) * np.exp(rng.normal(0, 4, 2048))).astype(np.float32)
+    x[:100] = 0
+    for store, table, v in ((ref.store_m, ref.E4M3, x), (ref.store_v, ref.E5M2, np.abs(x))):
+        draws = []
+        for k in range(64):
+            code, scale = store(v, ref.random_words(v.size, 0, k, 7))
+            draws.append(ref.load8(code, scale, table).astype(np.float64))
+        draws = np.array(draws)
+        unit = np.repeat(ref.power(scale.astype(np.int64) - 127), 256).astype(np.float64)
+        positive = np.unique(np.abs(table[np.isfinite(table)])).astype(np.float64)
+        a = np.abs(v.astype(np.float64)) / unit
+        below = positive[np.searchsorted(positive, a, side="right") - 1]
+        above = positive[np.minimum(np.searchsorted(positive, a), positive.size - 1)]
+        got = np.abs(draws) / unit
+        lifted = (got == positive[1]) & (a > 0) & (a < positive[1])          # v: never zero
+        assert np.all((got == below) | (got == above) | lifted)
+        assert np.all(draws[:, v == 0] == 0)
+        # the mean of 64 draws: a standard deviation of half a step / 8 at most; six of them
+        normal = a >= positive[1]
+        assert np.all(np.abs(got.mean(0) - a)[normal] <= (6 / 16 * (above - below) + 2.0 ** -16 * (above - below))[normal])
