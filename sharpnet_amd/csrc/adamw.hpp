@@ -46,13 +46,22 @@ __device__ __forceinline__ float new_parameter(float p, float m, float v, float 
     return p * keep - s.step_size * (m / (sqrtf(v) * s.root_scale + s.eps));
 }
 
-__device__ __forceinline__ f32x4 gradient4(const AdamwEntry& t, long long i, int left, float scale) {
-    f32x4 g;
+// Four elements of the gradient as they lie in memory, and what they are worth: the conversion is kept away from the load,
+// so that the other loads of the same elements do not wait for it.
+struct RawGradient {
+    f32x4 f;
+    bf16x4 b;
+};
+__device__ __forceinline__ RawGradient load_gradient(const AdamwEntry& t, long long i, int left, bool whole) {
+    RawGradient r;
     if (t.g_bf16)
-        g = load4(static_cast<const __bf16*>(t.g) + i, 0, left, t.whole && left >= 4);
+        r.b = load4_raw(static_cast<const __bf16*>(t.g) + i, 0, left, whole);
     else
-        g = load4(static_cast<const float*>(t.g) + i, 0, left, t.whole && left >= 4);
-    return g * scale;
+        r.f = load4_raw(static_cast<const float*>(t.g) + i, 0, left, whole);
+    return r;
+}
+__device__ __forceinline__ f32x4 gradient_of(const AdamwEntry& t, const RawGradient& r, float scale) {
+    return (t.g_bf16 ? widen(r.b) : r.f) * scale;
 }
 
 __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
@@ -67,8 +76,9 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restri
         if (i >= t.count) break;
         const int left = t.count - i < 4 ? (int)(t.count - i) : 4;
         const bool whole = t.whole && left == 4;
-        const f32x4 g = gradient4(t, i, left, s.grad_scale);
+        const RawGradient raw = load_gradient(t, i, left, whole);
         f32x4 pp = load4(t.p + i, 0, left, whole), mm = load4(m + i, 0, left, whole), vv = load4(v + i, 0, left, whole);
+        const f32x4 g = gradient_of(t, raw, s.grad_scale);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             mm[j] = moment1(mm[j], g[j], s);
@@ -127,9 +137,10 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restric
         const int left = t.count - i < 4 ? (int)(t.count - i) : 4;  // <= 0: behind the tensor's end
         const bool whole = t.whole && left == 4;
         unsigned int mbits = 0, vbits = 0;
-        f32x4 g = {0.0f, 0.0f, 0.0f, 0.0f}, pp = g, mm, vv;
+        RawGradient raw = {};
+        f32x4 pp = {0.0f, 0.0f, 0.0f, 0.0f}, mm, vv;
         if (left > 0) {
-            g = gradient4(t, i, left, s.grad_scale);
+            raw = load_gradient(t, i, left, whole);
             pp = load4(t.p + i, 0, left, whole);
             if (whole) {
                 mbits = *reinterpret_cast<const unsigned int*>(m8 + i);
@@ -141,6 +152,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restric
                 }
             }
         }
+        const f32x4 g = gradient_of(t, raw, s.grad_scale);
         const long long block = b0 / kAdamwBlock;
         const float m_unit = power_of_two((int)t.m_scale[block] - 127), v_unit = power_of_two((int)t.v_scale[block] - 127);
         mm[0] = __builtin_amdgcn_cvt_f32_fp8(mbits, 0), mm[1] = __builtin_amdgcn_cvt_f32_fp8(mbits, 1);

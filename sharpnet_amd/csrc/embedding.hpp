@@ -40,12 +40,16 @@ struct EmbeddingParams {
     int whole;        // rows of `in` and `out` can be accessed four elements at a time
     int lanes_log2;   // threads per row of a workgroup of 256
     int accumulate;   // gradient: dW += instead of dW =
-    int bins;         // ids per workgroup of the sort
+    int sort_blocks, sort_log2;  // buckets of the sort, a power of two
+    int fine_log2;               // ... over 256 of them: 2^fine_log2 times 256
+    int bins, bins_log2;         // ids of each (at most 512), and the bits that number them
     int chunk;        // sorted tokens per group of threads of the gradient
     long long chunk_blocks;  // workgroups that add up chunks; those behind them clear rows without tokens
-    int* order;       // [tokens]: token numbers, sorted by id
-    int* sorted;      // [tokens]: their ids
-    int* offsets;     // [vocabulary + 1]: where each id's run starts in `order`
+    int* order;       // [tokens]: token numbers, sorted by key (see embedding_sort_kernel)
+    int* sorted;      // [tokens]: their ids' keys
+    int* offsets;     // [sort_blocks * bins + 1]: where each key's run starts in `order`
+    int pieces;       // of embedding_bucket_kernel
+    int *piece_id, *piece_token, *piece_start;
     float* partial;   // [chunks][2][dim]: sums of the runs that came into a chunk / went on behind it
 };
 
@@ -61,63 +65,62 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         id[r] = t0 + r < p.tokens ? token_id(static_cast<const ID*>(p.ids), t0 + r, p.vocabulary) : -1;
-    f32x4 v[ROWS];
+    typename Raw4<TIN>::type v[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        v[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (id[r] >= 0) v[r] = load4(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in, c, p.dim, p.whole);
+        v[r] = typename Raw4<TIN>::type{};
+        if (id[r] >= 0) v[r] = load4_raw(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in, c, p.dim, p.whole);
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         if (t0 + r < p.tokens)
-            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out, c, p.dim, p.whole, v[r] * p.scale);
+            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out, c, p.dim, p.whole, widen(v[r]) * p.scale);
 }
 
-// Sorts the tokens by id in one launch: a workgroup owns `bins` consecutive ids and reads all of them.  Its 16 wavefronts
-// take a contiguous part of the tokens each and count their ids (LDS, [wavefront][id]) and the tokens with smaller ids
-// (which is where the workgroup's part of `order` starts); after a scan over (id, wavefront) every wavefront walks its
-// part again and puts each token behind the earlier ones of its id.  The order within an id is thus fixed: by wavefront,
-// then by position.  Reading the ids in every workgroup costs 256 x tokens x 4..8 bytes from L2 and saves the launches of
-// a radix sort.
-template <typename ID>
-__global__ void __launch_bounds__(1024) embedding_sort_kernel(const EmbeddingParams p) {
-    extern __shared__ int count[];  // [16][bins], then the cursors
-    __shared__ int below[16], wave_total[16];
-    constexpr int U = 8;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int lo = blockIdx.x * p.bins;
-    const int bins = p.vocabulary - lo < p.bins ? p.vocabulary - lo : p.bins;
-    for (int i = tid; i < 16 * bins; i += 1024) count[i] = 0;
-    __syncthreads();
-    const long long per = ((p.tokens + 1023) / 1024) * 64;
-    const long long begin = w * per < p.tokens ? w * per : p.tokens;
-    const long long end = begin + per < p.tokens ? begin + per : p.tokens;
-    const ID* ids = static_cast<const ID*>(p.ids);
-    int smaller = 0;
-    for (long long t = begin; t < end; t += 64 * U) {
-        int id[U];
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const long long tt = t + 64 * j + lane;
-            id[j] = tt < end ? token_id(ids, tt, p.vocabulary) : -1;
-            if (id[j] == p.padding) id[j] = -1;
-        }
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int b = id[j] - lo;
-            if (b >= 0 && b < bins) atomicAdd(&count[w * bins + b], 1);
-            smaller += id[j] >= 0 && b < 0;
-        }
+// The sort.  Ids are dealt out to the workgroups of embedding_sort_kernel in turn (words come by frequency in most
+// vocabularies: neighbours would put half of all tokens into one workgroup): id i is number i / B of bucket i % B, its key
+// rank * bins + i / B with the
+// buckets ranked by i % 256 first.  The workgroup of a bucket finds its tokens in the order of their positions, a contiguous part to
+// each of its 16 wavefronts, and counts them by wavefront and id in LDS; after a scan over (id, wavefront) every wavefront
+// puts its tokens behind the earlier ones of their ids.  The order within an id is that of the positions.
+// Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (6.6 us for 4000 tokens).
+// With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup reads its own alone
+// (65536 tokens: 34 us the first way, MEASURED the second).
+constexpr int kSortDirect = 8192; // tokens up to which every workgroup reads all ids
+constexpr int kPiece = 1024;      // tokens that a workgroup of embedding_bucket_kernel sorts
+constexpr int kBuckets = 256;     // ... by bucket (bucket modulo 256 if there are more)
+
+// The lanes of `in` whose value (bits wide) is this lane's.
+__device__ __forceinline__ unsigned long long same_value(bool in, int value, int bits) {
+    unsigned long long same = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long ones = __ballot((value >> b) & 1);
+        same &= (value >> b) & 1 ? ones : ~ones;
     }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) smaller += __shfl_xor(smaller, off, 64);
-    if (lane == 0) below[w] = smaller;
-    __syncthreads();
-    // ids' totals, scanned over the ids (at most 512: the first eight wavefronts)
-    int mine = 0;
-    if (tid < bins)
-        for (int k = 0; k < 16; ++k) mine += count[k * bins + tid];
-    int upto = mine;
+    return same;
+}
+
+// A place in the counters' order for every lane of `in`: behind the earlier tokens of the same value, by lane.
+__device__ __forceinline__ int take_place(bool in, int value, int bits, int* cursors) {
+    const int lane = threadIdx.x & 63;
+    const unsigned long long before = (1ULL << lane) - 1, same = same_value(in, value, bits);
+    int at = 0;
+    if (in) {
+        volatile int* cursor = &cursors[value];
+        at = *cursor + __popcll(same & before);
+        if ((same & ~before) == (1ULL << lane)) *cursor = at + 1;  // the last of its value
+    }
+    return at;
+}
+
+// count[waves][values] becomes the places where each wavefront's tokens of each value start, from `first` on; start: where
+// the value of this thread (threadIdx.x < values) starts, total: how many there are of it.  values <= 512, one per thread.
+__device__ __forceinline__ void scan_counts(int* count, int waves, int values, int first, int* wave_total, int& start, int& total) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    total = 0;
+    if (tid < values)
+        for (int k = 0; k < waves; ++k) total += count[k * values + tid];
+    int upto = total;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
         const int o = __shfl_up(upto, off, 64);
@@ -125,52 +128,179 @@ __global__ void __launch_bounds__(1024) embedding_sort_kernel(const EmbeddingPar
     }
     if (lane == 63) wave_total[w] = upto;
     __syncthreads();
-    int start = 0;
-    for (int k = 0; k < 16; ++k) start += below[k];
+    start = first + upto - total;
     for (int k = 0; k < w; ++k) start += wave_total[k];
-    start += upto - mine;
-    if (tid < bins) {
-        p.offsets[lo + tid] = start;
-        if (lo + tid == p.vocabulary - 1) p.offsets[p.vocabulary] = start + mine;
-        for (int k = 0; k < 16; ++k) {
-            const int n = count[k * bins + tid];
-            count[k * bins + tid] = start;
-            start += n;
+    if (tid < values) {
+        int at = start;
+        for (int k = 0; k < waves; ++k) {
+            const int n = count[k * values + tid];
+            count[k * values + tid] = at;
+            at += n;
         }
     }
     __syncthreads();
-    for (long long t = begin; t < end; t += 64 * U) {
-        int id[U];
+}
+
+// Pieces of kPiece tokens, sorted by bucket modulo 256: the piece's ids and positions at [piece * kPiece ...) of piece_id /
+// piece_token, where each bucket starts in the piece at piece_start[bucket][piece] (and the piece's end as bucket 256).
+template <typename ID>
+__global__ void __launch_bounds__(256) embedding_bucket_kernel(const EmbeddingParams p) {
+    __shared__ int count[4 * kBuckets], wave_total[4];
+    __shared__ int sorted_id[kPiece], sorted_token[kPiece];
+    constexpr int PER = kPiece / 256;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int mask = (p.sort_blocks < kBuckets ? p.sort_blocks : kBuckets) - 1;
+    for (int i = tid; i < 4 * kBuckets; i += 256) count[i] = 0;
+    const long long t0 = (long long)blockIdx.x * kPiece + w * (kPiece / 4) + lane;
+    int id[PER];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const long long tt = t + 64 * j + lane;
-            id[j] = tt < end ? token_id(ids, tt, p.vocabulary) : -1;
-            if (id[j] == p.padding) id[j] = -1;
-        }
+    for (int j = 0; j < PER; ++j) {
+        id[j] = t0 + 64 * j < p.tokens ? token_id(static_cast<const ID*>(p.ids), t0 + 64 * j, p.vocabulary) : -1;
+        if (id[j] == p.padding) id[j] = -1;
+    }
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            const int b = id[j] - lo;
-            const bool in = b >= 0 && b < bins;
-            unsigned long long left = __ballot(in);
-            while (left != 0) {  // one turn per distinct id among the 64 tokens
-                const int first = __ffsll(left) - 1;
-                const int bb = __shfl(b, first, 64);
-                const unsigned long long same = __ballot(in && b == bb);
-                int at = 0;
-                if (lane == first) at = atomicAdd(&count[w * bins + bb], __popcll(same));
-                at = __shfl(at, first, 64);
-                if (in && b == bb) {
-                    at += __popcll(same & ((1ULL << lane) - 1));
-                    p.order[at] = (int)(t + 64 * j + lane);
-                    p.sorted[at] = id[j];
-                }
-                left &= ~same;
-            }
-        }
+    for (int j = 0; j < PER; ++j)
+        if (id[j] >= 0) atomicAdd(&count[w * kBuckets + (id[j] & mask)], 1);
+    __syncthreads();
+    int start, total;
+    scan_counts(count, 4, kBuckets, 0, wave_total, start, total);
+    int* starts = p.piece_start + blockIdx.x;
+    starts[(long long)tid * p.pieces] = start;
+    if (tid == kBuckets - 1) {
+        starts[(long long)kBuckets * p.pieces] = start + total;
+        wave_total[0] = start + total;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int at = take_place(id[j] >= 0, id[j] & mask, 8, count + w * kBuckets);
+        if (id[j] >= 0) sorted_id[at] = id[j], sorted_token[at] = (int)(t0 + 64 * j);
+    }
+    __syncthreads();
+    const int n = wave_total[0];
+    for (int i = tid; i < n; i += 256) {
+        p.piece_id[(long long)blockIdx.x * kPiece + i] = sorted_id[i];
+        p.piece_token[(long long)blockIdx.x * kPiece + i] = sorted_token[i];
     }
 }
 
-__device__ __forceinline__ void put_gradient(const EmbeddingParams& p, int id, int c, f32x4 sum) {
+// How buckets are ranked: by their number modulo 256, then by the rest.
+__device__ __forceinline__ int rank_of_id(const EmbeddingParams& p, int id) {
+    const int b = id & (p.sort_blocks - 1);
+    return ((b & (kBuckets - 1)) << p.fine_log2) | (b / kBuckets);
+}
+
+// Puts the wavefronts' counts of this workgroup's ids in place and notes where each id starts.
+__device__ __forceinline__ void start_ids(const EmbeddingParams& p, int* count, const int* below, int* wave_total) {
+    const int tid = threadIdx.x, rank = blockIdx.x;
+    int first = 0, start, total;
+    for (int k = 0; k < 16; ++k) first += below[k];
+    scan_counts(count, 16, p.bins, first, wave_total, start, total);
+    if (tid < p.bins) p.offsets[rank * p.bins + tid] = start;
+    if (rank == p.sort_blocks - 1 && tid == p.bins - 1) p.offsets[p.sort_blocks * p.bins] = start + total;
+}
+
+// At most kSortDirect tokens.
+template <typename ID>
+__global__ void __launch_bounds__(1024) embedding_sort_kernel(const EmbeddingParams p) {
+    extern __shared__ int count[];  // [16][bins], then the cursors
+    __shared__ int below[16], wave_total[16];
+    constexpr int PER = kSortDirect / 1024;                  // tokens per lane
+    __shared__ unsigned short notes[16][kSortDirect / 16];  // places of the wavefront's tokens of this bucket in its part
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, rank = blockIdx.x;
+    for (int i = tid; i < 16 * p.bins; i += 1024) count[i] = 0;
+    __syncthreads();
+    const int per = (int)((p.tokens + 1023) / 1024) * 64;
+    const int begin = w * per, end = begin + per < p.tokens ? begin + per : (int)p.tokens;
+    const ID* ids = static_cast<const ID*>(p.ids);
+    const unsigned long long before = (1ULL << lane) - 1;
+    int smaller = 0, noted = 0, id[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int t = begin + 64 * j + lane;
+        id[j] = t < end ? token_id(ids, t, p.vocabulary) : -1;
+        if (id[j] == p.padding) id[j] = -1;
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        const int r = rank_of_id(p, id[j]);
+        const bool mine = id[j] >= 0 && r == rank;
+        smaller += id[j] >= 0 && r < rank;
+        const unsigned long long hits = __ballot(mine);
+        if (mine) {
+            atomicAdd(&count[w * p.bins + (id[j] >> p.sort_log2)], 1);
+            notes[w][noted + __popcll(hits & before)] = (unsigned short)(64 * j + lane);
+        }
+        noted += __popcll(hits);
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) smaller += __shfl_xor(smaller, off, 64);
+    if (lane == 0) below[w] = smaller;
+    __syncthreads();
+    start_ids(p, count, below, wave_total);
+    for (int k = 0; k < noted; k += 64) {
+        const bool in = k + lane < noted;
+        const int t = begin + (in ? notes[w][k + lane] : 0);
+        const int number = in ? token_id(ids, t, p.vocabulary) >> p.sort_log2 : 0;
+        const int at = take_place(in, number, p.bins_log2, count + w * p.bins);
+        if (in) p.order[at] = t, p.sorted[at] = rank * p.bins + number;
+    }
+}
+
+// From embedding_bucket_kernel's pieces; a wavefront takes a run of pieces.
+__global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const EmbeddingParams p) {
+    extern __shared__ int count[];  // [16][bins], then the cursors
+    __shared__ int below[16], wave_total[16];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, rank = blockIdx.x;
+    for (int i = tid; i < 16 * p.bins; i += 1024) count[i] = 0;
+    __syncthreads();
+    const int per = (p.pieces + 15) / 16;
+    const int begin = w * per < p.pieces ? w * per : p.pieces, end = begin + per < p.pieces ? begin + per : p.pieces;
+    const int* from = p.piece_start + (long long)(rank >> p.fine_log2) * p.pieces;
+    const int* to = from + p.pieces;
+    int smaller = 0;
+    // all tokens of the pieces' lists, up to 64 pieces' bounds at a time in the lanes
+    auto walk = [&](auto&& visit) {
+        for (int i0 = begin; i0 < end; i0 += 64) {
+            const int a_of = i0 + lane < end ? from[i0 + lane] : 0, b_of = i0 + lane < end ? to[i0 + lane] : 0;
+            const int here = end - i0 < 64 ? end - i0 : 64;
+            for (int i = 0; i < here; ++i) {
+                const int a = __shfl(a_of, i, 64), b = __shfl(b_of, i, 64);
+                const long long base = (long long)(i0 + i) * kPiece;
+                for (int k = a; k < b; k += 64) visit(base + k + lane, k + lane < b);
+            }
+        }
+    };
+    for (int i = begin + lane; i < end; i += 64) smaller += from[i];
+    walk([&](long long at, bool in) {
+        if (!in) return;
+        const int id = p.piece_id[at], r = rank_of_id(p, id);
+        if (r == rank)
+            atomicAdd(&count[w * p.bins + (id >> p.sort_log2)], 1);
+        else
+            smaller += r < rank;
+    });
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) smaller += __shfl_xor(smaller, off, 64);
+    if (lane == 0) below[w] = smaller;
+    __syncthreads();
+    start_ids(p, count, below, wave_total);
+    walk([&](long long from_at, bool in) {
+        const int id = in ? p.piece_id[from_at] : -1;
+        in = in && rank_of_id(p, id) == rank;
+        const int number = in ? id >> p.sort_log2 : 0;
+        const int at = take_place(in, number, p.bins_log2, count + w * p.bins);
+        if (in) p.order[at] = p.piece_token[from_at], p.sorted[at] = rank * p.bins + number;
+    });
+}
+
+__device__ __forceinline__ int id_of_key(const EmbeddingParams& p, int key) {
+    const int rank = key / p.bins;
+    return ((key - rank * p.bins) << p.sort_log2) | (rank >> p.fine_log2) | ((rank & ((1 << p.fine_log2) - 1)) * kBuckets);
+}
+
+__device__ __forceinline__ void put_gradient(const EmbeddingParams& p, int key, int c, f32x4 sum) {
+    const int id = id_of_key(p, key);
     float* row = static_cast<float*>(p.out) + (long long)id * p.ld_out;
     sum *= p.scale;
     if (p.accumulate) sum += load4(row, c, p.dim, p.whole);
@@ -187,19 +317,27 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     const int groups = 256 >> p.lanes_log2;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
+    const int keys = p.sort_blocks * p.bins;
     if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has
         constexpr int ROWS = 8;
         const long long r0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * ROWS;
+        bool clear[ROWS];
 #pragma unroll
         for (int k = 0; k < ROWS; ++k) {
-            const long long r = r0 + k;
-            if (r < p.vocabulary && p.offsets[r] == p.offsets[r + 1])
-                store4(static_cast<float*>(p.out) + r * p.ld_out, c, p.dim, p.whole, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+            const int r = (int)(r0 + k);
+            clear[k] = r0 + k < p.vocabulary;
+            if (clear[k]) {
+                const int key = rank_of_id(p, r) * p.bins + (r >> p.sort_log2);
+                clear[k] = p.offsets[key] == p.offsets[key + 1];
+            }
         }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out, c, p.dim, p.whole, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         return;
     }
     const long long k = (long long)blockIdx.x * groups + group;
-    const long long n = p.offsets[p.vocabulary];
+    const long long n = p.offsets[keys];
     const long long p0 = k * p.chunk;
     if (p0 >= n) return;
     const long long p1 = p0 + p.chunk < n ? p0 + p.chunk : n;
@@ -210,29 +348,37 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float* slot = p.partial + 2 * k * p.dim;
     const bool whole_slot = (p.dim & 3) == 0;
-    for (long long q = p0; q < p1; q += U) {
-        int id[U];
-        f32x4 v[U];
+    int key[U], token[U];
+    auto fetch = [&](long long q) {  // behind the chunk's end: its last token again
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const bool in = q + j < p1;
-            id[j] = in ? p.sorted[q + j] : -1;
-            v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (in) v[j] = load4(dy + (long long)p.order[q + j] * p.ld_in, c, p.dim, p.whole);
+            const long long at = q + j < p1 ? q + j : p1 - 1;
+            key[j] = p.sorted[at], token[j] = p.order[at];
         }
+    };
+    fetch(p0);
+    for (long long q = p0; q < p1; q += U) {
+        typename Raw4<T>::type v[U];
+        int now[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            if (id[j] < 0) continue;
-            if (id[j] != cur) {  // the run before has ended
+            v[j] = load4_raw(dy + (long long)token[j] * p.ld_in, c, p.dim, p.whole);
+            now[j] = q + j < p1 ? key[j] : -1;
+        }
+        if (q + U < p1) fetch(q + U);
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+            if (now[j] < 0) continue;
+            if (now[j] != cur) {  // the run before has ended
                 if (came_in)
                     store4(slot, c, p.dim, whole_slot, sum);
                 else
                     put_gradient(p, cur, c, sum);
                 came_in = false;
-                cur = id[j];
-                sum = v[j];
+                cur = now[j];
+                sum = widen(v[j]);
             } else {
-                sum += v[j];
+                sum += widen(v[j]);
             }
         }
     }
@@ -253,12 +399,12 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
     const long long k = (long long)blockIdx.x * groups + group;
-    const long long n = p.offsets[p.vocabulary];
+    const long long n = p.offsets[p.sort_blocks * p.bins];
     const long long last = (k + 1) * p.chunk - 1;
     if (last + 1 >= n) return;
-    const int id = p.sorted[last];
-    if (p.sorted[last + 1] != id || p.offsets[id] < k * p.chunk) return;
-    const long long k_end = (p.offsets[id + 1] - 1) / p.chunk;
+    const int key = p.sorted[last];
+    if (p.sorted[last + 1] != key || p.offsets[key] < k * p.chunk) return;
+    const long long k_end = (p.offsets[key + 1] - 1) / p.chunk;
     const bool whole_slot = (p.dim & 3) == 0;
     const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim, c, p.dim, whole_slot);
     double sum[4] = {first[0], first[1], first[2], first[3]};
@@ -274,7 +420,7 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum[e] += v[j][e];
     }
-    put_gradient(p, id, c, f32x4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
+    put_gradient(p, key, c, f32x4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
 }
 
 }  // namespace snhip

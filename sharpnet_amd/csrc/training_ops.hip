@@ -36,8 +36,8 @@ int embedding_check_desc(const snhip_embedding_desc* d) {
     if (d->tokens < 0 || d->vocabulary < 0 || d->dim < 0 || d->padding_index < -1) return SNHIP_STATUS_INVALID_VALUE;
     if ((d->ld_table != 0 && d->ld_table < d->dim) || (d->ld_output != 0 && d->ld_output < d->dim))
         return SNHIP_STATUS_INVALID_VALUE;
-    // token numbers and the places in the sorted order are 32-bit integers
-    if (d->tokens > 0x7fff0000LL || d->vocabulary > 0x7fff0000) return SNHIP_STATUS_NOT_SUPPORTED;
+    // token numbers, the places in the sorted order and the ids' keys in it are 32-bit integers
+    if (d->tokens > 0x7fff0000LL || d->vocabulary > 0x3fffffff) return SNHIP_STATUS_NOT_SUPPORTED;
     return SNHIP_STATUS_SUCCESS;
 }
 
@@ -58,21 +58,30 @@ EmbeddingParams embedding_params(const snhip_embedding_desc* d, const void* ids,
 }
 
 struct EmbeddingPlan {
-    int bins, chunk;
+    int sort_blocks, sort_log2, fine_log2, bins, bins_log2, chunk, pieces;
     long long chunks;
-    size_t order, sorted, offsets, partial, bytes;  // places in the workspace
+    size_t order, sorted, offsets, piece_id, piece_token, piece_start, partial, bytes;  // places in the workspace
 };
 EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
     EmbeddingPlan e{};
-    e.bins = ceil_div(d->vocabulary, 256);
+    // a workgroup of the sort per compute unit, more where it would get over 512 ids
+    e.sort_log2 = 0;
+    while ((1LL << e.sort_log2) < d->vocabulary && (e.sort_log2 < 8 || (512LL << e.sort_log2) < d->vocabulary)) ++e.sort_log2;
+    e.sort_blocks = 1 << e.sort_log2;
+    e.fine_log2 = e.sort_log2 > 8 ? e.sort_log2 - 8 : 0;
+    e.pieces = d->tokens > kSortDirect ? (int)((d->tokens + kPiece - 1) / kPiece) : 0;
+    e.bins = (int)(((long long)d->vocabulary + e.sort_blocks - 1) >> e.sort_log2);
     if (e.bins < 1) e.bins = 1;
-    if (e.bins > 512) e.bins = 512;
+    while ((1 << e.bins_log2) < e.bins) ++e.bins_log2;
     e.chunk = d->tokens >= 16384 ? 32 : 8;
     e.chunks = (d->tokens + e.chunk - 1) / e.chunk;
     e.order = 0;
     e.sorted = e.order + up256((size_t)d->tokens * 4);
     e.offsets = e.sorted + up256((size_t)d->tokens * 4);
-    e.partial = e.offsets + up256(((size_t)d->vocabulary + 1) * 4);
+    e.piece_id = e.offsets + up256(((size_t)e.sort_blocks * e.bins + 1) * 4);
+    e.piece_token = e.piece_id + up256((size_t)e.pieces * kPiece * 4);
+    e.piece_start = e.piece_token + up256((size_t)e.pieces * kPiece * 4);
+    e.partial = e.piece_start + up256((size_t)e.pieces * (kBuckets + 1) * 4);
     e.bytes = e.partial + up256((size_t)e.chunks * 2 * (size_t)d->dim * 4);
     return e;
 }
@@ -96,6 +105,16 @@ void embedding_forward_types(const EmbeddingParams& p, int table_type, int outpu
         embedding_forward_launch<ID, float, __bf16>(p, stream);
     else
         embedding_forward_launch<ID, float, float>(p, stream);
+}
+
+template <typename ID>
+void embedding_sort_launch(const EmbeddingParams& p, dim3 grid, size_t lds, hipStream_t stream) {
+    if (p.pieces == 0) {
+        hipLaunchKernelGGL(embedding_sort_kernel<ID>, grid, dim3(1024), lds, stream, p);
+    } else {
+        hipLaunchKernelGGL(embedding_bucket_kernel<ID>, dim3((unsigned)p.pieces), dim3(256), 0, stream, p);
+        hipLaunchKernelGGL(embedding_sort_pieces_kernel, grid, dim3(1024), lds, stream, p);
+    }
 }
 
 // ---- block norm ----------------------------------------------------------------------------------------------
@@ -348,20 +367,23 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     const int col_blocks = ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2);
     if (col_blocks > 65535) return SNHIP_STATUS_NOT_SUPPORTED;
     p.accumulate = accumulate != 0;
-    p.bins = e.bins, p.chunk = e.chunk;
+    p.sort_blocks = e.sort_blocks, p.sort_log2 = e.sort_log2, p.bins = e.bins, p.bins_log2 = e.bins_log2, p.chunk = e.chunk;
+    p.fine_log2 = e.fine_log2, p.pieces = e.pieces;
     char* ws = static_cast<char*>(workspace);
     p.order = reinterpret_cast<int*>(ws + e.order), p.sorted = reinterpret_cast<int*>(ws + e.sorted);
     p.offsets = reinterpret_cast<int*>(ws + e.offsets), p.partial = reinterpret_cast<float*>(ws + e.partial);
+    p.piece_id = reinterpret_cast<int*>(ws + e.piece_id), p.piece_token = reinterpret_cast<int*>(ws + e.piece_token);
+    p.piece_start = reinterpret_cast<int*>(ws + e.piece_start);
     const int groups = 256 >> p.lanes_log2;
     p.chunk_blocks = (e.chunks + groups - 1) / groups;
-    const dim3 sort_grid((unsigned)ceil_div(p.vocabulary, p.bins));
+    const dim3 sort_grid((unsigned)p.sort_blocks);
     const size_t lds = (size_t)16 * p.bins * sizeof(int);
     if (desc->id_type == SNHIP_TYPE_F32)
-        hipLaunchKernelGGL(embedding_sort_kernel<float>, sort_grid, dim3(1024), lds, h->stream, p);
+        embedding_sort_launch<float>(p, sort_grid, lds, h->stream);
     else if (desc->id_type == SNHIP_TYPE_I32)
-        hipLaunchKernelGGL(embedding_sort_kernel<int>, sort_grid, dim3(1024), lds, h->stream, p);
+        embedding_sort_launch<int>(p, sort_grid, lds, h->stream);
     else
-        hipLaunchKernelGGL(embedding_sort_kernel<long long>, sort_grid, dim3(1024), lds, h->stream, p);
+        embedding_sort_launch<long long>(p, sort_grid, lds, h->stream);
     const long long clear_blocks = p.accumulate ? 0 : ((long long)p.vocabulary + 8 * groups - 1) / (8 * groups);
     const dim3 grid((unsigned)(p.chunk_blocks + clear_blocks), (unsigned)col_blocks);
     if (desc->output_type == SNHIP_TYPE_BF16)
