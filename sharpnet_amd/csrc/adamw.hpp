@@ -9,6 +9,8 @@
 
 namespace snhip {
 
+typedef unsigned int u32_any __attribute__((aligned(1)));  // four bytes at any address
+
 constexpr int kAdamwBlock = 256;   // elements that share a power of two (states in 8 bits)
 constexpr int kAdamwChunk = 4096;  // elements of a tensor that a workgroup of 256 threads updates
 
@@ -21,7 +23,7 @@ struct AdamwEntry {
     long long count;
     long long first_chunk;  // of the launch
     float decay;
-    int g_bf16, whole;      // whole: every address allows four elements at a time
+    int g_bf16;
 };
 
 struct AdamwScalars {
@@ -42,8 +44,9 @@ __device__ __forceinline__ float moment2(float v, float g, const AdamwScalars& s
     const float a = v * s.beta2, b = (g * g) * s.rest2;
     return a + b;
 }
+// (the hardware's reciprocal, 1 ulp: the denominator is 0 or between 1e-23 and 1e20, where it is exact to that)
 __device__ __forceinline__ float new_parameter(float p, float m, float v, float keep, const AdamwScalars& s) {
-    return p * keep - s.step_size * (m / (sqrtf(v) * s.root_scale + s.eps));
+    return p * keep - s.step_size * (m * __builtin_amdgcn_rcpf(sqrtf(v) * s.root_scale + s.eps));
 }
 
 // Four elements of the gradient as they lie in memory, and what they are worth: the conversion is kept away from the load,
@@ -52,12 +55,12 @@ struct RawGradient {
     f32x4 f;
     bf16x4 b;
 };
-__device__ __forceinline__ RawGradient load_gradient(const AdamwEntry& t, long long i, int left, bool whole) {
+__device__ __forceinline__ RawGradient load_gradient(const AdamwEntry& t, long long i, int left) {
     RawGradient r;
     if (t.g_bf16)
-        r.b = load4_raw(static_cast<const __bf16*>(t.g) + i, 0, left, whole);
+        r.b = load4(static_cast<const __bf16*>(t.g) + i, left);
     else
-        r.f = load4_raw(static_cast<const float*>(t.g) + i, 0, left, whole);
+        r.f = load4(static_cast<const float*>(t.g) + i, left);
     return r;
 }
 __device__ __forceinline__ f32x4 gradient_of(const AdamwEntry& t, const RawGradient& r, float scale) {
@@ -75,9 +78,8 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restri
         const long long i = base + k * 1024 + threadIdx.x * 4;
         if (i >= t.count) break;
         const int left = t.count - i < 4 ? (int)(t.count - i) : 4;
-        const bool whole = t.whole && left == 4;
-        const RawGradient raw = load_gradient(t, i, left, whole);
-        f32x4 pp = load4(t.p + i, 0, left, whole), mm = load4(m + i, 0, left, whole), vv = load4(v + i, 0, left, whole);
+        const RawGradient raw = load_gradient(t, i, left);
+        f32x4 pp = load4(t.p + i, left), mm = load4(m + i, left), vv = load4(v + i, left);
         const f32x4 g = gradient_of(t, raw, s.grad_scale);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -85,10 +87,10 @@ __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restri
             vv[j] = moment2(vv[j], g[j], s);
             pp[j] = new_parameter(pp[j], mm[j], vv[j], keep, s);
         }
-        store4(t.p + i, 0, left, whole, pp);
-        store4(m + i, 0, left, whole, mm);
-        store4(v + i, 0, left, whole, vv);
-        if (t.copy != nullptr) store4(t.copy + i, 0, left, whole, pp);
+        store4(t.p + i, left, pp);
+        store4(m + i, left, mm);
+        store4(v + i, left, vv);
+        if (t.copy != nullptr) store4(t.copy + i, left, pp);
     }
 }
 
@@ -135,16 +137,15 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restric
         if (b0 >= t.count) break;
         const long long i = b0 + lane * 4;
         const int left = t.count - i < 4 ? (int)(t.count - i) : 4;  // <= 0: behind the tensor's end
-        const bool whole = t.whole && left == 4;
         unsigned int mbits = 0, vbits = 0;
         RawGradient raw = {};
         f32x4 pp = {0.0f, 0.0f, 0.0f, 0.0f}, mm, vv;
         if (left > 0) {
-            raw = load_gradient(t, i, left, whole);
-            pp = load4(t.p + i, 0, left, whole);
-            if (whole) {
-                mbits = *reinterpret_cast<const unsigned int*>(m8 + i);
-                vbits = *reinterpret_cast<const unsigned int*>(v8 + i);
+            raw = load_gradient(t, i, left);
+            pp = load4(t.p + i, left);
+            if (left == 4) {
+                mbits = *reinterpret_cast<const u32_any*>(m8 + i);
+                vbits = *reinterpret_cast<const u32_any*>(v8 + i);
             } else {
                 for (int j = 0; j < left; ++j) {
                     mbits |= (unsigned int)m8[i + j] << (8 * j);
@@ -199,11 +200,11 @@ __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restric
             if (!(fabsf(vv[j]) < __builtin_inff())) v_bytes[j] = 0x7fu;
         }
         if (left > 0) {
-            store4(t.p + i, 0, left, whole, pp);
-            if (t.copy != nullptr) store4(t.copy + i, 0, left, whole, pp);
-            if (whole) {
-                *reinterpret_cast<unsigned int*>(m8 + i) = m_bytes[0] | m_bytes[1] << 8 | m_bytes[2] << 16 | m_bytes[3] << 24;
-                *reinterpret_cast<unsigned int*>(v8 + i) = v_bytes[0] | v_bytes[1] << 8 | v_bytes[2] << 16 | v_bytes[3] << 24;
+            store4(t.p + i, left, pp);
+            if (t.copy != nullptr) store4(t.copy + i, left, pp);
+            if (left == 4) {
+                *reinterpret_cast<u32_any*>(m8 + i) = m_bytes[0] | m_bytes[1] << 8 | m_bytes[2] << 16 | m_bytes[3] << 24;
+                *reinterpret_cast<u32_any*>(v8 + i) = v_bytes[0] | v_bytes[1] << 8 | v_bytes[2] << 16 | v_bytes[3] << 24;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)

@@ -29,15 +29,21 @@ namespace {
 template <int TPR, int N>
 void forward(const BlockNormParams& p, hipStream_t stream) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
-    hipLaunchKernelGGL((block_norm_forward_kernel<Stream, Block, TPR, N>), dim3((unsigned)((p.rows + GROUPS - 1) / GROUPS)),
-                       dim3(NT), 0, stream, p);
+    const dim3 grid((unsigned)((p.rows + GROUPS - 1) / GROUPS));
+    if (p.exact)
+        hipLaunchKernelGGL((block_norm_forward_kernel<Stream, Block, TPR, N, true>), grid, dim3(NT), 0, stream, p);
+    else
+        hipLaunchKernelGGL((block_norm_forward_kernel<Stream, Block, TPR, N, false>), grid, dim3(NT), 0, stream, p);
 }
 
 template <int TPR, int N, int MODE, bool BIAS, bool GATE>
 void backward(const BlockNormParams& p, hipStream_t stream) {
     constexpr int NT = TPR > 256 ? TPR : 256;
-    hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE>), dim3((unsigned)p.chunks), dim3(NT),
-                       0, stream, p);
+    const dim3 grid((unsigned)p.chunks);
+    if (p.exact)
+        hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, true>), grid, dim3(NT), 0, stream, p);
+    else
+        hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, false>), grid, dim3(NT), 0, stream, p);
 }
 
 template <int TPR, int N>

@@ -2,6 +2,9 @@
 // snhip_block_norm_desc).  One pass over the rows forward and backward, a row in the registers of TPR threads (N pieces of
 // four columns each): every input is read once, every output written once, so both are bound by HBM.  Sums run in fp32:
 // per thread, then over the row's threads; the variance is taken around the mean, from the registers.
+// EXACT: dim is a multiple of four and rows start on 4-byte addresses: a thread's pieces are four neighbours each, one wide
+// access.  Otherwise the four elements of a piece are TPR columns apart, narrow accesses that neighbouring threads make side
+// by side.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -20,7 +23,8 @@ struct BlockNormParams {
     const void *du, *dh;
     void *dx, *dy, *d_gate;
     long long rows, ld_x, ld_y, ld_u, ld_h, ld_gate;
-    int dim, gate_rows, pre, post, act, whole;
+    int dim, gate_rows, pre, post, act;
+    int exact;                 // which instantiations serve it (EXACT)
     float eps, scale, inv_dim;
     // backward: a workgroup takes a chunk of rows
     float* partial;            // [vector][chunk][dim]: column sums of pre weight, pre bias, post weight, post bias, gate
@@ -31,16 +35,104 @@ struct BlockNormParams {
     int slot[5];               // which vector of `partial` a column sum goes to, -1: not wanted
 };
 
-// Sum of A and B over the TPR threads of a row.  Up to a wavefront: by shuffles.  Beyond: the wavefronts' sums meet in LDS;
-// `turn` alternates between two places, so that one barrier a sum is enough.
+// ---- pieces of a row -----------------------------------------------------------------------------------------------
+// Rows are read and written as buffers of their own length: the base is scalar, the place in the row a 32-bit offset (64-bit
+// addresses for every piece of every tensor took a third of the vector registers), what is read behind the row's end is zero
+// and what is written there is dropped, without a branch.  16 threads to a row share a wavefront with other rows, whose bases
+// differ: there plain accesses with the end checked.
+typedef unsigned int u32x2 __attribute__((vector_size(8)));
+typedef unsigned int u32x4 __attribute__((vector_size(16)));
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* row, int bytes) {
+    // raw buffer of 32-bit elements
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(row), 0, bytes, 0x00027000);
+}
+
+template <int TPR, bool EXACT>
+struct Piece {
+    // (a buffer's length counts in 32-bit elements: single bf16 elements go the plain way)
+    template <typename T>
+    static constexpr bool BUFFER = TPR >= 64 && (EXACT || sizeof(T) == 4);
+    // column of element j of piece n
+    __device__ __forceinline__ static int column(int n, int j, int lane) {
+        return EXACT ? 4 * (n * TPR + lane) + j : (4 * n + j) * TPR + lane;
+    }
+    template <typename T>
+    __device__ __forceinline__ static raw4<T> load(const T* row, int n, int lane, int dim) {
+        raw4<T> v = {};
+        if constexpr (BUFFER<T>) {
+            const __amdgpu_buffer_rsrc_t b = row_buffer(row, dim * (int)sizeof(T));
+            if constexpr (EXACT && sizeof(T) == 4) {
+                v = __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b128(b, 4 * column(n, 0, lane), 0, 0));
+            } else if constexpr (EXACT) {
+                v = __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b64(b, 2 * column(n, 0, lane), 0, 0));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    v[j] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(b, 4 * column(n, j, lane), 0, 0));
+            }
+        } else if constexpr (EXACT) {
+            if (column(n, 0, lane) < dim) v = load4_whole(row + column(n, 0, lane));
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (column(n, j, lane) < dim) v[j] = row[column(n, j, lane)];
+        }
+        return v;
+    }
+    template <typename T>
+    __device__ __forceinline__ static void store(T* row, int n, int lane, int dim, f32x4 value) {
+        const raw4<T> v = narrow(value, static_cast<const T*>(nullptr));
+        if constexpr (BUFFER<T>) {
+            const __amdgpu_buffer_rsrc_t b = row_buffer(row, dim * (int)sizeof(T));
+            if constexpr (EXACT && sizeof(T) == 4) {
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), b, 4 * column(n, 0, lane), 0, 0);
+            } else if constexpr (EXACT) {
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, v), b, 2 * column(n, 0, lane), 0, 0);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, (float)v[j]), b, 4 * column(n, j, lane), 0, 0);
+            }
+        } else if constexpr (EXACT) {
+            if (column(n, 0, lane) < dim) store4_whole(row + column(n, 0, lane), value);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (column(n, j, lane) < dim) row[column(n, j, lane)] = v[j];
+        }
+    }
+    // zeros behind the row's end, where a computation has left something else
+    __device__ __forceinline__ static f32x4 cut(f32x4 v, int n, int lane, int dim) {
+        if constexpr (EXACT) {
+            if (column(n, 0, lane) >= dim) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (column(n, j, lane) >= dim) v[j] = 0.0f;
+        }
+        return v;
+    }
+    // of a weight or bias vector; `missing` where there is none
+    __device__ __forceinline__ static f32x4 vector(const float* v, int n, int lane, int dim, float missing) {
+        if (v == nullptr) return f32x4{missing, missing, missing, missing};
+        return load(v, n, lane, dim);
+    }
+};
+
+// ---- sums over a row -----------------------------------------------------------------------------------------------
+// Over the TPR threads of a row, TPR = 16 or a multiple of 64.  Beyond a wavefront the wavefronts' sums meet in LDS; `turn`
+// alternates between two places, so that one barrier a sum is enough.
+template <int TPR>
+__device__ __forceinline__ float lanes_sum(float a) {
+    if constexpr (TPR == 16)
+        return row16_sum(a);
+    else
+        return wave64_sum(a);
+}
 template <int TPR>
 __device__ __forceinline__ void row_sums(float& a, float& b, float (*lds)[2][TPR / 64 + 1], int& turn) {
-    constexpr int W = TPR < 64 ? TPR : 64;
-#pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1) {
-        a += __shfl_xor(a, off, 64);
-        b += __shfl_xor(b, off, 64);
-    }
+    a = lanes_sum<TPR>(a), b = lanes_sum<TPR>(b);
     if constexpr (TPR > 64) {
         const int w = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) lds[turn][0][w] = a, lds[turn][1][w] = b;
@@ -53,9 +145,7 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float (*lds)[2][TPR
 }
 template <int TPR>
 __device__ __forceinline__ float row_sum(float a, float (*lds)[2][TPR / 64 + 1], int& turn) {
-    constexpr int W = TPR < 64 ? TPR : 64;
-#pragma unroll
-    for (int off = W / 2; off > 0; off >>= 1) a += __shfl_xor(a, off, 64);
+    a = lanes_sum<TPR>(a);
     if constexpr (TPR > 64) {
         const int w = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) lds[turn][0][w] = a;
@@ -68,29 +158,44 @@ __device__ __forceinline__ float row_sum(float a, float (*lds)[2][TPR / 64 + 1],
     return a;
 }
 
-// Columns [c, c + 4) of a weight or bias vector; `missing` where there is no vector; 0 behind the row's end.
-__device__ __forceinline__ f32x4 vector4(const float* v, int c, const BlockNormParams& p, float missing) {
-    if (v != nullptr) return load4(v, c, p.dim, p.whole);
-    f32x4 r;
+// ---- gate ------------------------------------------------------------------------------------------------------------
+// The sigmoid from the hardware's exponential and reciprocal (1 ulp each; the exponent's rounding adds |g| 2^-24).
+// tanh x = (1 - e) / (1 + e) with e = exp(-2 |x|) from |x| = 1/4 on, where the difference keeps its digits (4 ulp), and its
+// Taylor series to x^9 below (the next term is under 2^-26 of x).
+__device__ __forceinline__ f32x4 gate_values(f32x4 g, int act) {
+    if (act == GATE_SIGMOID) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = c + j < p.dim ? missing : 0.0f;
-    return r;
+        for (int j = 0; j < 4; ++j) g[j] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g[j] * -1.44269504088896341f));
+    } else if (act == GATE_TANH) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = g[j], a = fabsf(x), z = x * x;
+            const float e = __builtin_amdgcn_exp2f(a * -2.88539008177792681f);
+            const float large = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
+            const float series = ((((62.0f / 2835.0f * z - 17.0f / 315.0f) * z + 2.0f / 15.0f) * z - 1.0f / 3.0f) * z) * x + x;
+            g[j] = a < 0.25f ? series : large;
+        }
+    }
+    return g;
+}
+__device__ __forceinline__ f32x4 gate_slopes(f32x4 q, int act) {  // in terms of q = act(g)
+    if (act == GATE_SIGMOID) return q - q * q;
+    if (act == GATE_TANH) return 1.0f - q * q;
+    return f32x4{1.0f, 1.0f, 1.0f, 1.0f};
 }
 
-__device__ __forceinline__ float gate_value(float g, int act) {
-    return act == GATE_SIGMOID ? 1.0f / (1.0f + expf(-g)) : act == GATE_TANH ? tanhf(g) : g;
-}
-__device__ __forceinline__ float gate_slope(float q, int act) {  // in terms of q = act(g)
-    return act == GATE_SIGMOID ? q * (1.0f - q) : act == GATE_TANH ? 1.0f - q * q : 1.0f;
-}
-template <typename TB>
-__device__ __forceinline__ f32x4 gate4(const BlockNormParams& p, long long row, int c) {
-    if (p.gate_rows == 0) return load4(static_cast<const float*>(p.gate), c, p.dim, p.whole);
-    return load4(static_cast<const TB*>(p.gate) + row / p.gate_rows * p.ld_gate, c, p.dim, p.whole);
+// which row of the workgroup's rows this thread works on: the same for a wavefront where a row takes one or more
+template <int TPR>
+__device__ __forceinline__ int row_group() {
+    const int g = (int)threadIdx.x / TPR;
+    if constexpr (TPR >= 64)
+        return __builtin_amdgcn_readfirstlane(g);
+    else
+        return g;
 }
 
-// mean and 1 / deviation of the row in z
-template <int TPR, int N>
+// mean and 1 / deviation of the row in z (zeros behind its end)
+template <bool EXACT, int TPR, int N>
 __device__ __forceinline__ void row_statistics(const f32x4 (&z)[N], int lane, int kind, const BlockNormParams& p,
                                                float (*lds)[2][TPR / 64 + 1], int& turn, float& mean, float& rstd) {
     mean = 0.0f;
@@ -103,90 +208,90 @@ __device__ __forceinline__ void row_statistics(const f32x4 (&z)[N], int lane, in
     float s = 0.0f;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int c = 4 * (n * TPR + lane);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float d = z[n][j] - mean;
-            if (c + j < p.dim) s += d * d;
-        }
+        const f32x4 d = Piece<TPR, EXACT>::cut(z[n] - mean, n, lane, p.dim);
+        s += (d[0] * d[0] + d[1] * d[1]) + (d[2] * d[2] + d[3] * d[3]);
     }
-    rstd = 1.0f / sqrtf(row_sum<TPR>(s, lds, turn) * p.inv_dim + p.eps);
+    rstd = __builtin_amdgcn_rsqf(row_sum<TPR>(s, lds, turn) * p.inv_dim + p.eps);
 }
 
-template <typename TS, typename TB, int TPR, int N>
+template <typename TS, typename TB, int TPR, int N, bool EXACT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_forward_kernel(const BlockNormParams p) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
+    typedef Piece<TPR, EXACT> P;
     __shared__ float lds[2][2][TPR / 64 + 1];
     int turn = 0;
-    const int lane = threadIdx.x % TPR;
-    const long long row = (long long)blockIdx.x * GROUPS + threadIdx.x / TPR;
+    const int lane = threadIdx.x % TPR, dim = p.dim;
+    const long long row = (long long)blockIdx.x * GROUPS + row_group<TPR>();
     if (row >= p.rows) return;  // (with a barrier ahead a workgroup has one row)
     f32x4 u[N];
-    const TS* x = static_cast<const TS*>(p.x) + row * p.ld_x;
+    raw4<TS> x[N];
+#pragma unroll
+    for (int n = 0; n < N; ++n) x[n] = P::load(static_cast<const TS*>(p.x) + row * p.ld_x, n, lane, dim);
     float mean, rstd;
     if (p.y != nullptr) {
-        const TB* yr = static_cast<const TB*>(p.y) + row * p.ld_y;
+        raw4<TB> y_raw[N], g_raw[N];
+        const bool gate_in_rows = p.gate != nullptr && p.gate_rows != 0;
+#pragma unroll
+        for (int n = 0; n < N; ++n) y_raw[n] = P::load(static_cast<const TB*>(p.y) + row * p.ld_y, n, lane, dim);
+        if (gate_in_rows) {
+            const TB* gate = static_cast<const TB*>(p.gate) + (long long)((unsigned int)row / (unsigned int)p.gate_rows) * p.ld_gate;
+#pragma unroll
+            for (int n = 0; n < N; ++n) g_raw[n] = P::load(gate, n, lane, dim);
+        }
         f32x4 y[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = 4 * (n * TPR + lane);
-            y[n] = u[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (c < p.dim) {
-                y[n] = load4(yr, c, p.dim, p.whole);
-                u[n] = load4(x, c, p.dim, p.whole);
+        for (int n = 0; n < N; ++n) y[n] = widen(y_raw[n]);
+        if (p.post != NORM_NONE) {
+            row_statistics<EXACT, TPR, N>(y, lane, p.post, p, lds, turn, mean, rstd);
+            if (p.post_s != nullptr && lane == 0) p.post_s[2 * row] = mean, p.post_s[2 * row + 1] = rstd;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                    y[n] = (y[n] - mean) * rstd * P::vector(p.post_w, n, lane, dim, 1.0f) + P::vector(p.post_b, n, lane, dim, 0.0f);
             }
         }
-        if (p.post != NORM_NONE) {
-            row_statistics<TPR, N>(y, lane, p.post, p, lds, turn, mean, rstd);
-            if (p.post_s != nullptr && lane == 0) p.post_s[2 * row] = mean, p.post_s[2 * row + 1] = rstd;
+        if (p.gate != nullptr) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                f32x4 g;
+                if (gate_in_rows)
+                    g = widen(g_raw[n]);
+                else
+                    g = P::load(static_cast<const float*>(p.gate), n, lane, dim);
+                y[n] *= gate_values(g, p.act);
+            }
         }
         TS* ur = static_cast<TS*>(p.u) + row * p.ld_u;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = 4 * (n * TPR + lane);
-            if (c >= p.dim) continue;
-            f32x4 v = y[n];
-            if (p.post != NORM_NONE) v = (v - mean) * rstd * vector4(p.post_w, c, p, 1.0f) + vector4(p.post_b, c, p, 0.0f);
-            if (p.gate != nullptr) {
-                const f32x4 g = gate4<TB>(p, row, c);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] *= gate_value(g[j], p.act);
-            }
-            u[n] = as_stored(u[n] + p.scale * v, static_cast<const TS*>(nullptr));
-            store4(ur, c, p.dim, p.whole, u[n]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (c + j >= p.dim) u[n][j] = 0.0f;
+            u[n] = as_stored<TS>(widen(x[n]) + p.scale * y[n]);
+            P::store(ur, n, lane, dim, u[n]);
+            u[n] = P::cut(u[n], n, lane, dim);
         }
     } else {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = 4 * (n * TPR + lane);
-            u[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (c < p.dim) u[n] = load4(x, c, p.dim, p.whole);
-        }
+        for (int n = 0; n < N; ++n) u[n] = widen(x[n]);
     }
     if (p.pre == NORM_NONE) return;
-    row_statistics<TPR, N>(u, lane, p.pre, p, lds, turn, mean, rstd);
+    row_statistics<EXACT, TPR, N>(u, lane, p.pre, p, lds, turn, mean, rstd);
     if (p.pre_s != nullptr && lane == 0) p.pre_s[2 * row] = mean, p.pre_s[2 * row + 1] = rstd;
     TB* hr = static_cast<TB*>(p.h) + row * p.ld_h;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int c = 4 * (n * TPR + lane);
-        if (c < p.dim)
-            store4(hr, c, p.dim, p.whole, (u[n] - mean) * rstd * vector4(p.pre_w, c, p, 1.0f) + vector4(p.pre_b, c, p, 0.0f));
+        P::store(hr, n, lane, dim, (u[n] - mean) * rstd * P::vector(p.pre_w, n, lane, dim, 1.0f) + P::vector(p.pre_b, n, lane, dim, 0.0f));
     }
 }
 
-// dz = dN(z) * dn for the row in registers: in: hat = z normed, a = dn * weight; out: a becomes dz
+// dz = dN(z) * dn for the row in registers: in: hat = z normed, a = dn * weight (zeros behind the row's end); out: a becomes dz
 template <int TPR, int N>
 __device__ __forceinline__ void row_gradient(f32x4 (&a)[N], const f32x4 (&hat)[N], int kind, float rstd, const BlockNormParams& p,
                                              float (*lds)[2][TPR / 64 + 1], int& turn) {
     float s = 0.0f, m = 0.0f;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s += a[n][j] * hat[n][j], m += a[n][j];
+    for (int n = 0; n < N; ++n) {
+        const f32x4 q = a[n] * hat[n];
+        s += (q[0] + q[1]) + (q[2] + q[3]);
+        m += (a[n][0] + a[n][1]) + (a[n][2] + a[n][3]);
+    }
     if (kind == NORM_LAYER) {
         row_sums<TPR>(s, m, lds, turn);
         m *= p.inv_dim;
@@ -202,13 +307,15 @@ __device__ __forceinline__ void row_gradient(f32x4 (&a)[N], const f32x4 (&hat)[N
 // MODE 0: no block (the pre norm alone), 1: a block without a norm behind it, 2: with one.  BIAS / GATE: column sums for
 // biases / a gate are kept.  A workgroup walks a chunk of rows and keeps the column sums of its columns in registers; at the
 // end it writes them to `partial`, and column_parts_kernel adds the chunks in order.
-template <typename TS, typename TB, int TPR, int N, int MODE, bool BIAS, bool GATE>
+template <typename TS, typename TB, int TPR, int N, int MODE, bool BIAS, bool GATE, bool EXACT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_kernel(const BlockNormParams p) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
+    typedef Piece<TPR, EXACT> P;
+    constexpr bool HAS_Y = MODE == 2 || GATE;
     __shared__ float lds[2][2][TPR / 64 + 1];
-    __shared__ float meet[GROUPS > 1 ? GROUPS * TPR * N * 4 : 1];
+    __shared__ f32x4 meet[GROUPS > 1 ? GROUPS * TPR * N : 1];
     int turn = 0;
-    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    const int lane = threadIdx.x % TPR, group = row_group<TPR>(), dim = p.dim;
     constexpr f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 acc_w[N], acc_b[BIAS ? N : 1], acc_pw[MODE == 2 ? N : 1], acc_pb[MODE == 2 && BIAS ? N : 1], acc_g[GATE ? N : 1];
 #pragma unroll
@@ -219,135 +326,146 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
         if constexpr (MODE == 2 && BIAS) acc_pb[n] = zero;
         if constexpr (GATE) acc_g[n] = zero;
     }
-    // segments of rows: with `flush` the gate groups of this chunk that this group of threads takes, else one
+    // this group's rows: r, r + step ... below r_end.  With `flush` they are whole gate groups, and gate_row counts them;
+    // else all have the same gate row
     const long long chunk = blockIdx.x;
-    long long seg = chunk, seg_end = chunk + 1, seg_step = 1;
+    long long r, r_end, gate_row;
+    int step = 1;
     if (p.flush) {
-        seg = chunk * p.groups_per_chunk;
-        seg_end = seg + p.groups_per_chunk < p.gate_groups ? seg + p.groups_per_chunk : p.gate_groups;
-        seg += group, seg_step = GROUPS;
+        const int each = p.groups_per_chunk / GROUPS;  // a multiple
+        gate_row = chunk * p.groups_per_chunk + group * each;
+        r = gate_row * p.rows_per_group, r_end = r + each * p.rows_per_group;
+        if (r_end > p.rows) r_end = p.rows;
+    } else {
+        gate_row = chunk / p.chunks_per_group;
+        r_end = (gate_row + 1) * p.rows_per_group < p.rows ? (gate_row + 1) * p.rows_per_group : p.rows;
+        r = gate_row * p.rows_per_group + (chunk - gate_row * p.chunks_per_group) * p.rows_per_chunk;
+        if (r + p.rows_per_chunk < r_end) r_end = r + p.rows_per_chunk;
+        r += group, step = GROUPS;
     }
-    for (; seg < seg_end; seg += seg_step) {
-        long long r, r_end, r_step;
-        if (p.flush) {
-            r = seg * p.rows_per_group, r_step = 1;
-            r_end = r + p.rows_per_group < p.rows ? r + p.rows_per_group : p.rows;
-        } else {
-            const long long g = chunk / p.chunks_per_group, part = chunk % p.chunks_per_group;
-            const long long g_end = (g + 1) * p.rows_per_group < p.rows ? (g + 1) * p.rows_per_group : p.rows;
-            r = g * p.rows_per_group + part * p.rows_per_chunk;
-            r_end = r + p.rows_per_chunk < g_end ? r + p.rows_per_chunk : g_end;
-            r += group, r_step = GROUPS;
+    long long left_in_group = p.rows_per_group;
+    const bool gate_in_rows = p.gate_rows != 0;
+
+    // what the norm ahead of the next block needs of a row, and what the norm behind this one needs: the first part of the
+    // next row and the second part of this one are under way while the other is worked on
+    struct Ahead {
+        raw4<TS> u[N], du[N];
+        raw4<TB> dh[N];
+        float mean, rstd;
+    } ahead = {};
+    struct Behind {
+        raw4<TB> y[HAS_Y ? N : 1], g[GATE ? N : 1];
+        float mean, rstd;
+    };
+    auto fetch_ahead = [&](long long row) {
+        if (p.dh != nullptr) {
+            ahead.mean = p.pre_s[2 * row], ahead.rstd = p.pre_s[2 * row + 1];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                ahead.u[n] = P::load(static_cast<const TS*>(p.u) + row * p.ld_u, n, lane, dim);
+                ahead.dh[n] = P::load(static_cast<const TB*>(p.dh) + row * p.ld_h, n, lane, dim);
+            }
         }
-        for (; r < r_end; r += r_step) {
-            f32x4 t[N], hat[N];
+        if (p.du != nullptr)
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+                ahead.du[n] = P::load(static_cast<const TS*>(p.du) + row * p.ld_u, n, lane, dim);
+    };
+    if (r < r_end) fetch_ahead(r);
+    for (; r < r_end; r += step) {
+        const bool last_of_group = p.flush && (left_in_group == 1 || r + step >= r_end);
+        Behind now = {};
+        if constexpr (HAS_Y)
+#pragma unroll
+            for (int n = 0; n < N; ++n) now.y[n] = P::load(static_cast<const TB*>(p.y) + r * p.ld_y, n, lane, dim);
+        if constexpr (MODE == 2) now.mean = p.post_s[2 * r], now.rstd = p.post_s[2 * r + 1];
+        if constexpr (GATE)
+            if (gate_in_rows)
+#pragma unroll
+                for (int n = 0; n < N; ++n)
+                    now.g[n] = P::load(static_cast<const TB*>(p.gate) + gate_row * p.ld_gate, n, lane, dim);
+        f32x4 t[N], hat[N];
+        if (p.dh != nullptr) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int c = 4 * (n * TPR + lane);
-                t[n] = zero;
-                if (p.du != nullptr && c < p.dim) t[n] = load4(static_cast<const TS*>(p.du) + r * p.ld_u, c, p.dim, p.whole);
+                    const f32x4 dh = widen(ahead.dh[n]);
+                hat[n] = (widen(ahead.u[n]) - ahead.mean) * ahead.rstd;
+                acc_w[n] += dh * hat[n];
+                if constexpr (BIAS) acc_b[n] += dh;
+                t[n] = dh * P::vector(p.pre_w, n, lane, dim, 1.0f);
             }
-            if (p.dh != nullptr) {
-                f32x4 a[N];
-                const float mean = p.pre_s[2 * r], rstd = p.pre_s[2 * r + 1];
+            row_gradient<TPR, N>(t, hat, p.pre, ahead.rstd, p, lds, turn);
+            if (p.du != nullptr)
 #pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const int c = 4 * (n * TPR + lane);
-                    a[n] = hat[n] = zero;
-                    if (c < p.dim) {
-                        const f32x4 dh = load4(static_cast<const TB*>(p.dh) + r * p.ld_h, c, p.dim, p.whole);
-                        hat[n] = (load4(static_cast<const TS*>(p.u) + r * p.ld_u, c, p.dim, p.whole) - mean) * rstd;
-                        acc_w[n] += dh * hat[n];
-                        if constexpr (BIAS) acc_b[n] += dh;
-                        a[n] = dh * vector4(p.pre_w, c, p, 1.0f);
-                    }
-                }
-                row_gradient<TPR, N>(a, hat, p.pre, rstd, p, lds, turn);
+                for (int n = 0; n < N; ++n) t[n] += widen(ahead.du[n]);
+        } else {
 #pragma unroll
-                for (int n = 0; n < N; ++n) t[n] += a[n];
-            }
+            for (int n = 0; n < N; ++n) t[n] = widen(ahead.du[n]);
+        }
+        if (r + step < r_end) fetch_ahead(r + step);
+#pragma unroll
+        for (int n = 0; n < N; ++n) P::store(static_cast<TS*>(p.dx) + r * p.ld_x, n, lane, dim, t[n]);
+        if constexpr (MODE > 0) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                const int c = 4 * (n * TPR + lane);
-                if (c < p.dim) store4(static_cast<TS*>(p.dx) + r * p.ld_x, c, p.dim, p.whole, t[n]);
-            }
-            if constexpr (MODE > 0) {
-                float mean = 0.0f, rstd = 1.0f;
-                if constexpr (MODE == 2) mean = p.post_s[2 * r], rstd = p.post_s[2 * r + 1];
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const int c = 4 * (n * TPR + lane);
-                    t[n] *= p.scale;
-                    if (c >= p.dim) {
-                        t[n] = hat[n] = zero;
-                        continue;
-                    }
-                    if constexpr (MODE == 2 || GATE) {
-                        const f32x4 y = load4(static_cast<const TB*>(p.y) + r * p.ld_y, c, p.dim, p.whole);
-                        hat[n] = MODE == 2 ? (y - mean) * rstd : y;
-                    }
-                    f32x4 w;
-                    if constexpr (MODE == 2) w = vector4(p.post_w, c, p, 1.0f);
-                    if constexpr (GATE) {
-                        const f32x4 g = gate4<TB>(p, r, c);
-                        f32x4 v = hat[n];
-                        if constexpr (MODE == 2) v = v * w + vector4(p.post_b, c, p, 0.0f);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float q = gate_value(g[j], p.act);
-                            acc_g[n][j] += t[n][j] * v[j] * gate_slope(q, p.act);
-                            t[n][j] *= q;
-                        }
-                    }
-                    if constexpr (MODE == 2) {
-                        acc_pw[n] += t[n] * hat[n];
-                        if constexpr (BIAS) acc_pb[n] += t[n];
-                        t[n] *= w;
-                    }
+                    t[n] = P::cut(t[n] * p.scale, n, lane, dim);
+                if constexpr (HAS_Y) {
+                    hat[n] = widen(now.y[n]);
+                    if constexpr (MODE == 2) hat[n] = (hat[n] - now.mean) * now.rstd;
                 }
-                if constexpr (MODE == 2) row_gradient<TPR, N>(t, hat, p.post, rstd, p, lds, turn);
-#pragma unroll
-                for (int n = 0; n < N; ++n) {
-                    const int c = 4 * (n * TPR + lane);
-                    if (c < p.dim) store4(static_cast<TB*>(p.dy) + r * p.ld_y, c, p.dim, p.whole, t[n]);
+                f32x4 w;
+                if constexpr (MODE == 2) w = P::vector(p.post_w, n, lane, dim, 1.0f);
+                if constexpr (GATE) {
+                    f32x4 v = hat[n], g;
+                    if constexpr (MODE == 2) v = v * w + P::vector(p.post_b, n, lane, dim, 0.0f);
+                    if (gate_in_rows)
+                        g = widen(now.g[n]);
+                    else
+                        g = P::load(static_cast<const float*>(p.gate), n, lane, dim);
+                    const f32x4 q = gate_values(g, p.act);
+                    acc_g[n] += t[n] * v * gate_slopes(q, p.act);
+                    t[n] *= q;
+                }
+                if constexpr (MODE == 2) {
+                    acc_pw[n] += t[n] * hat[n];
+                    if constexpr (BIAS) acc_pb[n] += t[n];
+                    t[n] *= w;
                 }
             }
+            if constexpr (MODE == 2) row_gradient<TPR, N>(t, hat, p.post, now.rstd, p, lds, turn);
+#pragma unroll
+            for (int n = 0; n < N; ++n) P::store(static_cast<TB*>(p.dy) + r * p.ld_y, n, lane, dim, t[n]);
         }
         if constexpr (GATE) {
-            if (p.flush) {  // the whole group's rows are in
-                if (p.d_gate != nullptr) {
+            if (last_of_group) {  // the group's rows are in
+                if (p.d_gate != nullptr)
 #pragma unroll
-                    for (int n = 0; n < N; ++n) {
-                        const int c = 4 * (n * TPR + lane);
-                        if (c < p.dim) store4(static_cast<TB*>(p.d_gate) + seg * p.ld_gate, c, p.dim, p.whole, acc_g[n]);
-                    }
-                }
+                    for (int n = 0; n < N; ++n)
+                        P::store(static_cast<TB*>(p.d_gate) + gate_row * p.ld_gate, n, lane, dim, acc_g[n]);
 #pragma unroll
                 for (int n = 0; n < N; ++n) acc_g[n] = zero;
             }
         }
+        if (last_of_group) ++gate_row;
+        left_in_group = last_of_group ? p.rows_per_group : left_in_group - 1;
     }
     // the column sums of the chunk; groups of threads that share the columns meet in LDS
     auto put = [&](const f32x4* acc, int slot) {
         if (slot < 0) return;  // the same for the whole launch
-        float* out = p.partial + ((long long)slot * p.chunks + chunk) * p.dim;
-        const bool whole = (p.dim & 3) == 0;
+        float* out = p.partial + ((long long)slot * p.chunks + chunk) * dim;
         if constexpr (GROUPS > 1) {
             __syncthreads();
 #pragma unroll
-            for (int n = 0; n < N; ++n) *reinterpret_cast<f32x4*>(&meet[(group * TPR * N + n * TPR + lane) * 4]) = acc[n];
+            for (int n = 0; n < N; ++n) meet[(group * N + n) * TPR + lane] = acc[n];
             __syncthreads();
             for (int k = threadIdx.x; k < TPR * N; k += NT) {
-                f32x4 s = *reinterpret_cast<f32x4*>(&meet[k * 4]);
-                for (int g = 1; g < GROUPS; ++g) s += *reinterpret_cast<f32x4*>(&meet[(g * TPR * N + k) * 4]);
-                if (4 * k < p.dim) store4(out, 4 * k, p.dim, whole, s);
+                f32x4 s = meet[k];
+                for (int g = 1; g < GROUPS; ++g) s += meet[g * TPR * N + k];
+                P::store(out, k / TPR, k % TPR, dim, s);
             }
         } else {
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
-                const int c = 4 * (n * TPR + lane);
-                if (c < p.dim) store4(out, c, p.dim, whole, acc[n]);
-            }
+            for (int n = 0; n < N; ++n) P::store(out, n, lane, dim, acc[n]);
         }
     };
     put(acc_w, p.slot[0]);

@@ -37,7 +37,6 @@ struct EmbeddingParams {
     int vocabulary, dim;
     int padding;      // id whose tokens add nothing to the gradient, or -1
     float scale;
-    int whole;        // rows of `in` and `out` can be accessed four elements at a time
     int lanes_log2;   // threads per row of a workgroup of 256
     int accumulate;   // gradient: dW += instead of dW =
     int sort_blocks, sort_log2;  // buckets of the sort, a power of two
@@ -65,16 +64,16 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         id[r] = t0 + r < p.tokens ? token_id(static_cast<const ID*>(p.ids), t0 + r, p.vocabulary) : -1;
-    typename Raw4<TIN>::type v[ROWS];
+    raw4<TIN> v[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        v[r] = typename Raw4<TIN>::type{};
-        if (id[r] >= 0) v[r] = load4_raw(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in, c, p.dim, p.whole);
+        v[r] = raw4<TIN>{};
+        if (id[r] >= 0) v[r] = load4(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in + c, p.dim - c);
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         if (t0 + r < p.tokens)
-            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out, c, p.dim, p.whole, widen(v[r]) * p.scale);
+            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out + c, p.dim - c, widen(v[r]) * p.scale);
 }
 
 // The sort.  Ids are dealt out to the workgroups of embedding_sort_kernel in turn (words come by frequency in most
@@ -259,15 +258,27 @@ __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const Embed
     const int* from = p.piece_start + (long long)(rank >> p.fine_log2) * p.pieces;
     const int* to = from + p.pieces;
     int smaller = 0;
-    // all tokens of the pieces' lists, up to 64 pieces' bounds at a time in the lanes
+    // All tokens of the pieces' lists: the bounds of up to 64 pieces in the lanes, their lengths summed up, and lane by lane
+    // the piece that the next token is in.  (A piece has a handful of tokens of a bucket: a turn for each would wait for
+    // memory as often as there are pieces.)
     auto walk = [&](auto&& visit) {
         for (int i0 = begin; i0 < end; i0 += 64) {
-            const int a_of = i0 + lane < end ? from[i0 + lane] : 0, b_of = i0 + lane < end ? to[i0 + lane] : 0;
-            const int here = end - i0 < 64 ? end - i0 : 64;
-            for (int i = 0; i < here; ++i) {
-                const int a = __shfl(a_of, i, 64), b = __shfl(b_of, i, 64);
-                const long long base = (long long)(i0 + i) * kPiece;
-                for (int k = a; k < b; k += 64) visit(base + k + lane, k + lane < b);
+            const int a = i0 + lane < end ? from[i0 + lane] : 0, length = i0 + lane < end ? to[i0 + lane] - a : 0;
+            int upto = length;
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) {
+                const int o = __shfl_up(upto, off, 64);
+                if (lane >= off) upto += o;
+            }
+            const int all = __shfl(upto, 63, 64);
+            for (int k = 0; k < all; k += 64) {
+                const int q = k + lane;
+                int piece = 0;  // the first whose `upto` is above q
+#pragma unroll
+                for (int half = 32; half > 0; half >>= 1)
+                    if (__shfl(upto, piece + half - 1, 64) <= q) piece += half;
+                const int at = q - (__shfl(upto, piece & 63, 64) - __shfl(length, piece & 63, 64)) + __shfl(a, piece & 63, 64);
+                visit((long long)(i0 + (piece & 63)) * kPiece + at, q < all);
             }
         }
     };
@@ -301,10 +312,10 @@ __device__ __forceinline__ int id_of_key(const EmbeddingParams& p, int key) {
 
 __device__ __forceinline__ void put_gradient(const EmbeddingParams& p, int key, int c, f32x4 sum) {
     const int id = id_of_key(p, key);
-    float* row = static_cast<float*>(p.out) + (long long)id * p.ld_out;
+    float* row = static_cast<float*>(p.out) + (long long)id * p.ld_out + c;
     sum *= p.scale;
-    if (p.accumulate) sum += load4(row, c, p.dim, p.whole);
-    store4(row, c, p.dim, p.whole, sum);
+    if (p.accumulate) sum += load4(row, p.dim - c);
+    store4(row, p.dim - c, sum);
 }
 
 // A group of threads adds up `chunk` consecutive sorted tokens, U rows of dy under way at a time.  A run of equal ids that
@@ -317,6 +328,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     const int groups = 256 >> p.lanes_log2;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
+    const int left = p.dim - c;
     const int keys = p.sort_blocks * p.bins;
     if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has
         constexpr int ROWS = 8;
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
         }
 #pragma unroll
         for (int k = 0; k < ROWS; ++k)
-            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out, c, p.dim, p.whole, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         return;
     }
     const long long k = (long long)blockIdx.x * groups + group;
@@ -341,13 +353,12 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     const long long p0 = k * p.chunk;
     if (p0 >= n) return;
     const long long p1 = p0 + p.chunk < n ? p0 + p.chunk : n;
-    const T* dy = static_cast<const T*>(p.in);
+    const T* dy = static_cast<const T*>(p.in) + c;
     int cur = p.sorted[p0];
     bool came_in = p0 > 0 && p.sorted[p0 - 1] == cur;
     const bool goes_on = p1 < n && p.sorted[p1] == p.sorted[p1 - 1];
     f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    float* slot = p.partial + 2 * k * p.dim;
-    const bool whole_slot = (p.dim & 3) == 0;
+    float* slot = p.partial + 2 * k * p.dim + c;
     int key[U], token[U];
     auto fetch = [&](long long q) {  // behind the chunk's end: its last token again
 #pragma unroll
@@ -358,11 +369,11 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     };
     fetch(p0);
     for (long long q = p0; q < p1; q += U) {
-        typename Raw4<T>::type v[U];
+        raw4<T> v[U];
         int now[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            v[j] = load4_raw(dy + (long long)token[j] * p.ld_in, c, p.dim, p.whole);
+            v[j] = load4(dy + (long long)token[j] * p.ld_in, left);
             now[j] = q + j < p1 ? key[j] : -1;
         }
         if (q + U < p1) fetch(q + U);
@@ -371,7 +382,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
             if (now[j] < 0) continue;
             if (now[j] != cur) {  // the run before has ended
                 if (came_in)
-                    store4(slot, c, p.dim, whole_slot, sum);
+                    store4(slot, left, sum);
                 else
                     put_gradient(p, cur, c, sum);
                 came_in = false;
@@ -383,9 +394,9 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
         }
     }
     if (came_in)
-        store4(slot, c, p.dim, whole_slot, sum);
+        store4(slot, left, sum);
     else if (goes_on)
-        store4(slot + p.dim, c, p.dim, whole_slot, sum);
+        store4(slot + p.dim, left, sum);
     else
         put_gradient(p, cur, c, sum);
 }
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
 // The rows whose run crosses the end of a chunk: the group of the chunk where the run starts adds its part and those of the
 // chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).
 __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingParams p) {
-    constexpr int U = 8;
+    constexpr int U = 32;
     const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
     const int groups = 256 >> p.lanes_log2;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
@@ -405,15 +416,15 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
     const int key = p.sorted[last];
     if (p.sorted[last + 1] != key || p.offsets[key] < k * p.chunk) return;
     const long long k_end = (p.offsets[key + 1] - 1) / p.chunk;
-    const bool whole_slot = (p.dim & 3) == 0;
-    const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim, c, p.dim, whole_slot);
+    const int left = p.dim - c;
+    const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim + c, left);
     double sum[4] = {first[0], first[1], first[2], first[3]};
     for (long long q = k + 1; q <= k_end; q += U) {
         f32x4 v[U];
 #pragma unroll
         for (int j = 0; j < U; ++j) {
             v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (q + j <= k_end) v[j] = load4(p.partial + 2 * (q + j) * p.dim, c, p.dim, whole_slot);
+            if (q + j <= k_end) v[j] = load4(p.partial + 2 * (q + j) * p.dim + c, left);
         }
 #pragma unroll
         for (int j = 0; j < U; ++j)

@@ -48,9 +48,6 @@ EmbeddingParams embedding_params(const snhip_embedding_desc* d, const void* ids,
     const long long ldt = d->ld_table != 0 ? d->ld_table : d->dim, ldo = d->ld_output != 0 ? d->ld_output : d->dim;
     p.ld_in = backward ? ldo : ldt, p.ld_out = backward ? ldt : ldo;
     p.padding = backward && d->padding_index < d->vocabulary ? d->padding_index : -1;
-    const int in_type = backward ? d->output_type : d->table_type, out_type = backward ? SNHIP_TYPE_F32 : d->output_type;
-    p.whole = d->dim % 4 == 0 && ldt % 4 == 0 && ldo % 4 == 0 && aligned(in, 4 * type_bytes(in_type)) &&
-              aligned(out, 4 * type_bytes(out_type));
     const int units = ceil_div(d->dim, 4);
     p.lanes_log2 = 3;
     while (p.lanes_log2 < 8 && (1 << p.lanes_log2) < units) ++p.lanes_log2;
@@ -212,11 +209,13 @@ BlockNormParams block_norm_params(const snhip_block_norm_desc* d) {
     p.ld_h = d->ld_h ? d->ld_h : d->dim, p.ld_gate = d->ld_gate ? d->ld_gate : d->dim;
     p.pre = d->pre_norm, p.post = d->post_norm, p.act = d->gate_activation;
     p.eps = d->epsilon, p.scale = d->residual_scale, p.inv_dim = 1.0f / (float)(d->dim > 0 ? d->dim : 1);
-    const size_t sb = 4 * type_bytes(d->stream_type), bb = 4 * type_bytes(d->block_type), gb = d->gate_rows == 0 ? 16 : bb;
-    p.whole = p.dim % 4 == 0 && p.ld_x % 4 == 0 && p.ld_y % 4 == 0 && p.ld_u % 4 == 0 && p.ld_h % 4 == 0 && p.ld_gate % 4 == 0 &&
-              aligned(d->x, sb) && aligned(d->u, sb) && aligned(d->du, sb) && aligned(d->dx, sb) && aligned(d->y, bb) &&
-              aligned(d->h, bb) && aligned(d->dh, bb) && aligned(d->dy, bb) && aligned(d->gate, gb) && aligned(d->d_gate, gb) &&
-              aligned(d->pre_weight, 16) && aligned(d->pre_bias, 16) && aligned(d->post_weight, 16) && aligned(d->post_bias, 16);
+    // four bf16 in one access need a 4-byte address; fp32 rows always have one
+    const bool block_ok = d->block_type == SNHIP_TYPE_F32 ||
+                          (p.ld_y % 2 == 0 && p.ld_h % 2 == 0 && p.ld_gate % 2 == 0 && aligned(d->y, 4) && aligned(d->h, 4) &&
+                           aligned(d->dh, 4) && aligned(d->dy, 4) && aligned(d->gate, 4) && aligned(d->d_gate, 4));
+    const bool stream_ok = d->stream_type == SNHIP_TYPE_F32 || (p.ld_x % 2 == 0 && p.ld_u % 2 == 0 && aligned(d->x, 4) &&
+                                                                aligned(d->u, 4) && aligned(d->du, 4) && aligned(d->dx, 4));
+    p.exact = p.dim % 4 == 0 && block_ok && stream_ok;
     return p;
 }
 
@@ -260,7 +259,7 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
         if (t.count < 0 || !is_storage_type(t.gradient_type) || !isfinite(t.weight_decay)) return SNHIP_STATUS_INVALID_VALUE;
         AdamwEntry& e = entries[(size_t)k];
         e = AdamwEntry{t.parameter, t.gradient, t.moment1, t.moment2, t.scale1, t.scale2, static_cast<__bf16*>(t.bf16_copy),
-                       t.count, chunks, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16, 0};
+                       t.count, chunks, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16};
         if (t.count == 0) continue;
         const size_t gb = type_bytes(t.gradient_type);
         if (t.parameter == nullptr || t.gradient == nullptr || t.moment1 == nullptr || t.moment2 == nullptr ||
@@ -269,8 +268,6 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
         if (!aligned(t.parameter, 4) || !aligned(t.gradient, gb) || !aligned(t.moment1, sb) || !aligned(t.moment2, sb) ||
             !aligned(t.bf16_copy, 2))
             return SNHIP_STATUS_INVALID_VALUE;
-        e.whole = aligned(t.parameter, 16) && aligned(t.gradient, 4 * gb) && aligned(t.moment1, 4 * sb) &&
-                  aligned(t.moment2, 4 * sb) && aligned(t.bf16_copy, 8);
         const size_t n = (size_t)t.count, blocks = (n + kAdamwBlock - 1) / kAdamwBlock;
         auto add = [&ranges](const void* p, size_t bytes, bool written) {
             const uintptr_t b = reinterpret_cast<uintptr_t>(p);

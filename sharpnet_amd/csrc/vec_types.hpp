@@ -1,4 +1,4 @@
-// Loads and stores of the row operators: four consecutive elements of a row at a time, fp32 or bf16 in memory, fp32 in
+// Loads, stores and sums of the row operators: four consecutive elements of a row at a time, fp32 or bf16 in memory, fp32 in
 // registers.
 #pragma once
 #include <hip/hip_runtime.h>
@@ -7,61 +7,83 @@ namespace snhip {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+// the same at any address of an element: the hardware takes wide accesses there, a row may start anywhere
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef bf16x4 bf16x4_any __attribute__((aligned(2)));
 
 template <typename T>
 struct Raw4;  // four elements as they lie in memory
 template <>
 struct Raw4<float> {
     typedef f32x4 type;
+    typedef f32x4_any any;
 };
 template <>
 struct Raw4<__bf16> {
     typedef bf16x4 type;
+    typedef bf16x4_any any;
 };
-
-// Elements [c, c + 4) of a row of `cols`; `whole`: the row starts on four elements' alignment and cols is a multiple of
-// four, so the piece is one 16- or 8-byte access; otherwise element by element, zeros behind the row's end.
-// As they lie in memory: nothing is done with them in the branch, so nothing waits for them there and the loads of several
-// rows are under way together (a conversion beside each load costs half the bandwidth).
 template <typename T>
-__device__ __forceinline__ typename Raw4<T>::type load4_raw(const T* row, int c, int cols, bool whole) {
-    typedef typename Raw4<T>::type raw;
-    if (whole) return *reinterpret_cast<const raw*>(row + c);
-    raw v = {(T)0.0f, (T)0.0f, (T)0.0f, (T)0.0f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < cols) v[j] = row[c + j];
-    return v;
-}
+using raw4 = typename Raw4<T>::type;
+
 __device__ __forceinline__ f32x4 widen(f32x4 v) { return v; }
 __device__ __forceinline__ f32x4 widen(bf16x4 v) { return __builtin_convertvector(v, f32x4); }
-template <typename T>
-__device__ __forceinline__ f32x4 load4(const T* row, int c, int cols, bool whole) {
-    return widen(load4_raw(row, c, cols, whole));
-}
-__device__ __forceinline__ void store4(float* row, int c, int cols, bool whole, f32x4 v) {
-    if (whole) {
-        *reinterpret_cast<f32x4*>(row + c) = v;
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < cols) row[c + j] = v[j];
-}
-// (the conversion rounds to nearest even)
-__device__ __forceinline__ void store4(__bf16* row, int c, int cols, bool whole, f32x4 v) {
-    if (whole) {
-        *reinterpret_cast<bf16x4*>(row + c) = __builtin_convertvector(v, bf16x4);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (c + j < cols) row[c + j] = (__bf16)v[j];
-}
+// (rounds to nearest even)
+__device__ __forceinline__ f32x4 narrow(f32x4 v, const float*) { return v; }
+__device__ __forceinline__ bf16x4 narrow(f32x4 v, const __bf16*) { return __builtin_convertvector(v, bf16x4); }
 // v as it reads back after a store in type T
-__device__ __forceinline__ f32x4 as_stored(f32x4 v, const float*) { return v; }
-__device__ __forceinline__ f32x4 as_stored(f32x4 v, const __bf16*) {
-    return __builtin_convertvector(__builtin_convertvector(v, bf16x4), f32x4);
+template <typename T>
+__device__ __forceinline__ f32x4 as_stored(f32x4 v) {
+    return widen(narrow(v, static_cast<const T*>(nullptr)));
+}
+
+// Four whole elements from `at` on.  The loads return them as they lie in memory: a conversion beside each load would wait
+// for it, and the loads of several rows would not be under way together (half the bandwidth).
+template <typename T>
+__device__ __forceinline__ raw4<T> load4_whole(const T* at) {
+    return *reinterpret_cast<const typename Raw4<T>::any*>(at);
+}
+template <typename T>
+__device__ __forceinline__ void store4_whole(T* at, f32x4 v) {
+    *reinterpret_cast<typename Raw4<T>::any*>(at) = narrow(v, static_cast<const T*>(nullptr));
+}
+// The same for a piece of which `left` elements exist (0 or less: none): one access, or element by element at a row's end;
+// what does not exist reads as zero.
+template <typename T>
+__device__ __forceinline__ raw4<T> load4(const T* at, int left) {
+    if (left >= 4) return load4_whole(at);
+    raw4<T> v = {};
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < left) v[j] = at[j];
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* at, int left, f32x4 v) {
+    if (left >= 4) return store4_whole(at, v);
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+        if (j < left) at[j] = (T)v[j];
+}
+
+// Sums over 16 neighbouring lanes / over the wavefront, in every lane of them, without going through LDS: rotations within
+// rows of 16 lanes are free operands of the additions (ds_bpermute, what a shuffle becomes, is a round trip each).
+template <int ROTATE>
+__device__ __forceinline__ float add_rotated(float v) {
+    constexpr int row_ror = 0x120;
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), row_ror + ROTATE, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+    v = add_rotated<8>(v);
+    v = add_rotated<4>(v);
+    v = add_rotated<2>(v);
+    return add_rotated<1>(v);
+}
+__device__ __forceinline__ float wave64_sum(float v) {
+    const int r = __float_as_int(row16_sum(v));
+    const float a = __int_as_float(__builtin_amdgcn_readlane(r, 0)), b = __int_as_float(__builtin_amdgcn_readlane(r, 16));
+    const float c = __int_as_float(__builtin_amdgcn_readlane(r, 32)), d = __int_as_float(__builtin_amdgcn_readlane(r, 48));
+    return (a + b) + (c + d);
 }
 
 }  // namespace snhip
