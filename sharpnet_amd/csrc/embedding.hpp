@@ -5,8 +5,8 @@
 //
 // Both are bound by HBM.  The gradient is built without float atomics, in an order that depends on the ids alone, so its
 // bits repeat: the tokens are sorted by id (embedding_sort_kernel), runs of equal ids are added up in chunks of the sorted
-// order (embedding_grad_kernel, which also clears the rows that no token has), and runs that cross a chunk's end are
-// joined from their chunks' sums (embedding_join_kernel).
+// order (embedding_grad_kernel), and runs that cross a chunk's end are joined from their chunks' sums
+// (embedding_join_kernel, which also clears the rows that no token has).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -43,12 +43,14 @@ struct EmbeddingParams {
     int fine_log2;               // ... over 256 of them: 2^fine_log2 times 256
     int bins, bins_log2;         // ids of each (at most 512), and the bits that number them
     int chunk;        // sorted tokens per group of threads of the gradient
-    long long chunk_blocks;  // workgroups that add up chunks; those behind them clear rows without tokens
+    long long chunk_blocks;  // workgroups that add up or join chunks; those behind them clear rows without tokens
     int* order;       // [tokens]: token numbers, sorted by key (see embedding_sort_kernel)
     int* sorted;      // [tokens]: their ids' keys
     int* offsets;     // [sort_blocks * bins + 1]: where each key's run starts in `order`
     int pieces;       // of embedding_bucket_kernel
     int *piece_id, *piece_token, *piece_start;
+    long long chunks;
+    int* crossing;    // [chunks][2]: key of the run that starts in the chunk and goes on behind it (or -1), its last chunk
     float* partial;   // [chunks][2][dim]: sums of the runs that came into a chunk / went on behind it
 };
 
@@ -81,10 +83,10 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 // rank * bins + i / B with the
 // buckets ranked by i % 256 first.  The workgroup of a bucket finds its tokens in the order of their positions, a contiguous part to
 // each of its 16 wavefronts, and counts them by wavefront and id in LDS; after a scan over (id, wavefront) every wavefront
-// puts its tokens behind the earlier ones of their ids.  The order within an id is that of the positions.
+// puts its tokens behind the earlier ones of their ids.  The order of all this is a function of the ids alone.
 // Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (6.6 us for 4000 tokens).
 // With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup reads its own alone
-// (65536 tokens: 34 us the first way, MEASURED the second).
+// (65536 tokens: 34 us the first way, 22 us the second).
 constexpr int kSortDirect = 8192; // tokens up to which every workgroup reads all ids
 constexpr int kPiece = 1024;      // tokens that a workgroup of embedding_bucket_kernel sorts
 constexpr int kBuckets = 256;     // ... by bucket (bucket modulo 256 if there are more)
@@ -250,7 +252,7 @@ __global__ void __launch_bounds__(1024) embedding_sort_kernel(const EmbeddingPar
 __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const EmbeddingParams p) {
     extern __shared__ int count[];  // [16][bins], then the cursors
     __shared__ int below[16], wave_total[16];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, rank = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), rank = blockIdx.x;
     for (int i = tid; i < 16 * p.bins; i += 1024) count[i] = 0;
     __syncthreads();
     const int per = (p.pieces + 15) / 16;
@@ -258,34 +260,36 @@ __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const Embed
     const int* from = p.piece_start + (long long)(rank >> p.fine_log2) * p.pieces;
     const int* to = from + p.pieces;
     int smaller = 0;
-    // All tokens of the pieces' lists: the bounds of up to 64 pieces in the lanes, their lengths summed up, and lane by lane
-    // the piece that the next token is in.  (A piece has a handful of tokens of a bucket: a turn for each would wait for
-    // memory as often as there are pieces.)
-    auto walk = [&](auto&& visit) {
-        for (int i0 = begin; i0 < end; i0 += 64) {
-            const int a = i0 + lane < end ? from[i0 + lane] : 0, length = i0 + lane < end ? to[i0 + lane] - a : 0;
-            int upto = length;
+    // All tokens of the pieces' lists, eight pieces at a time: a piece has a handful of tokens of a bucket, and one after the
+    // other each would wait for memory.
+    auto walk = [&](bool tokens, auto&& visit) {
+        constexpr int U = 8;
+        for (int i0 = begin; i0 < end; i0 += U) {
+            int a[U], b[U], longest = 0;
 #pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int o = __shfl_up(upto, off, 64);
-                if (lane >= off) upto += o;
+            for (int j = 0; j < U; ++j) {
+                const int i = i0 + j < end ? i0 + j : end - 1;
+                a[j] = from[i], b[j] = i0 + j < end ? to[i] : 0;
+                longest = b[j] - a[j] > longest ? b[j] - a[j] : longest;
             }
-            const int all = __shfl(upto, 63, 64);
-            for (int k = 0; k < all; k += 64) {
-                const int q = k + lane;
-                int piece = 0;  // the first whose `upto` is above q
+            for (int k = 0; k < longest; k += 64) {
+                int id[U], token[U];
 #pragma unroll
-                for (int half = 32; half > 0; half >>= 1)
-                    if (__shfl(upto, piece + half - 1, 64) <= q) piece += half;
-                const int at = q - (__shfl(upto, piece & 63, 64) - __shfl(length, piece & 63, 64)) + __shfl(a, piece & 63, 64);
-                visit((long long)(i0 + (piece & 63)) * kPiece + at, q < all);
+                for (int j = 0; j < U; ++j) {
+                    const int at = a[j] + k + lane;
+                    const long long place = (long long)(i0 + j) * kPiece + at;
+                    id[j] = at < b[j] ? p.piece_id[place] : -1;
+                    token[j] = tokens && at < b[j] ? p.piece_token[place] : 0;
+                }
+#pragma unroll
+                for (int j = 0; j < U; ++j) visit(id[j], token[j]);
             }
         }
     };
     for (int i = begin + lane; i < end; i += 64) smaller += from[i];
-    walk([&](long long at, bool in) {
-        if (!in) return;
-        const int id = p.piece_id[at], r = rank_of_id(p, id);
+    walk(false, [&](int id, int) {
+        if (id < 0) return;
+        const int r = rank_of_id(p, id);
         if (r == rank)
             atomicAdd(&count[w * p.bins + (id >> p.sort_log2)], 1);
         else
@@ -296,12 +300,12 @@ __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const Embed
     if (lane == 0) below[w] = smaller;
     __syncthreads();
     start_ids(p, count, below, wave_total);
-    walk([&](long long from_at, bool in) {
-        const int id = in ? p.piece_id[from_at] : -1;
-        in = in && rank_of_id(p, id) == rank;
+    walk(true, [&](int id, int token) {
+        const bool in = id >= 0 && rank_of_id(p, id) == rank;
+        if (__ballot(in) == 0) return;
         const int number = in ? id >> p.sort_log2 : 0;
         const int at = take_place(in, number, p.bins_log2, count + w * p.bins);
-        if (in) p.order[at] = p.piece_token[from_at], p.sorted[at] = rank * p.bins + number;
+        if (in) p.order[at] = token, p.sorted[at] = rank * p.bins + number;
     });
 }
 
@@ -330,28 +334,13 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     if (c >= p.dim) return;
     const int left = p.dim - c;
     const int keys = p.sort_blocks * p.bins;
-    if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has
-        constexpr int ROWS = 8;
-        const long long r0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * ROWS;
-        bool clear[ROWS];
-#pragma unroll
-        for (int k = 0; k < ROWS; ++k) {
-            const int r = (int)(r0 + k);
-            clear[k] = r0 + k < p.vocabulary;
-            if (clear[k]) {
-                const int key = rank_of_id(p, r) * p.bins + (r >> p.sort_log2);
-                clear[k] = p.offsets[key] == p.offsets[key + 1];
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < ROWS; ++k)
-            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-        return;
-    }
     const long long k = (long long)blockIdx.x * groups + group;
     const long long n = p.offsets[keys];
     const long long p0 = k * p.chunk;
-    if (p0 >= n) return;
+    if (p0 >= n) {
+        if (c == 0 && k < p.chunks) p.crossing[2 * k] = -1;
+        return;
+    }
     const long long p1 = p0 + p.chunk < n ? p0 + p.chunk : n;
     const T* dy = static_cast<const T*>(p.in) + c;
     int cur = p.sorted[p0];
@@ -371,11 +360,15 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     for (long long q = p0; q < p1; q += U) {
         raw4<T> v[U];
         int now[U];
+        if (left >= 4) {  // (read once: kept out of the caches, 59 -> 44 us for 65536 rows of 1024 bf16)
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            v[j] = load4(dy + (long long)token[j] * p.ld_in, left);
-            now[j] = q + j < p1 ? key[j] : -1;
+            for (int j = 0; j < U; ++j) v[j] = load4_once(dy + (long long)token[j] * p.ld_in);
+        } else {
+#pragma unroll
+            for (int j = 0; j < U; ++j) v[j] = load4(dy + (long long)token[j] * p.ld_in, left);
         }
+#pragma unroll
+        for (int j = 0; j < U; ++j) now[j] = q + j < p1 ? key[j] : -1;
         if (q + U < p1) fetch(q + U);
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -393,6 +386,11 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
             }
         }
     }
+    if (c == 0) {  // (the first column's thread) what the join has to know of this chunk
+        const bool starts = !came_in && goes_on;
+        p.crossing[2 * k] = starts ? cur : -1;
+        p.crossing[2 * k + 1] = starts ? (int)((p.offsets[cur + 1] - 1) / p.chunk) : 0;
+    }
     if (came_in)
         store4(slot, left, sum);
     else if (goes_on)
@@ -402,21 +400,37 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
 }
 
 // The rows whose run crosses the end of a chunk: the group of the chunk where the run starts adds its part and those of the
-// chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).
+// chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).  The same launch clears the rows that
+// no token has: the few long sums wait for memory while the stores go out.
 __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingParams p) {
-    constexpr int U = 32;
+    constexpr int U = 8;
     const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
     const int groups = 256 >> p.lanes_log2;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
-    const long long k = (long long)blockIdx.x * groups + group;
-    const long long n = p.offsets[p.sort_blocks * p.bins];
-    const long long last = (k + 1) * p.chunk - 1;
-    if (last + 1 >= n) return;
-    const int key = p.sorted[last];
-    if (p.sorted[last + 1] != key || p.offsets[key] < k * p.chunk) return;
-    const long long k_end = (p.offsets[key + 1] - 1) / p.chunk;
     const int left = p.dim - c;
+    if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has
+        constexpr int ROWS = 8;
+        const long long r0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * ROWS;
+        bool clear[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const int r = (int)(r0 + k);
+            clear[k] = r0 + k < p.vocabulary;
+            if (clear[k]) {
+                const int key = rank_of_id(p, r) * p.bins + (r >> p.sort_log2);
+                clear[k] = p.offsets[key] == p.offsets[key + 1];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k)
+            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+        return;
+    }
+    const long long k = (long long)blockIdx.x * groups + group;
+    if (k >= p.chunks) return;
+    const int key = p.crossing[2 * k], k_end = p.crossing[2 * k + 1];
+    if (key < 0) return;
     const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim + c, left);
     double sum[4] = {first[0], first[1], first[2], first[3]};
     for (long long q = k + 1; q <= k_end; q += U) {

@@ -57,7 +57,7 @@ EmbeddingParams embedding_params(const snhip_embedding_desc* d, const void* ids,
 struct EmbeddingPlan {
     int sort_blocks, sort_log2, fine_log2, bins, bins_log2, chunk, pieces;
     long long chunks;
-    size_t order, sorted, offsets, piece_id, piece_token, piece_start, partial, bytes;  // places in the workspace
+    size_t order, sorted, offsets, piece_id, piece_token, piece_start, crossing, partial, bytes;  // places in the workspace
 };
 EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
     EmbeddingPlan e{};
@@ -78,7 +78,8 @@ EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
     e.piece_id = e.offsets + up256(((size_t)e.sort_blocks * e.bins + 1) * 4);
     e.piece_token = e.piece_id + up256((size_t)e.pieces * kPiece * 4);
     e.piece_start = e.piece_token + up256((size_t)e.pieces * kPiece * 4);
-    e.partial = e.piece_start + up256((size_t)e.pieces * (kBuckets + 1) * 4);
+    e.crossing = e.piece_start + up256((size_t)e.pieces * (kBuckets + 1) * 4);
+    e.partial = e.crossing + up256((size_t)e.chunks * 8);
     e.bytes = e.partial + up256((size_t)e.chunks * 2 * (size_t)d->dim * 4);
     return e;
 }
@@ -169,9 +170,10 @@ struct BlockNormPlan {
     int groups_per_chunk, chunks_per_group, rows_per_chunk, chunks;
     size_t bytes;
 };
-// How the rows are cut into chunks, one workgroup each.  kBlockNormChunks of them keep every compute unit busy; each more
-// costs its column sums' way to memory and back.
-constexpr long long kBlockNormChunks = 1024;
+// How the rows are cut into chunks, one workgroup each: as many as are on the compute units at a time (two workgroups of 512
+// threads or more to a unit, four smaller ones).  More would only add column sums on their way to memory and back
+// (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us).
+long long block_norm_chunks(int dim) { return dim > 2048 ? 512 : 1024; }
 BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     BlockNormPlan b{};
     const bool gate_rows = d->gate != nullptr && d->gate_rows > 0;
@@ -179,7 +181,8 @@ BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     if (b.rows_per_group < 1) b.rows_per_group = 1;
     b.groups = (d->rows + b.rows_per_group - 1) / b.rows_per_group;
     const int at_once = block_norm_backward_groups(d->dim);
-    long long c = (d->rows + kBlockNormChunks - 1) / kBlockNormChunks;
+    const long long wanted = block_norm_chunks(d->dim);
+    long long c = (d->rows + wanted - 1) / wanted;
     if (c < at_once) c = at_once;
     b.flush = gate_rows && b.rows_per_group <= c;
     if (b.flush) {
@@ -190,10 +193,10 @@ BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
         b.rows_per_chunk = (int)((b.rows_per_group + b.chunks_per_group - 1) / b.chunks_per_group);
         b.chunks = (int)(b.groups * b.chunks_per_group);
     }
-    const bool wanted[5] = {d->d_pre_weight != nullptr && d->dh != nullptr, d->d_pre_bias != nullptr && d->dh != nullptr,
+    const bool sums[5] = {d->d_pre_weight != nullptr && d->dh != nullptr, d->d_pre_bias != nullptr && d->dh != nullptr,
                             d->d_post_weight != nullptr && d->post_norm != SNHIP_NORM_NONE,
                             d->d_post_bias != nullptr && d->post_norm != SNHIP_NORM_NONE, d->d_gate != nullptr && !b.flush};
-    for (int k = 0; k < 5; ++k) b.slots[k] = wanted[k] ? b.vectors++ : -1;
+    for (int k = 0; k < 5; ++k) b.slots[k] = sums[k] ? b.vectors++ : -1;
     b.bytes = up256((size_t)b.vectors * (size_t)b.chunks * (size_t)d->dim * 4);
     return b;
 }
@@ -371,6 +374,7 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     p.offsets = reinterpret_cast<int*>(ws + e.offsets), p.partial = reinterpret_cast<float*>(ws + e.partial);
     p.piece_id = reinterpret_cast<int*>(ws + e.piece_id), p.piece_token = reinterpret_cast<int*>(ws + e.piece_token);
     p.piece_start = reinterpret_cast<int*>(ws + e.piece_start);
+    p.crossing = reinterpret_cast<int*>(ws + e.crossing), p.chunks = e.chunks;
     const int groups = 256 >> p.lanes_log2;
     p.chunk_blocks = (e.chunks + groups - 1) / groups;
     const dim3 sort_grid((unsigned)p.sort_blocks);
@@ -382,13 +386,17 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     else
         embedding_sort_launch<long long>(p, sort_grid, lds, h->stream);
     const long long clear_blocks = p.accumulate ? 0 : ((long long)p.vocabulary + 8 * groups - 1) / (8 * groups);
-    const dim3 grid((unsigned)(p.chunk_blocks + clear_blocks), (unsigned)col_blocks);
-    if (desc->output_type == SNHIP_TYPE_BF16)
-        hipLaunchKernelGGL(embedding_grad_kernel<__bf16>, grid, dim3(256), 0, h->stream, p);
-    else
-        hipLaunchKernelGGL(embedding_grad_kernel<float>, grid, dim3(256), 0, h->stream, p);
-    if (e.chunks > 1)
-        hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)p.chunk_blocks, (unsigned)col_blocks), dim3(256), 0, h->stream, p);
+    const dim3 chunk_grid((unsigned)p.chunk_blocks, (unsigned)col_blocks);
+    if (p.chunk_blocks > 0) {
+        if (desc->output_type == SNHIP_TYPE_BF16)
+            hipLaunchKernelGGL(embedding_grad_kernel<__bf16>, chunk_grid, dim3(256), 0, h->stream, p);
+        else
+            hipLaunchKernelGGL(embedding_grad_kernel<float>, chunk_grid, dim3(256), 0, h->stream, p);
+    }
+    if (e.chunks <= 1) p.chunk_blocks = 0;  // nothing to join
+    if (p.chunk_blocks + clear_blocks > 0)
+        hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)(p.chunk_blocks + clear_blocks), (unsigned)col_blocks), dim3(256), 0,
+                           h->stream, p);
     return hip_to_status(hipGetLastError());
 }
 
@@ -520,10 +528,10 @@ int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
     s.eps = (float)d->epsilon, s.grad_scale = d->gradient_scale;
     s.key0 = (unsigned int)d->seed, s.key1 = (unsigned int)(d->seed >> 32), s.step = (unsigned int)d->step;
     const AdamwEntry* entries = static_cast<const AdamwEntry*>(a->table);
-    if (a->state_bits == 32)
-        hipLaunchKernelGGL(adamw32_kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
-    else
-        hipLaunchKernelGGL(adamw8_kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
+    const bool once = a->chunks * kAdamwChunk >= kAdamwOnce;
+    const auto kernel = a->state_bits == 32 ? (once ? adamw32_kernel<true> : adamw32_kernel<false>)
+                                            : (once ? adamw8_kernel<true> : adamw8_kernel<false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
     return hip_to_status(hipGetLastError());
 }
 

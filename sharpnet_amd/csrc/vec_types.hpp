@@ -47,20 +47,29 @@ template <typename T>
 __device__ __forceinline__ void store4_whole(T* at, f32x4 v) {
     *reinterpret_cast<typename Raw4<T>::any*>(at) = narrow(v, static_cast<const T*>(nullptr));
 }
+// The same for data that is read or written once and will not be found in a cache again.
+template <typename T>
+__device__ __forceinline__ raw4<T> load4_once(const T* at) {
+    return __builtin_nontemporal_load(reinterpret_cast<const typename Raw4<T>::any*>(at));
+}
+template <typename T>
+__device__ __forceinline__ void store4_once(T* at, f32x4 v) {
+    __builtin_nontemporal_store(narrow(v, static_cast<const T*>(nullptr)), reinterpret_cast<typename Raw4<T>::any*>(at));
+}
 // The same for a piece of which `left` elements exist (0 or less: none): one access, or element by element at a row's end;
 // what does not exist reads as zero.
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ raw4<T> load4(const T* at, int left) {
-    if (left >= 4) return load4_whole(at);
+    if (left >= 4) return ONCE ? load4_once(at) : load4_whole(at);
     raw4<T> v = {};
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < left) v[j] = at[j];
     return v;
 }
-template <typename T>
+template <typename T, bool ONCE = false>
 __device__ __forceinline__ void store4(T* at, int left, f32x4 v) {
-    if (left >= 4) return store4_whole(at, v);
+    if (left >= 4) return ONCE ? store4_once(at, v) : store4_whole(at, v);
 #pragma unroll
     for (int j = 0; j < 3; ++j)
         if (j < left) at[j] = (T)v[j];

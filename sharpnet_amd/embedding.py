@@ -6,9 +6,13 @@ float32 (the reference's form, rounded toward zero), int32 or int64; an id outsi
 row of y is zeros and it adds nothing to the gradient.
 """
 import ctypes
+import math
 
 from .gpu_tensor import GPUTensor
 from .hiplib import EmbeddingDesc, TYPES, check_status
+
+_ID_TYPES = {k: TYPES[k] for k in ("float32", "int32", "int64")}
+_ROW_TYPES = {k: TYPES[k] for k in ("float32", "bfloat16")}
 
 
 class WordEmbedding:
@@ -22,17 +26,22 @@ class WordEmbedding:
         self.Wrapper = gpu_wrapper
         self._workspace = None
         self._workspaceBytes = 0
+        # a call fills in every field that is not of the layer itself
+        self._d = EmbeddingDesc(vocabulary=self.VocabularySize, dim=self.EmbeddingDim, padding_index=self.PaddingIndex, scale=self.Scale)
+        self._need = ctypes.c_size_t()
 
     def _desc(self, x, rows, table_type):
         """rows: y or dy, (..., EmbeddingDim) with one row per id of x."""
-        if x.Type not in ("float32", "int32", "int64"):
+        if x.Type not in _ID_TYPES:
             raise ValueError("ids must be float32, int32 or int64, not %s" % x.Type)
-        if rows.Type not in ("float32", "bfloat16") or table_type not in ("float32", "bfloat16"):
+        if rows.Type not in _ROW_TYPES or table_type not in _ROW_TYPES:
             raise ValueError("rows and table must be float32 or bfloat16, not %s and %s" % (rows.Type, table_type))
-        if rows.Shape[-1] != self.EmbeddingDim or rows.Count != x.Count * self.EmbeddingDim:
+        tokens = math.prod(x.Shape)
+        if rows.Shape[-1] != self.EmbeddingDim or math.prod(rows.Shape) != tokens * self.EmbeddingDim:
             raise ValueError("%s ids and rows of %s do not fit an embedding dimension of %d" % (x.Shape, rows.Shape, self.EmbeddingDim))
-        return EmbeddingDesc(id_type=TYPES[x.Type], table_type=TYPES[table_type], output_type=TYPES[rows.Type], tokens=x.Count,
-                             vocabulary=self.VocabularySize, dim=self.EmbeddingDim, padding_index=self.PaddingIndex, scale=self.Scale)
+        d = self._d
+        d.id_type, d.table_type, d.output_type, d.tokens = _ID_TYPES[x.Type], _ROW_TYPES[table_type], _ROW_TYPES[rows.Type], tokens
+        return d
 
     def _check_table(self, table):
         if table.Shape != [self.VocabularySize, self.EmbeddingDim]:
@@ -42,8 +51,9 @@ class WordEmbedding:
         """y (ids' shape + EmbeddingDim) = Scale * wordEmbedding[x]."""
         self._check_table(wordEmbedding)
         d = self._desc(x, y, wordEmbedding.Type)
-        for t in (y, x, wordEmbedding):
-            t.AssertIsNotDisposed()
+        y.AssertIsNotDisposed()
+        x.AssertIsNotDisposed()
+        wordEmbedding.AssertIsNotDisposed()
         check_status(y._lib.snhip_embedding_forward(y.Wrapper.handle, ctypes.byref(d), x.Pointer, wordEmbedding.Pointer,
                                                     y.Pointer), "snhip_embedding_forward")
 
@@ -62,9 +72,10 @@ class WordEmbedding:
         if dWordEmbedding.Type != "float32":
             raise ValueError("the table's gradient must be float32, not %s" % dWordEmbedding.Type)
         d = self._desc(x, dy, "float32")
-        for t in (dWordEmbedding, x, dy):
-            t.AssertIsNotDisposed()
-        need = ctypes.c_size_t()
+        dWordEmbedding.AssertIsNotDisposed()
+        x.AssertIsNotDisposed()
+        dy.AssertIsNotDisposed()
+        need = self._need
         check_status(dy._lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_embedding_backward_workspace_size")
         if workspace is None:

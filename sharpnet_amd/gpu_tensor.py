@@ -17,6 +17,7 @@ All arithmetic happens in libsharpnet_hip.so on the GPU; numpy is used only to
 stage host data for the H2D / D2H copies.
 """
 import ctypes
+import math
 
 import numpy as np
 
@@ -155,10 +156,7 @@ class GPUWrapper:
 
 
 def _prod(xs):
-    p = 1
-    for x in xs:
-        p *= int(x)
-    return p
+    return math.prod(int(x) for x in xs)
 
 
 # element types: numpy type of the host copy (bfloat16 travels as float32 values) and bytes in device memory
@@ -212,7 +210,7 @@ class GPUTensor:
     # -- shape helpers (Tensor.cs:18-21,1521-1526) ---------------------------
     @property
     def Count(self):
-        return _prod(self.Shape)
+        return math.prod(self.Shape)
 
     @property
     def Dimension(self):

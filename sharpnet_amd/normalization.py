@@ -6,6 +6,7 @@ in libsharpnet_hip.so.  x is the residual stream, y the output of the block behi
 what the next block reads.
 """
 import ctypes
+import math
 
 from .gpu_tensor import GPUTensor
 from .hiplib import (ACT_NONE, ACT_SIGMOID, ACT_TANH, BlockNormDesc, NORM_LAYER, NORM_NONE, NORM_RMS, SharpNetHipError, CublasStatus,
@@ -14,10 +15,15 @@ from .hiplib import (ACT_NONE, ACT_SIGMOID, ACT_TANH, BlockNormDesc, NORM_LAYER,
 _NORMS = {None: NORM_NONE, "none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAYER}
 _GATES = {None: ACT_NONE, "none": ACT_NONE, "sigmoid": ACT_SIGMOID, "tanh": ACT_TANH,
           "CUDNN_ACTIVATION_IDENTITY": ACT_NONE, "CUDNN_ACTIVATION_SIGMOID": ACT_SIGMOID, "CUDNN_ACTIVATION_TANH": ACT_TANH}
+_ROW_TYPES = {k: TYPES[k] for k in ("float32", "bfloat16")}
 
 
-def _pointer(t):
-    return t.Pointer if t is not None else None
+def _live(t):
+    """The address of a tensor that is there, None for None."""
+    if t is None:
+        return None
+    t.AssertIsNotDisposed()
+    return t.Pointer
 
 
 class BlockNorm:
@@ -31,67 +37,68 @@ class BlockNorm:
         if gateActivation not in _GATES:
             raise SharpNetHipError(CublasStatus.CUBLAS_STATUS_NOT_SUPPORTED, "gate activation %r" % (gateActivation,))
         self.EmbeddingDim = int(embeddingDim)
+        self._vectorShape = [self.EmbeddingDim]
         self.PreNorm, self.PostNorm, self.GateActivation = _NORMS[preNorm], _NORMS[postNorm], _GATES[gateActivation]
         self.ResidualScale, self.Epsilon = float(residualScale), float(epsilon)
         self.Wrapper = gpu_wrapper
         self._workspace = None
         self._workspaceBytes = 0
+        # one descriptor for each direction; a call fills in every field that is not of the layer itself
+        layer = dict(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=self.EmbeddingDim,
+                     epsilon=self.Epsilon, residual_scale=self.ResidualScale)
+        self._forward, self._backward, self._need = BlockNormDesc(**layer), BlockNormDesc(**layer), ctypes.c_size_t()
 
-    def _rows(self, t, name, rows, type_=None):
+    def _rows(self, t, name, shape, type_):
+        """t is None or has rows like those of shape, in the given type."""
         if t is None:
             return
-        t.AssertIsNotDisposed()
-        if t.Shape[-1] != self.EmbeddingDim or t.Count != rows * self.EmbeddingDim:
-            raise ValueError("%s is %s, expected %d rows of %d" % (name, t.Shape, rows, self.EmbeddingDim))
-        if type_ is not None and t.Type != type_:
+        if t.Shape != shape and (t.Shape[-1] != self.EmbeddingDim or math.prod(t.Shape) != math.prod(shape)):
+            raise ValueError("%s is %s, expected the rows of %s" % (name, t.Shape, shape))
+        if t.Type != type_:
             raise ValueError("%s is %s, expected %s" % (name, t.Type, type_))
 
     def _vector(self, t, name):
-        if t is None:
-            return
-        t.AssertIsNotDisposed()
-        if t.Count != self.EmbeddingDim or t.Type != "float32":
+        if t is not None and (t.Type != "float32" or (t.Shape != self._vectorShape and math.prod(t.Shape) != self.EmbeddingDim)):
             raise ValueError("%s is %s %s, expected %d float32" % (name, t.Type, t.Shape, self.EmbeddingDim))
 
-    def _desc(self, stream, blocks, rows, y, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
-        block = next((t for t in blocks if t is not None), stream)
-        for t in blocks:
-            self._rows(t, "a tensor of the blocks", rows, block.Type)
-        for t, name in ((preWeight, "preWeight"), (preBias, "preBias"), (postWeight, "postWeight"), (postBias, "postBias")):
-            self._vector(t, name)
+    def _fill(self, d, stream, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
+        """What both directions have: sizes and types, gate, weights, statistics."""
+        if self.EmbeddingDim <= 0 or stream.Shape[-1] != self.EmbeddingDim:
+            raise ValueError("rows of %s do not fit an embedding dimension of %d" % (stream.Shape, self.EmbeddingDim))
+        if stream.Type not in _ROW_TYPES or block.Type not in _ROW_TYPES:
+            raise ValueError("rows must be float32 or bfloat16, not %s and %s" % (stream.Type, block.Type))
+        rows = math.prod(stream.Shape) // self.EmbeddingDim
+        self._vector(preWeight, "preWeight")
+        self._vector(preBias, "preBias")
+        self._vector(postWeight, "postWeight")
+        self._vector(postBias, "postBias")
         for t, name in ((preStatistics, "preStatistics"), (postStatistics, "postStatistics")):
-            if t is not None and (t.Count != 2 * rows or t.Type != "float32"):
+            if t is not None and (math.prod(t.Shape) != 2 * rows or t.Type != "float32"):
                 raise ValueError("%s is %s %s, expected (%d, 2) float32" % (name, t.Type, t.Shape, rows))
-        if gate is not None and gateRows == 0:
-            self._vector(gate, "gate")
-        elif gate is not None:
-            if gateRows < 0:
-                raise ValueError("gateRows is %d" % gateRows)
-            self._rows(gate, "gate", -(-rows // gateRows), block.Type)
-        for t in (stream, block):
-            if t.Type not in ("float32", "bfloat16"):
-                raise ValueError("rows must be float32 or bfloat16, not %s" % t.Type)
-        return BlockNormDesc(stream_type=TYPES[stream.Type], block_type=TYPES[block.Type], pre_norm=self.PreNorm, post_norm=self.PostNorm,
-                             gate_activation=self.GateActivation, dim=self.EmbeddingDim, gate_rows=gateRows, rows=rows,
-                             epsilon=self.Epsilon, residual_scale=self.ResidualScale, pre_weight=_pointer(preWeight),
-                             pre_bias=_pointer(preBias), post_weight=_pointer(postWeight), post_bias=_pointer(postBias),
-                             gate=_pointer(gate), y=_pointer(y), pre_statistics=_pointer(preStatistics),
-                             post_statistics=_pointer(postStatistics))
-
-    def _row_count(self, t):
-        if self.EmbeddingDim <= 0 or t.Shape[-1] != self.EmbeddingDim:
-            raise ValueError("rows of %s do not fit an embedding dimension of %d" % (t.Shape, self.EmbeddingDim))
-        return t.Count // self.EmbeddingDim
+        if gateRows < 0:
+            raise ValueError("gateRows is %d" % gateRows)
+        if gate is not None:
+            if gateRows == 0:
+                self._vector(gate, "gate")
+            else:
+                self._rows(gate, "gate", [-(-rows // gateRows), self.EmbeddingDim], block.Type)
+        d.rows, d.gate_rows = rows, gateRows
+        d.stream_type, d.block_type = _ROW_TYPES[stream.Type], _ROW_TYPES[block.Type]
+        d.gate, d.pre_weight, d.pre_bias = _live(gate), _live(preWeight), _live(preBias)
+        d.post_weight, d.post_bias = _live(postWeight), _live(postBias)
+        d.pre_statistics, d.post_statistics = _live(preStatistics), _live(postStatistics)
 
     def ForwardPropagation(self, x, h, y=None, u=None, gate=None, gateRows=0, preWeight=None, preBias=None, postWeight=None,
                            postBias=None, preStatistics=None, postStatistics=None):
         """h and u from x and y; h is None for a join without a norm ahead of the next block, y and u for a norm without a
         block.  gateRows: rows that share a row of the gate (0: the gate is one vector)."""
-        rows = self._row_count(x)
-        d = self._desc(x, (y, h), rows, y, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
-        self._rows(x, "x", rows)
-        self._rows(u, "u", rows, x.Type)
-        d.x, d.u, d.h = x.Pointer, _pointer(u), _pointer(h)
+        d, shape = self._forward, x.Shape
+        block = h if h is not None else y if y is not None else x
+        self._fill(d, x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
+        self._rows(y, "y", shape, block.Type)
+        self._rows(h, "h", shape, block.Type)
+        self._rows(u, "u", shape, x.Type)
+        d.x, d.y, d.u, d.h = _live(x), _live(y), _live(u), _live(h)
         check_status(x._lib.snhip_block_norm_forward(x.Wrapper.handle, ctypes.byref(d)), "snhip_block_norm_forward")
 
     def BackwardPropagation(self, dx, u, dh, du=None, y=None, dy=None, gate=None, dGate=None, gateRows=0, preWeight=None,
@@ -100,19 +107,23 @@ class BlockNorm:
         """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics; gradients that are
         None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
-        rows = self._row_count(dx)
-        d = self._desc(dx, (y, dh, dy), rows, y, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
-        for t, name in ((dx, "dx"), (u, "u"), (du, "du")):
-            self._rows(t, name, rows, dx.Type)
+        d, shape = self._backward, dx.Shape
+        block = next((t for t in (dh, y, dy) if t is not None), dx)
+        self._fill(d, dx, block, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
+        for t, name in ((y, "y"), (dh, "dh"), (dy, "dy")):
+            self._rows(t, name, shape, block.Type)
+        for t, name in ((u, "u"), (du, "du")):
+            self._rows(t, name, shape, dx.Type)
         for t, name in ((dPreWeight, "dPreWeight"), (dPreBias, "dPreBias"), (dPostWeight, "dPostWeight"), (dPostBias, "dPostBias")):
             self._vector(t, name)
         if dGate is not None and (gate is None or dGate.Shape != gate.Shape or dGate.Type != gate.Type):
             raise ValueError("dGate must have the gate's shape and type")
-        d.u, d.dx, d.dh, d.du, d.dy = _pointer(u), dx.Pointer, _pointer(dh), _pointer(du), _pointer(dy)
-        d.d_gate, d.d_pre_weight, d.d_pre_bias = _pointer(dGate), _pointer(dPreWeight), _pointer(dPreBias)
-        d.d_post_weight, d.d_post_bias, d.accumulate = _pointer(dPostWeight), _pointer(dPostBias), int(bool(accumulate))
-        need = ctypes.c_size_t()
-        check_status(dx._lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
+        d.y, d.u, d.dx, d.dh, d.du, d.dy = _live(y), _live(u), _live(dx), _live(dh), _live(du), _live(dy)
+        d.d_gate, d.d_pre_weight, d.d_pre_bias = _live(dGate), _live(dPreWeight), _live(dPreBias)
+        d.d_post_weight, d.d_post_bias = _live(dPostWeight), _live(dPostBias)
+        d.accumulate = 1 if accumulate else 0
+        need, lib = self._need, dx._lib
+        check_status(lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_block_norm_backward_workspace_size")
         if workspace is None and need.value:
             if self._workspaceBytes < need.value:
@@ -123,7 +134,7 @@ class BlockNorm:
                 self._workspaceBytes = need.value
             workspace = self._workspace
         nbytes = workspace.Count * workspace.ElementBytes if workspace is not None else 0
-        check_status(dx._lib.snhip_block_norm_backward(dx.Wrapper.handle, ctypes.byref(d), _pointer(workspace), nbytes),
+        check_status(lib.snhip_block_norm_backward(dx.Wrapper.handle, ctypes.byref(d), _live(workspace), nbytes),
                      "snhip_block_norm_backward")
 
     def Dispose(self):
