@@ -389,7 +389,8 @@ typedef struct snhip_embedding_desc {
 } snhip_embedding_desc;
 int snhip_sizeof_embedding_desc(void);
 int snhip_embedding_forward(void* handle, const snhip_embedding_desc* desc, const void* ids, const void* table, void* y);
-/* Bytes of device memory that snhip_embedding_backward needs for a descriptor (the sorted order and partial sums). */
+/* Bytes of device memory that snhip_embedding_backward needs for a descriptor (the sorted order and partial sums); 0 is
+ * possible. */
 int snhip_embedding_backward_workspace_size(const snhip_embedding_desc* desc, size_t* bytes);
 /* Writes every row of table_gradient (zeros where no token has the id), or adds to it with accumulate != 0.  workspace is
  * scratch for this call (16-byte aligned; less than the size above is refused with status 7): the caller's own, so that

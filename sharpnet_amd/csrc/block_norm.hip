@@ -67,6 +67,7 @@ void backward_kind(const BlockNormParams& p, BlockNormKind k, hipStream_t stream
 void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
     const int units = (p.dim + 3) / 4;
     if (units <= 16) return forward<16, 1>(p, stream);
+    if (units <= 32) return forward<16, 2>(p, stream);
     if (units <= 64) return forward<64, 1>(p, stream);
     if (p.rows <= 512) {
         if (units <= 256) return forward<256, 1>(p, stream);
@@ -84,6 +85,7 @@ void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
 void SNHIP_BACKWARD(const BlockNormParams& p, BlockNormKind kind, hipStream_t stream) {
     const int units = (p.dim + 3) / 4;
     if (units <= 16) return backward_kind<16, 1>(p, kind, stream);
+    if (units <= 32) return backward_kind<16, 2>(p, kind, stream);
     if (units <= 64) return backward_kind<64, 1>(p, kind, stream);
     if (units <= 128) return backward_kind<64, 2>(p, kind, stream);
     if (units <= 256) return backward_kind<256, 1>(p, kind, stream);

@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
     typedef Piece<TPR, EXACT> P;
     constexpr bool HAS_Y = MODE == 2 || GATE;
     __shared__ float lds[2][2][TPR / 64 + 1];
-    __shared__ f32x4 meet[GROUPS > 1 ? GROUPS * TPR * N : 1];
+    constexpr int VECTORS = 1 + (BIAS ? 1 : 0) + (MODE == 2 ? 1 + (BIAS ? 1 : 0) : 0) + (GATE ? 1 : 0);  // of column sums
+    __shared__ f32x4 meet[GROUPS > 1 ? VECTORS * GROUPS * TPR * N : 1];
     int turn = 0;
     const int lane = threadIdx.x % TPR, group = row_group<TPR>(), dim = p.dim;
     constexpr f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -427,29 +428,42 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
         left_in_group = last_of_group ? p.rows_per_group : left_in_group - 1;
     }
     // the column sums of the chunk; groups of threads that share the columns meet in LDS
-    auto put = [&](const f32x4* acc, int slot) {
-        if (slot < 0) return;  // the same for the whole launch
-        float* out = p.partial + ((long long)slot * p.chunks + chunk) * dim;
-        if constexpr (GROUPS > 1) {
-            __syncthreads();
+    auto every = [&](auto&& each) {  // the sums there are, with the slot of each
+        each(acc_w, 0);
+        if constexpr (BIAS) each(acc_b, 1);
+        if constexpr (MODE == 2) each(acc_pw, 2);
+        if constexpr (MODE == 2 && BIAS) each(acc_pb, 3);
+        if constexpr (GATE) each(acc_g, 4);
+    };
+    if constexpr (GROUPS > 1) {
+        constexpr int PIECES = TPR * N;
+        int v = 0;
+        every([&](const f32x4* acc, int) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) meet[(group * N + n) * TPR + lane] = acc[n];
-            __syncthreads();
-            for (int k = threadIdx.x; k < TPR * N; k += NT) {
-                f32x4 s = meet[k];
-                for (int g = 1; g < GROUPS; ++g) s += meet[g * TPR * N + k];
-                P::store(out, k / TPR, k % TPR, dim, s);
-            }
-        } else {
+            for (int n = 0; n < N; ++n) meet[(v * GROUPS + group) * PIECES + n * TPR + lane] = acc[n];
+            ++v;
+        });
+        __syncthreads();
+        for (int k = threadIdx.x; k < VECTORS * PIECES; k += NT) {
+            const int piece = k % PIECES, vector = k / PIECES;
+            int slot = -1, at = 0;
+            every([&](const f32x4*, int s) {
+                if (at == vector) slot = p.slot[s];
+                ++at;
+            });
+            if (slot < 0) continue;
+            f32x4 s = meet[vector * GROUPS * PIECES + piece];
+            for (int g = 1; g < GROUPS; ++g) s += meet[(vector * GROUPS + g) * PIECES + piece];
+            store4(p.partial + ((long long)slot * p.chunks + chunk) * dim + 4 * piece, dim - 4 * piece, s);
+        }
+    } else {
+        every([&](const f32x4* acc, int s) {
+            if (p.slot[s] < 0) return;
+            float* out = p.partial + ((long long)p.slot[s] * p.chunks + chunk) * dim;
 #pragma unroll
             for (int n = 0; n < N; ++n) P::store(out, n, lane, dim, acc[n]);
-        }
-    };
-    put(acc_w, p.slot[0]);
-    if constexpr (BIAS) put(acc_b, p.slot[1]);
-    if constexpr (MODE == 2) put(acc_pw, p.slot[2]);
-    if constexpr (MODE == 2 && BIAS) put(acc_pb, p.slot[3]);
-    if constexpr (GATE) put(acc_g, p.slot[4]);
+        });
+    }
 }
 
 }  // namespace snhip

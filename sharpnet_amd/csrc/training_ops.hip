@@ -55,6 +55,7 @@ EmbeddingParams embedding_params(const snhip_embedding_desc* d, const void* ids,
 }
 
 struct EmbeddingPlan {
+    bool small;  // embedding_small_kernel: no workspace
     int sort_blocks, sort_log2, fine_log2, bins, bins_log2, chunk, pieces;
     long long chunks;
     size_t order, sorted, offsets, piece_id, piece_token, piece_start, crossing, partial, bytes;  // places in the workspace
@@ -70,6 +71,8 @@ EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
     e.bins = (int)(((long long)d->vocabulary + e.sort_blocks - 1) >> e.sort_log2);
     if (e.bins < 1) e.bins = 1;
     while ((1 << e.bins_log2) < e.bins) ++e.bins_log2;
+    e.small = d->tokens <= kSmallTokens && d->tokens * d->dim <= kSmallElements && e.fine_log2 == 0;
+    if (e.small) return e;
     e.chunk = d->tokens >= 16384 ? 32 : 8;
     e.chunks = (d->tokens + e.chunk - 1) / e.chunk;
     e.order = 0;
@@ -103,6 +106,15 @@ void embedding_forward_types(const EmbeddingParams& p, int table_type, int outpu
         embedding_forward_launch<ID, float, __bf16>(p, stream);
     else
         embedding_forward_launch<ID, float, float>(p, stream);
+}
+
+template <typename ID>
+void embedding_small_launch(const EmbeddingParams& p, int type, dim3 grid, size_t lds, hipStream_t stream) {
+    lds = std::max(lds, (size_t)1024 * sizeof(f32x4));
+    if (type == SNHIP_TYPE_BF16)
+        hipLaunchKernelGGL((embedding_small_kernel<ID, __bf16>), grid, dim3(1024), lds, stream, p);
+    else
+        hipLaunchKernelGGL((embedding_small_kernel<ID, float>), grid, dim3(1024), lds, stream, p);
 }
 
 template <typename ID>
@@ -170,10 +182,10 @@ struct BlockNormPlan {
     int groups_per_chunk, chunks_per_group, rows_per_chunk, chunks;
     size_t bytes;
 };
-// How the rows are cut into chunks, one workgroup each: as many as are on the compute units at a time (two workgroups of 512
-// threads or more to a unit, four smaller ones).  More would only add column sums on their way to memory and back
+// How the rows are cut into chunks, one workgroup each: as many as are on the compute units at a time (two workgroups to a
+// unit for long rows, four for short ones).  More would only add column sums on their way to memory and back
 // (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us).
-long long block_norm_chunks(int dim) { return dim > 2048 ? 512 : 1024; }
+long long block_norm_chunks(int dim) { return dim > 1024 ? 512 : 1024; }
 BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     BlockNormPlan b{};
     const bool gate_rows = d->gate != nullptr && d->gate_rows > 0;
@@ -360,7 +372,7 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     if (!aligned(ids, type_bytes(desc->id_type)) || !aligned(dy, type_bytes(desc->output_type)) || !aligned(table_gradient, 4))
         return SNHIP_STATUS_INVALID_VALUE;
     const EmbeddingPlan e = embedding_plan(desc);
-    if (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < e.bytes) return SNHIP_STATUS_INVALID_VALUE;
+    if (e.bytes > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspace_bytes < e.bytes)) return SNHIP_STATUS_INVALID_VALUE;
     DeviceScope scope(h->device);
     if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
     EmbeddingParams p = embedding_params(desc, ids, dy, table_gradient, true);
@@ -369,6 +381,17 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     p.accumulate = accumulate != 0;
     p.sort_blocks = e.sort_blocks, p.sort_log2 = e.sort_log2, p.bins = e.bins, p.bins_log2 = e.bins_log2, p.chunk = e.chunk;
     p.fine_log2 = e.fine_log2, p.pieces = e.pieces;
+    const dim3 sort_grid((unsigned)p.sort_blocks);
+    const size_t lds = (size_t)16 * p.bins * sizeof(int);
+    if (e.small) {
+        if (desc->id_type == SNHIP_TYPE_F32)
+            embedding_small_launch<float>(p, desc->output_type, sort_grid, lds, h->stream);
+        else if (desc->id_type == SNHIP_TYPE_I32)
+            embedding_small_launch<int>(p, desc->output_type, sort_grid, lds, h->stream);
+        else
+            embedding_small_launch<long long>(p, desc->output_type, sort_grid, lds, h->stream);
+        return hip_to_status(hipGetLastError());
+    }
     char* ws = static_cast<char*>(workspace);
     p.order = reinterpret_cast<int*>(ws + e.order), p.sorted = reinterpret_cast<int*>(ws + e.sorted);
     p.offsets = reinterpret_cast<int*>(ws + e.offsets), p.partial = reinterpret_cast<float*>(ws + e.partial);
@@ -377,8 +400,6 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     p.crossing = reinterpret_cast<int*>(ws + e.crossing), p.chunks = e.chunks;
     const int groups = 256 >> p.lanes_log2;
     p.chunk_blocks = (e.chunks + groups - 1) / groups;
-    const dim3 sort_grid((unsigned)p.sort_blocks);
-    const size_t lds = (size_t)16 * p.bins * sizeof(int);
     if (desc->id_type == SNHIP_TYPE_F32)
         embedding_sort_launch<float>(p, sort_grid, lds, h->stream);
     else if (desc->id_type == SNHIP_TYPE_I32)

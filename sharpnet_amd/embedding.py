@@ -78,7 +78,7 @@ class WordEmbedding:
         need = self._need
         check_status(dy._lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_embedding_backward_workspace_size")
-        if workspace is None:
+        if workspace is None and need.value:
             if self._workspaceBytes < need.value:
                 if self._workspace is not None:
                     self._workspace.Wrapper.synchronize()
@@ -87,8 +87,10 @@ class WordEmbedding:
                 self._workspaceBytes = need.value
             workspace = self._workspace
         check_status(dy._lib.snhip_embedding_backward(dy.Wrapper.handle, ctypes.byref(d), x.Pointer, dy.Pointer,
-                                                      dWordEmbedding.Pointer, int(bool(accumulate)), workspace.Pointer,
-                                                      workspace.Count * workspace.ElementBytes), "snhip_embedding_backward")
+                                                      dWordEmbedding.Pointer, int(bool(accumulate)),
+                                                      workspace.Pointer if workspace is not None else None,
+                                                      workspace.Count * workspace.ElementBytes if workspace is not None else 0),
+                     "snhip_embedding_backward")
 
     def Dispose(self):
         if self._workspace is not None:

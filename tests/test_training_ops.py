@@ -66,7 +66,11 @@ def test_embedding_pointer_checks(lib, handle):
     for args in ((None, A, A), (A, None, A), (A, A, None), (A + 2, A, A), (A, A + 2, A), (A, A, A + 1)):
         assert lib.snhip_embedding_forward(handle, r, *args) == BAD, args
     assert lib.snhip_embedding_backward_workspace_size(r, None) == BAD
-    assert lib.snhip_embedding_backward_workspace_size(r, ctypes.byref(n)) == 0
+    # few tokens: no scratch memory
+    assert lib.snhip_embedding_backward_workspace_size(r, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.snhip_embedding_backward(handle, r, A, A, A, 0, None, 0) == OK_SO_FAR
+    d.tokens = 5000
+    assert lib.snhip_embedding_backward_workspace_size(r, ctypes.byref(n)) == 0 and n.value > 0
     full = n.value
     for args in ((None, A, A, 0, A, full), (A, None, A, 0, A, full), (A, A, None, 0, A, full), (A, A, A, 0, None, full),
                  (A, A, A, 0, A + 4, full), (A, A, A, 0, A, full - 1), (A, A + 1, A, 0, A, full), (A, A, A + 2, 0, A, full)):
@@ -75,7 +79,7 @@ def test_embedding_pointer_checks(lib, handle):
     d.tokens = 0      # nothing to look up, nothing to add
     assert lib.snhip_embedding_forward(handle, r, None, None, None) == 0
     assert lib.snhip_embedding_backward(handle, r, None, None, None, 1, None, 0) == 0
-    assert lib.snhip_embedding_backward(handle, r, None, None, None, 0, A, full) == BAD   # the gradient has to be cleared
+    assert lib.snhip_embedding_backward(handle, r, None, None, None, 0, None, 0) == BAD   # the gradient has to be cleared
     d.id_type, d.tokens = hiplib.TYPE_I64, 4
     assert lib.snhip_embedding_forward(handle, r, A + 4, A, A) == BAD
 
