@@ -60,8 +60,10 @@ struct Piece {
                 return __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b128(b, 4 * c, 0, 0));
             else
                 return __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b64(b, 2 * c, 0, 0));
+        } else if constexpr (EXACT) {
+            return load4_whole(row + (c < dim ? c : dim - 4));
         } else {
-            return load4(row + c, dim - c);
+            return load4_row(row, c, dim);
         }
     }
     template <typename T>
@@ -78,6 +80,16 @@ struct Piece {
             store4(row + c, dim - c, v);
         }
     }
+    // what a loaded piece is worth: zeros behind the row's end
+    template <typename R>
+    __device__ __forceinline__ static f32x4 value(R raw, int n, int lane, int dim) {
+        if constexpr (BUFFER)
+            return widen(raw);
+        else if constexpr (EXACT)
+            return cut(widen(raw), n, lane, dim);
+        else
+            return existing(widen(raw), dim - column(n, lane), __ballot(dim - column(n, lane) < 4) != 0);
+    }
     // zeros behind the row's end, where a computation has left something else
     __device__ __forceinline__ static f32x4 cut(f32x4 v, int n, int lane, int dim) {
         const int c = column(n, lane);
@@ -93,7 +105,7 @@ struct Piece {
     // of a weight or bias vector; `missing` where there is none
     __device__ __forceinline__ static f32x4 vector(const float* v, int n, int lane, int dim, float missing) {
         if (v == nullptr) return f32x4{missing, missing, missing, missing};
-        return load(v, n, lane, dim);
+        return value(load(v, n, lane, dim), n, lane, dim);
     }
 };
 
@@ -217,7 +229,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_forward_kern
         }
         f32x4 y[N];
 #pragma unroll
-        for (int n = 0; n < N; ++n) y[n] = widen(y_raw[n]);
+        for (int n = 0; n < N; ++n) y[n] = P::value(y_raw[n], n, lane, dim);
         if (p.post != NORM_NONE) {
             row_statistics<EXACT, TPR, N>(y, lane, p.post, p, lds, turn, mean, rstd);
             if (p.post_s != nullptr && lane == 0) p.post_s[2 * row] = mean, p.post_s[2 * row + 1] = rstd;
@@ -231,22 +243,22 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_forward_kern
             for (int n = 0; n < N; ++n) {
                 f32x4 g;
                 if (gate_in_rows)
-                    g = widen(g_raw[n]);
+                    g = P::value(g_raw[n], n, lane, dim);
                 else
-                    g = P::load(static_cast<const float*>(p.gate), n, lane, dim);
+                    g = P::vector(static_cast<const float*>(p.gate), n, lane, dim, 1.0f);
                 y[n] *= gate_values(g, p.act);
             }
         }
         TS* ur = static_cast<TS*>(p.u) + row * p.ld_u;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            u[n] = as_stored<TS>(widen(x[n]) + p.scale * y[n]);
+            u[n] = as_stored<TS>(P::value(x[n], n, lane, dim) + p.scale * y[n]);
             P::store(ur, n, lane, dim, u[n]);
             u[n] = P::cut(u[n], n, lane, dim);
         }
     } else {
 #pragma unroll
-        for (int n = 0; n < N; ++n) u[n] = widen(x[n]);
+        for (int n = 0; n < N; ++n) u[n] = P::value(x[n], n, lane, dim);
     }
     if (p.pre == NORM_NONE) return;
     row_statistics<EXACT, TPR, N>(u, lane, p.pre, p, lds, turn, mean, rstd);
@@ -366,8 +378,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
         if (p.dh != nullptr) {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
-                    const f32x4 dh = widen(ahead.dh[n]);
-                hat[n] = (widen(ahead.u[n]) - ahead.mean) * ahead.rstd;
+                    const f32x4 dh = P::value(ahead.dh[n], n, lane, dim);
+                hat[n] = (P::value(ahead.u[n], n, lane, dim) - ahead.mean) * ahead.rstd;
                 acc_w[n] += dh * hat[n];
                 if constexpr (BIAS) acc_b[n] += dh;
                 t[n] = dh * P::vector(p.pre_w, n, lane, dim, 1.0f);
@@ -375,10 +387,10 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
             row_gradient<TPR, N>(t, hat, p.pre, ahead.rstd, p, lds, turn);
             if (p.du != nullptr)
 #pragma unroll
-                for (int n = 0; n < N; ++n) t[n] += widen(ahead.du[n]);
+                for (int n = 0; n < N; ++n) t[n] += P::value(ahead.du[n], n, lane, dim);
         } else {
 #pragma unroll
-            for (int n = 0; n < N; ++n) t[n] = widen(ahead.du[n]);
+            for (int n = 0; n < N; ++n) t[n] = P::value(ahead.du[n], n, lane, dim);
         }
         if (r + step < r_end) fetch_ahead(r + step);
 #pragma unroll
@@ -388,7 +400,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
             for (int n = 0; n < N; ++n) {
                     t[n] = P::cut(t[n] * p.scale, n, lane, dim);
                 if constexpr (HAS_Y) {
-                    hat[n] = widen(now.y[n]);
+                    hat[n] = P::value(now.y[n], n, lane, dim);
                     if constexpr (MODE == 2) hat[n] = (hat[n] - now.mean) * now.rstd;
                 }
                 f32x4 w;
@@ -397,9 +409,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
                     f32x4 v = hat[n], g;
                     if constexpr (MODE == 2) v = v * w + P::vector(p.post_b, n, lane, dim, 0.0f);
                     if (gate_in_rows)
-                        g = widen(now.g[n]);
+                        g = P::value(now.g[n], n, lane, dim);
                     else
-                        g = P::load(static_cast<const float*>(p.gate), n, lane, dim);
+                        g = P::vector(static_cast<const float*>(p.gate), n, lane, dim, 1.0f);
                     const f32x4 q = gate_values(g, p.act);
                     acc_g[n] += t[n] * v * gate_slopes(q, p.act);
                     t[n] *= q;

@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
     const long long t0 = ((long long)blockIdx.x * groups + group) * ROWS;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
+    const bool ends = __ballot(p.dim - c < 4) != 0;
     int id[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
@@ -70,12 +71,12 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
         v[r] = raw4<TIN>{};
-        if (id[r] >= 0) v[r] = load4(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in + c, p.dim - c);
+        if (id[r] >= 0) v[r] = load4_row(static_cast<const TIN*>(p.in) + (long long)id[r] * p.ld_in, c, p.dim);
     }
 #pragma unroll
     for (int r = 0; r < ROWS; ++r)
         if (t0 + r < p.tokens)
-            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out + c, p.dim - c, widen(v[r]) * p.scale);
+            store4(static_cast<TOUT*>(p.out) + (t0 + r) * p.ld_out + c, p.dim - c, existing(widen(v[r]), p.dim - c, ends) * p.scale);
 }
 
 // The sort.  Ids are dealt out to the workgroups of embedding_sort_kernel in turn (words come by frequency in most
@@ -333,6 +334,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
     const int left = p.dim - c;
+    const bool ends = __ballot(left < 4) != 0;
     const int keys = p.sort_blocks * p.bins;
     const long long k = (long long)blockIdx.x * groups + group;
     const long long n = p.offsets[keys];
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
         return;
     }
     const long long p1 = p0 + p.chunk < n ? p0 + p.chunk : n;
-    const T* dy = static_cast<const T*>(p.in) + c;
+    const T* dy = static_cast<const T*>(p.in);
     int cur = p.sorted[p0];
     bool came_in = p0 > 0 && p.sorted[p0 - 1] == cur;
     const bool goes_on = p1 < n && p.sorted[p1] == p.sorted[p1 - 1];
@@ -360,12 +362,14 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
     for (long long q = p0; q < p1; q += U) {
         raw4<T> v[U];
         int now[U];
-        if (left >= 4) {  // (read once: kept out of the caches, 59 -> 44 us for 65536 rows of 1024 bf16)
+        // (read once: kept out of the caches, 59 -> 44 us for 65536 rows of 1024 bf16)
+        if (p.dim >= 4) {
+            const T* at = dy + (left >= 4 ? c : p.dim - 4);  // as load4_row
 #pragma unroll
-            for (int j = 0; j < U; ++j) v[j] = load4_once(dy + (long long)token[j] * p.ld_in);
+            for (int j = 0; j < U; ++j) v[j] = load4_once(at + (long long)token[j] * p.ld_in);
         } else {
 #pragma unroll
-            for (int j = 0; j < U; ++j) v[j] = load4(dy + (long long)token[j] * p.ld_in, left);
+            for (int j = 0; j < U; ++j) v[j] = load4_row(dy + (long long)token[j] * p.ld_in, c, p.dim);
         }
 #pragma unroll
         for (int j = 0; j < U; ++j) now[j] = q + j < p1 ? key[j] : -1;
@@ -380,9 +384,9 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
                     put_gradient(p, cur, c, sum);
                 came_in = false;
                 cur = now[j];
-                sum = widen(v[j]);
+                sum = existing(widen(v[j]), left, ends);
             } else {
-                sum += widen(v[j]);
+                sum += existing(widen(v[j]), left, ends);
             }
         }
     }
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
 // chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).  The same launch clears the rows that
 // no token has: the few long sums wait for memory while the stores go out.
 __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingParams p) {
-    constexpr int U = 8;
+    constexpr int U = 16;
     const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
     const int groups = 256 >> p.lanes_log2;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
@@ -459,8 +463,9 @@ constexpr long long kSmallElements = 1LL << 19;
 template <typename ID, typename T>
 __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingParams p) {
     extern __shared__ int count[];  // [16][bins], then the cursors; at the end the groups' sums, 16 KB
-    __shared__ int wave_total[16], starts[513];
+    __shared__ int wave_total[16], starts[513], long_runs[kSmallTokens / kLongRun], n_long;
     constexpr int PER = kSmallTokens / 1024, U = 8;
+    if (threadIdx.x == 0) n_long = 0;
     __shared__ unsigned short notes[16][kSmallTokens / 16], order[kSmallTokens];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, rank = blockIdx.x, bins = p.bins;
     for (int i = tid; i < 16 * bins; i += 1024) count[i] = 0;
@@ -488,7 +493,10 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
     __syncthreads();
     int start, total;
     scan_counts(count, 16, bins, 0, wave_total, start, total);
-    if (tid < bins) starts[tid] = start;
+    if (tid < bins) {
+        starts[tid] = start;
+        if (total > kLongRun) long_runs[atomicAdd(&n_long, 1)] = tid;  // (in any order: their rows have nothing to do with each other)
+    }
     if (tid == bins - 1) starts[bins] = start + total;
     for (int k = 0; k < noted; k += 64) {
         const bool in = k + lane < noted;
@@ -502,7 +510,8 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
     f32x4* sums = reinterpret_cast<f32x4*>(count);
     for (int c0 = 0; c0 < p.dim; c0 += 4 << p.lanes_log2) {
         const int c = c0 + 4 * glane, left = p.dim - c;
-        const T* dy = static_cast<const T*>(p.in) + c;
+        const bool ends = __ballot(left < 4) != 0;
+        const T* dy = static_cast<const T*>(p.in);
         // rows first, first + step ... of a run
         auto add_up = [&](int first, int last, int step) {
             f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -512,10 +521,10 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     v[j] = raw4<T>{};
-                    if (q + j * step < last) v[j] = load4(dy + (long long)order[q + j * step] * p.ld_in, left);
+                    if (q + j * step < last) v[j] = load4_row(dy + (long long)order[q + j * step] * p.ld_in, c, p.dim);
                 }
 #pragma unroll
-                for (int j = 0; j < U; ++j) sum += widen(v[j]);
+                for (int j = 0; j < U; ++j) sum += existing(widen(v[j]), left, ends);
             }
             return sum;
         };
@@ -528,9 +537,8 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
             else if (!p.accumulate)
                 store4(static_cast<float*>(p.out) + row * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         }
-        for (int number = 0; number < bins; ++number) {
-            const int a = starts[number], b = starts[number + 1];
-            if (b - a <= kLongRun) continue;  // the same for the whole workgroup
+        for (int k = 0; k < n_long; ++k) {
+            const int number = long_runs[k], a = starts[number], b = starts[number + 1];
             __syncthreads();
             sums[tid] = add_up(a + group, b, groups);
             __syncthreads();

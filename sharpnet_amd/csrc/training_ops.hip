@@ -73,7 +73,8 @@ EmbeddingPlan embedding_plan(const snhip_embedding_desc* d) {
     while ((1 << e.bins_log2) < e.bins) ++e.bins_log2;
     e.small = d->tokens <= kSmallTokens && d->tokens * d->dim <= kSmallElements && e.fine_log2 == 0;
     if (e.small) return e;
-    e.chunk = d->tokens >= 16384 ? 32 : 8;
+    // short chunks for few tokens (more threads at work), long ones for many (fewer parts of frequent words to join)
+    e.chunk = d->tokens >= 16384 ? 32 : d->tokens > kSmallTokens ? 16 : 8;
     e.chunks = (d->tokens + e.chunk - 1) / e.chunk;
     e.order = 0;
     e.sorted = e.order + up256((size_t)d->tokens * 4);

@@ -75,6 +75,31 @@ __device__ __forceinline__ void store4(T* at, int left, f32x4 v) {
         if (j < left) at[j] = (T)v[j];
 }
 
+// Columns [c, c + 4) of a row of dim elements, c a multiple of four: the loads of many rows without a branch in between.  Near
+// the row's end (and behind it) the row's last four elements are read; existing() moves those that are asked for to their
+// places and clears the rest, once they are used.
+template <typename T, bool ONCE = false>
+__device__ __forceinline__ raw4<T> load4_row(const T* row, int c, int dim) {
+    if (dim >= 4) {
+        const T* at = row + (c < dim - 4 ? c : dim - 4);
+        return ONCE ? load4_once(at) : load4_whole(at);
+    }
+    raw4<T> v = {};
+#pragma unroll
+    for (int j = 0; j < 3; ++j)  // (a row of up to three: as the end of one of four)
+        if (c == 0 && j < dim) v[j + 4 - dim] = row[j];
+    return v;
+}
+// `ends`: whether a lane of the wavefront is at a row's end (most pieces have none: nothing to do).
+__device__ __forceinline__ f32x4 existing(f32x4 v, int left, bool ends) {
+    if (!ends || left >= 4) return v;
+    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (left == 3) r = f32x4{v[1], v[2], v[3], 0.0f};
+    if (left == 2) r = f32x4{v[2], v[3], 0.0f, 0.0f};
+    if (left == 1) r[0] = v[3];
+    return r;
+}
+
 // Sums over 16 neighbouring lanes / over the wavefront, in every lane of them, without going through LDS: rotations within
 // rows of 16 lanes are free operands of the additions (ds_bpermute, what a shuffle becomes, is a round trip each).
 template <int ROTATE>
