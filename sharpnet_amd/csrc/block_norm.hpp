@@ -49,14 +49,17 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const void* row, in
 
 template <int TPR, bool EXACT>
 struct Piece {
-    static constexpr bool BUFFER = EXACT && TPR >= 64;
+    template <typename T>
+    static constexpr bool BUFFER = TPR >= 64 && (EXACT || sizeof(T) == 4);
     __device__ __forceinline__ static int column(int n, int lane) { return 4 * (n * TPR + lane); }
     template <typename T>
     __device__ __forceinline__ static raw4<T> load(const T* row, int n, int lane, int dim) {
         const int c = column(n, lane);
-        if constexpr (BUFFER) {
+        if constexpr (BUFFER<T>) {
             const __amdgpu_buffer_rsrc_t b = row_buffer(row, dim * (int)sizeof(T));
-            if constexpr (sizeof(T) == 4)
+            if constexpr (!EXACT)  // (a row of such a kernel has over 64 elements) as load4_row
+                return __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b128(b, 4 * (c < dim - 4 ? c : dim - 4), 0, 0));
+            else if constexpr (sizeof(T) == 4)
                 return __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b128(b, 4 * c, 0, 0));
             else
                 return __builtin_bit_cast(raw4<T>, __builtin_amdgcn_raw_buffer_load_b64(b, 2 * c, 0, 0));
@@ -69,10 +72,18 @@ struct Piece {
     template <typename T>
     __device__ __forceinline__ static void store(T* row, int n, int lane, int dim, f32x4 v) {
         const int c = column(n, lane);
-        if constexpr (BUFFER) {
+        if constexpr (BUFFER<T>) {
             const __amdgpu_buffer_rsrc_t b = row_buffer(row, dim * (int)sizeof(T));
             const raw4<T> r = narrow(v, static_cast<const T*>(nullptr));
-            if constexpr (sizeof(T) == 4)
+            if constexpr (!EXACT) {
+                if (c + 4 <= dim) {
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), b, 4 * c, 0, 0);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)  // (dropped behind the row's end)
+                        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned int, (float)v[j]), b, 4 * (c + j), 0, 0);
+                }
+            } else if constexpr (sizeof(T) == 4)
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, r), b, 4 * c, 0, 0);
             else
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, r), b, 2 * c, 0, 0);
@@ -83,7 +94,7 @@ struct Piece {
     // what a loaded piece is worth: zeros behind the row's end
     template <typename R>
     __device__ __forceinline__ static f32x4 value(R raw, int n, int lane, int dim) {
-        if constexpr (BUFFER)
+        if constexpr (EXACT && TPR >= 64)
             return widen(raw);
         else if constexpr (EXACT)
             return cut(widen(raw), n, lane, dim);
@@ -300,7 +311,7 @@ template <typename TS, typename TB, int TPR, int N, int MODE, bool BIAS, bool GA
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_kernel(const BlockNormParams p) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
     typedef Piece<TPR, EXACT> P;
-    constexpr bool HAS_Y = MODE == 2 || GATE;
+    constexpr bool HAS_Y = MODE == 2 || GATE, BOTH = N == 1 || TPR == 16;
     __shared__ float lds[2][2][TPR / 64 + 1];
     constexpr int VECTORS = 1 + (BIAS ? 1 : 0) + (MODE == 2 ? 1 + (BIAS ? 1 : 0) : 0) + (GATE ? 1 : 0);  // of column sums
     __shared__ f32x4 meet[GROUPS > 1 ? VECTORS * GROUPS * TPR * N : 1];
@@ -337,7 +348,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
     const bool gate_in_rows = p.gate_rows != 0;
 
     // what the norm ahead of the next block needs of a row, and what the norm behind this one needs: the first part of the
-    // next row and the second part of this one are under way while the other is worked on
+    // next row and the second part of this one are under way while the other is worked on.  (BOTH: with a piece or two to a
+    // thread the work on the first is over too soon for that, and there are registers for the next row's second part, too.)
     struct Ahead {
         raw4<TS> u[N], du[N];
         raw4<TB> dh[N];
@@ -361,19 +373,24 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
             for (int n = 0; n < N; ++n)
                 ahead.du[n] = P::load(static_cast<const TS*>(p.du) + row * p.ld_u, n, lane, dim);
     };
-    if (r < r_end) fetch_ahead(r);
-    for (; r < r_end; r += step) {
-        const bool last_of_group = p.flush && (left_in_group == 1 || r + step >= r_end);
-        Behind now = {};
+    auto fetch_behind = [&](Behind& w, long long row, long long g_row) {
         if constexpr (HAS_Y)
 #pragma unroll
-            for (int n = 0; n < N; ++n) now.y[n] = P::load(static_cast<const TB*>(p.y) + r * p.ld_y, n, lane, dim);
-        if constexpr (MODE == 2) now.mean = p.post_s[2 * r], now.rstd = p.post_s[2 * r + 1];
+            for (int n = 0; n < N; ++n) w.y[n] = P::load(static_cast<const TB*>(p.y) + row * p.ld_y, n, lane, dim);
+        if constexpr (MODE == 2) w.mean = p.post_s[2 * row], w.rstd = p.post_s[2 * row + 1];
         if constexpr (GATE)
             if (gate_in_rows)
 #pragma unroll
-                for (int n = 0; n < N; ++n)
-                    now.g[n] = P::load(static_cast<const TB*>(p.gate) + gate_row * p.ld_gate, n, lane, dim);
+                for (int n = 0; n < N; ++n) w.g[n] = P::load(static_cast<const TB*>(p.gate) + g_row * p.ld_gate, n, lane, dim);
+    };
+    Behind now = {};
+    if (r < r_end) {
+        fetch_ahead(r);
+        if constexpr (BOTH) fetch_behind(now, r, gate_row);
+    }
+    for (; r < r_end; r += step) {
+        const bool last_of_group = p.flush && (left_in_group == 1 || r + step >= r_end);
+        if constexpr (!BOTH) fetch_behind(now, r, gate_row);
         f32x4 t[N], hat[N];
         if (p.dh != nullptr) {
 #pragma unroll
@@ -392,7 +409,11 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
 #pragma unroll
             for (int n = 0; n < N; ++n) t[n] = P::value(ahead.du[n], n, lane, dim);
         }
-        if (r + step < r_end) fetch_ahead(r + step);
+        Behind next = {};
+        if (r + step < r_end) {
+            fetch_ahead(r + step);
+            if constexpr (BOTH) fetch_behind(next, r + step, last_of_group ? gate_row + 1 : gate_row);
+        }
 #pragma unroll
         for (int n = 0; n < N; ++n) P::store(static_cast<TS*>(p.dx) + r * p.ld_x, n, lane, dim, t[n]);
         if constexpr (MODE > 0) {
@@ -438,6 +459,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
         }
         if (last_of_group) ++gate_row;
         left_in_group = last_of_group ? p.rows_per_group : left_in_group - 1;
+        if constexpr (BOTH) now = next;
     }
     // the column sums of the chunk; groups of threads that share the columns meet in LDS
     auto every = [&](auto&& each) {  // the sums there are, with the slot of each

@@ -87,9 +87,9 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 // puts its tokens behind the earlier ones of their ids.  The order of all this is a function of the ids alone.
 // Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (6.6 us for 4000 tokens).
 // With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup reads its own alone
-// (65536 tokens: 34 us the first way, 22 us the second).
+// (65536 tokens: 34 us the first way, 18 us the second).
 constexpr int kSortDirect = 8192; // tokens up to which every workgroup reads all ids
-constexpr int kPiece = 1024;      // tokens that a workgroup of embedding_bucket_kernel sorts
+constexpr int kPiece = 512;       // tokens that a workgroup of embedding_bucket_kernel sorts
 constexpr int kBuckets = 256;     // ... by bucket (bucket modulo 256 if there are more)
 
 // The lanes of `in` whose value (bits wide) is this lane's.
@@ -102,7 +102,8 @@ __device__ __forceinline__ unsigned long long same_value(bool in, int value, int
     return same;
 }
 
-// A place in the counters' order for every lane of `in`: behind the earlier tokens of the same value, by lane.
+// The place of every lane of `in` among the wavefront's tokens of its value: behind those that `cursors` has counted so far
+// and those of the lanes before; counts them.
 __device__ __forceinline__ int take_place(bool in, int value, int bits, int* cursors) {
     const int lane = threadIdx.x & 63;
     const unsigned long long before = (1ULL << lane) - 1, same = same_value(in, value, bits);
@@ -115,13 +116,18 @@ __device__ __forceinline__ int take_place(bool in, int value, int bits, int* cur
     return at;
 }
 
-// count[waves][values] becomes the places where each wavefront's tokens of each value start, from `first` on; start: where
+// count[WAVES][values] becomes the places where each wavefront's tokens of each value start, from `first` on; start: where
 // the value of this thread (threadIdx.x < values) starts, total: how many there are of it.  values <= 512, one per thread.
-__device__ __forceinline__ void scan_counts(int* count, int waves, int values, int first, int* wave_total, int& start, int& total) {
+template <int WAVES>
+__device__ __forceinline__ void scan_counts(int* count, int values, int first, int* wave_total, int& start, int& total) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    int n[WAVES];
     total = 0;
-    if (tid < values)
-        for (int k = 0; k < waves; ++k) total += count[k * values + tid];
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+        n[k] = tid < values ? count[k * values + tid] : 0;
+        total += n[k];
+    }
     int upto = total;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -131,14 +137,13 @@ __device__ __forceinline__ void scan_counts(int* count, int waves, int values, i
     if (lane == 63) wave_total[w] = upto;
     __syncthreads();
     start = first + upto - total;
-    for (int k = 0; k < w; ++k) start += wave_total[k];
-    if (tid < values) {
-        int at = start;
-        for (int k = 0; k < waves; ++k) {
-            const int n = count[k * values + tid];
-            count[k * values + tid] = at;
-            at += n;
-        }
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) start += k < w ? wave_total[k] : 0;
+    int at = start;
+#pragma unroll
+    for (int k = 0; k < WAVES; ++k) {
+        if (tid < values) count[k * values + tid] = at;
+        at += n[k];
     }
     __syncthreads();
 }
@@ -161,12 +166,12 @@ __global__ void __launch_bounds__(256) embedding_bucket_kernel(const EmbeddingPa
         if (id[j] == p.padding) id[j] = -1;
     }
     __syncthreads();
+    int place[PER];  // among the wavefront's tokens of the bucket
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-        if (id[j] >= 0) atomicAdd(&count[w * kBuckets + (id[j] & mask)], 1);
+    for (int j = 0; j < PER; ++j) place[j] = take_place(id[j] >= 0, id[j] & mask, 8, count + w * kBuckets);
     __syncthreads();
     int start, total;
-    scan_counts(count, 4, kBuckets, 0, wave_total, start, total);
+    scan_counts<4>(count, kBuckets, 0, wave_total, start, total);
     int* starts = p.piece_start + blockIdx.x;
     starts[(long long)tid * p.pieces] = start;
     if (tid == kBuckets - 1) {
@@ -175,8 +180,9 @@ __global__ void __launch_bounds__(256) embedding_bucket_kernel(const EmbeddingPa
     }
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int at = take_place(id[j] >= 0, id[j] & mask, 8, count + w * kBuckets);
-        if (id[j] >= 0) sorted_id[at] = id[j], sorted_token[at] = (int)(t0 + 64 * j);
+        if (id[j] < 0) continue;
+        const int at = count[w * kBuckets + (id[j] & mask)] + place[j];
+        sorted_id[at] = id[j], sorted_token[at] = (int)(t0 + 64 * j);
     }
     __syncthreads();
     const int n = wave_total[0];
@@ -196,8 +202,9 @@ __device__ __forceinline__ int rank_of_id(const EmbeddingParams& p, int id) {
 __device__ __forceinline__ void start_ids(const EmbeddingParams& p, int* count, const int* below, int* wave_total) {
     const int tid = threadIdx.x, rank = blockIdx.x;
     int first = 0, start, total;
+#pragma unroll
     for (int k = 0; k < 16; ++k) first += below[k];
-    scan_counts(count, 16, p.bins, first, wave_total, start, total);
+    scan_counts<16>(count, p.bins, first, wave_total, start, total);
     if (tid < p.bins) p.offsets[rank * p.bins + tid] = start;
     if (rank == p.sort_blocks - 1 && tid == p.bins - 1) p.offsets[p.sort_blocks * p.bins] = start + total;
 }
@@ -260,54 +267,72 @@ __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const Embed
     const int begin = w * per < p.pieces ? w * per : p.pieces, end = begin + per < p.pieces ? begin + per : p.pieces;
     const int* from = p.piece_start + (long long)(rank >> p.fine_log2) * p.pieces;
     const int* to = from + p.pieces;
-    int smaller = 0;
-    // All tokens of the pieces' lists, eight pieces at a time: a piece has a handful of tokens of a bucket, and one after the
-    // other each would wait for memory.
-    auto walk = [&](bool tokens, auto&& visit) {
-        constexpr int U = 8;
-        for (int i0 = begin; i0 < end; i0 += U) {
-            int a[U], b[U], longest = 0;
+    // Eight pieces at a time: a piece has a handful of tokens of a bucket, and one after the other each would wait for memory.
+    constexpr int U = 8;
+    int a[U], b[U], longest = 0, id[U], token[U], place[U];
+    int* counts = count + w * p.bins;  // this wavefront's
+    auto bounds = [&](int i0) {
+        longest = 0;
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                const int i = i0 + j < end ? i0 + j : end - 1;
-                a[j] = from[i], b[j] = i0 + j < end ? to[i] : 0;
-                longest = b[j] - a[j] > longest ? b[j] - a[j] : longest;
-            }
-            for (int k = 0; k < longest; k += 64) {
-                int id[U], token[U];
+        for (int j = 0; j < U; ++j) {
+            const int i = i0 + j < end ? i0 + j : end - 1;
+            a[j] = from[i], b[j] = i0 + j < end ? to[i] : 0;
+        }
 #pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    const int at = a[j] + k + lane;
-                    const long long place = (long long)(i0 + j) * kPiece + at;
-                    id[j] = at < b[j] ? p.piece_id[place] : -1;
-                    token[j] = tokens && at < b[j] ? p.piece_token[place] : 0;
-                }
+        for (int j = 0; j < U; ++j) longest = b[j] - a[j] > longest ? b[j] - a[j] : longest;
+    };
+    auto fetch = [&](int i0, int k) {  // up to 64 tokens of each, from the k-th on
 #pragma unroll
-                for (int j = 0; j < U; ++j) visit(id[j], token[j]);
-            }
+        for (int j = 0; j < U; ++j) {
+            const int at = a[j] + k + lane;
+            const long long place = (long long)(i0 + j) * kPiece + at;
+            id[j] = at < b[j] ? p.piece_id[place] : -1;
+            token[j] = at < b[j] ? p.piece_token[place] : 0;
         }
     };
-    for (int i = begin + lane; i < end; i += 64) smaller += from[i];
-    walk(false, [&](int id, int) {
-        if (id < 0) return;
-        const int r = rank_of_id(p, id);
-        if (r == rank)
-            atomicAdd(&count[w * p.bins + (id >> p.sort_log2)], 1);
-        else
-            smaller += r < rank;
-    });
+    int smaller = 0;
+    for (int i0 = begin; i0 < end; i0 += U) {
+        bounds(i0);
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (lane == 0 && i0 + j < end) smaller += a[j];
+        for (int k = 0; k < longest; k += 64) {
+            fetch(i0, k);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const int r = rank_of_id(p, id[j]);
+                smaller += id[j] >= 0 && r < rank;
+                if (r != rank) id[j] = -1;
+                if (__ballot(id[j] >= 0) != 0) place[j] = take_place(id[j] >= 0, id[j] >> p.sort_log2, p.bins_log2, counts);
+            }
+        }
+    }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) smaller += __shfl_xor(smaller, off, 64);
     if (lane == 0) below[w] = smaller;
     __syncthreads();
     start_ids(p, count, below, wave_total);
-    walk(true, [&](int id, int token) {
-        const bool in = id >= 0 && rank_of_id(p, id) == rank;
-        if (__ballot(in) == 0) return;
-        const int number = in ? id >> p.sort_log2 : 0;
-        const int at = take_place(in, number, p.bins_log2, count + w * p.bins);
-        if (in) p.order[at] = token, p.sorted[at] = rank * p.bins + number;
-    });
+    const bool held = begin < end && end - begin <= U && longest > 0 && longest <= 64;  // all of this wavefront's tokens are in its registers still
+    auto put = [&](int j, int at) { p.order[at] = token[j], p.sorted[at] = rank * p.bins + (id[j] >> p.sort_log2); };
+    if (held) {
+#pragma unroll
+        for (int j = 0; j < U; ++j)
+            if (id[j] >= 0) put(j, counts[id[j] >> p.sort_log2] + place[j]);
+        return;
+    }
+    for (int i0 = begin; i0 < end; i0 += U) {
+        bounds(i0);
+        for (int k = 0; k < longest; k += 64) {
+            fetch(i0, k);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                const bool in = id[j] >= 0 && rank_of_id(p, id[j]) == rank;
+                if (__ballot(in) == 0) continue;
+                const int at = take_place(in, id[j] >> p.sort_log2, p.bins_log2, counts);
+                if (in) put(j, at);
+            }
+        }
+    }
 }
 
 __device__ __forceinline__ int id_of_key(const EmbeddingParams& p, int key) {
@@ -403,6 +428,8 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
         put_gradient(p, cur, c, sum);
 }
 
+constexpr int kClearRows = 8;  // that a group of threads looks at
+
 // The rows whose run crosses the end of a chunk: the group of the chunk where the run starts adds its part and those of the
 // chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).  The same launch clears the rows that
 // no token has: the few long sums wait for memory while the stores go out.
@@ -413,22 +440,20 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
     const int left = p.dim - c;
-    if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has
-        constexpr int ROWS = 8;
-        const long long r0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * ROWS;
-        bool clear[ROWS];
+    if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has, in the order of their keys: neighbours in `offsets`
+        const int keys = p.sort_blocks * p.bins;
+        const long long k0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * kClearRows;
+        if (k0 >= keys) return;
+        const int first = (int)k0, here = keys - first < kClearRows ? keys - first : kClearRows;
+        int at[kClearRows + 1];
 #pragma unroll
-        for (int k = 0; k < ROWS; ++k) {
-            const int r = (int)(r0 + k);
-            clear[k] = r0 + k < p.vocabulary;
-            if (clear[k]) {
-                const int key = rank_of_id(p, r) * p.bins + (r >> p.sort_log2);
-                clear[k] = p.offsets[key] == p.offsets[key + 1];
-            }
+        for (int k = 0; k <= kClearRows; ++k) at[k] = p.offsets[first + (k < here ? k : here)];
+#pragma unroll
+        for (int k = 0; k < kClearRows; ++k) {
+            const int id = id_of_key(p, first + k);
+            if (k < here && at[k] == at[k + 1] && id < p.vocabulary)
+                store4(static_cast<float*>(p.out) + (long long)id * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         }
-#pragma unroll
-        for (int k = 0; k < ROWS; ++k)
-            if (clear[k]) store4(static_cast<float*>(p.out) + (r0 + k) * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         return;
     }
     const long long k = (long long)blockIdx.x * groups + group;
@@ -492,7 +517,7 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
     }
     __syncthreads();
     int start, total;
-    scan_counts(count, 16, bins, 0, wave_total, start, total);
+    scan_counts<16>(count, bins, 0, wave_total, start, total);
     if (tid < bins) {
         starts[tid] = start;
         if (total > kLongRun) long_runs[atomicAdd(&n_long, 1)] = tid;  // (in any order: their rows have nothing to do with each other)

@@ -407,7 +407,8 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
         embedding_sort_launch<int>(p, sort_grid, lds, h->stream);
     else
         embedding_sort_launch<long long>(p, sort_grid, lds, h->stream);
-    const long long clear_blocks = p.accumulate ? 0 : ((long long)p.vocabulary + 8 * groups - 1) / (8 * groups);
+    const long long keys = (long long)p.sort_blocks * p.bins;
+    const long long clear_blocks = p.accumulate ? 0 : (keys + kClearRows * groups - 1) / (kClearRows * groups);
     const dim3 chunk_grid((unsigned)p.chunk_blocks, (unsigned)col_blocks);
     if (p.chunk_blocks > 0) {
         if (desc->output_type == SNHIP_TYPE_BF16)
