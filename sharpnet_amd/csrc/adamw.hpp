@@ -1,6 +1,10 @@
 // AdamW over the elements of many tensors in one launch (definitions: include/sharpnet_hip.h, snhip_adamw_create).
 // Bound by HBM: 28 bytes an element with states in 32 bits, 16 with states in 8 (and an fp32 gradient), each read and
-// written once.  ONCE: around the caches, for plans that are larger than they are (kAdamwOnce).
+// written once; the 8-bit form comes near the vector units' rate, too (some 90 instructions an element, a third of them the
+// random words).
+// A workgroup of 256 threads updates a chunk of a tensor, one or four turns of 1024 elements, four neighbours to a thread and
+// turn.  MANY: a plan of kAdamwMany elements or more, in chunks of four turns and around the caches.
+// FULL: all of a turn's elements exist; the tail of a tensor goes the other way.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -11,12 +15,14 @@ namespace snhip {
 
 typedef unsigned int u32_any __attribute__((aligned(1)));  // four bytes at any address
 
-constexpr int kAdamwBlock = 256;   // elements that share a power of two (states in 8 bits)
-constexpr int kAdamwChunk = 4096;  // elements of a tensor that a workgroup of 256 threads updates
-
-// Elements from which on a plan's data does not go through the caches: a step on 4 million (112 MB of fp32 states) finds some
-// of it in the 256 MB behind the L2s again, a step on more than they hold does not and runs at 5.3 instead of 5.15 TB/s.
-constexpr long long kAdamwOnce = 1LL << 23;
+constexpr int kAdamwBlock = 256;  // elements that share a power of two (states in 8 bits)
+constexpr int kAdamwTurn = 1024;  // elements of a workgroup's turn
+// Elements from which on a chunk is four turns (2048 chunks, eight for each compute unit: below that one turn a chunk brings
+// more threads to work) and the data does not go through the caches: a step on 4 million (112 MB of fp32 states) finds some
+// of it in the 256 MB behind the L2s again, a step on more than they hold does not and runs at 5.45 instead of 5.15 TB/s.
+constexpr long long kAdamwMany = 1LL << 23;
+template <bool MANY>
+constexpr int kAdamwTurns = MANY ? 4 : 1;
 
 struct AdamwEntry {
     float* p;
@@ -48,71 +54,128 @@ __device__ __forceinline__ float moment2(float v, float g, const AdamwScalars& s
     const float a = v * s.beta2, b = (g * g) * s.rest2;
     return a + b;
 }
-// (the hardware's reciprocal, 1 ulp: the denominator is 0 or between 1e-23 and 1e20, where it is exact to that)
+// (The hardware's square root, 1 ulp for a normal number: a smaller one goes in times 2^96.  The hardware's reciprocal, 1 ulp:
+// the denominator is 0 or between 1e-23 and 1e20.)
 __device__ __forceinline__ float new_parameter(float p, float m, float v, float keep, const AdamwScalars& s) {
-    return p * keep - s.step_size * (m * __builtin_amdgcn_rcpf(sqrtf(v) * s.root_scale + s.eps));
+    const bool tiny = v < 0x1p-96f;
+    const float root = __builtin_amdgcn_sqrtf(tiny ? v * 0x1p+96f : v) * (tiny ? s.root_scale * 0x1p-48f : s.root_scale);
+    return p * keep - s.step_size * (m * __builtin_amdgcn_rcpf(root + s.eps));
 }
 
+// ---- access ------------------------------------------------------------------------------------------------------
+// Elements [i, i + 4) from a base that is the same for the whole wavefront (`left` of them exist if not FULL).  The addresses
+// come out of a table in memory: that they are global memory has to be said.
+#define SNHIP_GLOBAL __attribute__((address_space(1)))
+template <typename T, bool ONCE, bool FULL>
+__device__ __forceinline__ raw4<T> take4(const T* base, unsigned int i, int left) {
+    if constexpr (FULL) {
+        typedef typename Raw4<T>::any any;
+        const SNHIP_GLOBAL any* at = (const SNHIP_GLOBAL any*)((const SNHIP_GLOBAL char*)base + i * (unsigned int)sizeof(T));
+        return ONCE ? __builtin_nontemporal_load(at) : *at;
+    } else {
+        return load4<T, ONCE>(base + i, left);
+    }
+}
+template <typename T, bool ONCE, bool FULL>
+__device__ __forceinline__ void give4(T* base, unsigned int i, int left, f32x4 v) {
+    if constexpr (FULL) {
+        typedef typename Raw4<T>::any any;
+        SNHIP_GLOBAL any* at = (SNHIP_GLOBAL any*)((SNHIP_GLOBAL char*)base + i * (unsigned int)sizeof(T));
+        if (ONCE)
+            __builtin_nontemporal_store(narrow(v, static_cast<const T*>(nullptr)), at);
+        else
+            *at = narrow(v, static_cast<const T*>(nullptr));
+    } else {
+        store4<T, ONCE>(base + i, left, v);
+    }
+}
+// four bytes of an 8-bit state
+template <bool FULL>
+__device__ __forceinline__ unsigned int take_bytes(const unsigned char* base, unsigned int i, int left) {
+    if constexpr (FULL) return *(const SNHIP_GLOBAL u32_any*)((const SNHIP_GLOBAL char*)base + i);
+    unsigned int bytes = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < left) bytes |= (unsigned int)base[i + j] << (8 * j);
+    return bytes;
+}
+template <bool FULL>
+__device__ __forceinline__ void give_bytes(unsigned char* base, unsigned int i, int left, unsigned int bytes) {
+    if constexpr (FULL) {
+        *(SNHIP_GLOBAL u32_any*)((SNHIP_GLOBAL char*)base + i) = bytes;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (j < left) base[i + j] = (unsigned char)(bytes >> (8 * j));
+}
 // Four elements of the gradient as they lie in memory, and what they are worth: the conversion is kept away from the load,
 // so that the other loads of the same elements do not wait for it.
 struct RawGradient {
     f32x4 f;
     bf16x4 b;
 };
-template <bool ONCE>
-__device__ __forceinline__ RawGradient load_gradient(const AdamwEntry& t, long long i, int left) {
-    RawGradient r;
+template <bool ONCE, bool FULL>
+__device__ __forceinline__ RawGradient take_gradient(const AdamwEntry& t, long long from, unsigned int i, int left) {
+    RawGradient r = {};
     if (t.g_bf16)
-        r.b = load4<__bf16, ONCE>(static_cast<const __bf16*>(t.g) + i, left);
+        r.b = take4<__bf16, ONCE, FULL>(static_cast<const __bf16*>(t.g) + from, i, left);
     else
-        r.f = load4<float, ONCE>(static_cast<const float*>(t.g) + i, left);
+        r.f = take4<float, ONCE, FULL>(static_cast<const float*>(t.g) + from, i, left);
     return r;
 }
 __device__ __forceinline__ f32x4 gradient_of(const AdamwEntry& t, const RawGradient& r, float scale) {
     return (t.g_bf16 ? widen(r.b) : r.f) * scale;
 }
 
-template <bool ONCE>
+// ---- states in 32 bits -----------------------------------------------------------------------------------------------
+template <bool ONCE, bool FULL>
+__device__ __forceinline__ void adamw32_turn(const AdamwEntry& t, long long from, float keep, const AdamwScalars& s) {
+    const unsigned int i = threadIdx.x * 4;
+    const int left = FULL || t.count - from - i >= 4 ? 4 : (int)(t.count - from - i);
+    if (left <= 0) return;
+    float *p = t.p + from, *m = static_cast<float*>(t.m) + from, *v = static_cast<float*>(t.v) + from;
+    const RawGradient raw = take_gradient<ONCE, FULL>(t, from, i, left);
+    f32x4 pp = take4<float, ONCE, FULL>(p, i, left), mm = take4<float, ONCE, FULL>(m, i, left), vv = take4<float, ONCE, FULL>(v, i, left);
+    const f32x4 g = gradient_of(t, raw, s.grad_scale);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        mm[j] = moment1(mm[j], g[j], s);
+        vv[j] = moment2(vv[j], g[j], s);
+        pp[j] = new_parameter(pp[j], mm[j], vv[j], keep, s);
+    }
+    give4<float, ONCE, FULL>(p, i, left, pp);
+    give4<float, ONCE, FULL>(m, i, left, mm);
+    give4<float, ONCE, FULL>(v, i, left, vv);
+    if (t.copy != nullptr) give4<__bf16, ONCE, FULL>(t.copy + from, i, left, pp);
+}
+
+template <bool MANY>
 __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
                                                       AdamwScalars s) {
     const AdamwEntry t = entries[owner[blockIdx.x]];
-    const long long base = (blockIdx.x - t.first_chunk) * kAdamwChunk;
+    const long long base = (blockIdx.x - t.first_chunk) * (kAdamwTurns<MANY> * kAdamwTurn);
     const float keep = 1.0f - s.rate * t.decay;
-    float *m = static_cast<float*>(t.m), *v = static_cast<float*>(t.v);
+    if (base + kAdamwTurns<MANY> * kAdamwTurn <= t.count) {
 #pragma unroll
-    for (int k = 0; k < kAdamwChunk / 1024; ++k) {
-        const long long i = base + k * 1024 + threadIdx.x * 4;
-        if (i >= t.count) break;
-        const int left = t.count - i < 4 ? (int)(t.count - i) : 4;
-        const RawGradient raw = load_gradient<ONCE>(t, i, left);
-        f32x4 pp = load4<float, ONCE>(t.p + i, left), mm = load4<float, ONCE>(m + i, left), vv = load4<float, ONCE>(v + i, left);
-        const f32x4 g = gradient_of(t, raw, s.grad_scale);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mm[j] = moment1(mm[j], g[j], s);
-            vv[j] = moment2(vv[j], g[j], s);
-            pp[j] = new_parameter(pp[j], mm[j], vv[j], keep, s);
-        }
-        store4<float, ONCE>(t.p + i, left, pp);
-        store4<float, ONCE>(m + i, left, mm);
-        store4<float, ONCE>(v + i, left, vv);
-        if (t.copy != nullptr) store4<__bf16, ONCE>(t.copy + i, left, pp);
+        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw32_turn<MANY, true>(t, base + k * kAdamwTurn, keep, s);
+    } else {
+        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw32_turn<MANY, false>(t, base + k * kAdamwTurn, keep, s);
     }
 }
 
-// ---- states in 8 bits ------------------------------------------------------------------------------------------
-// |x| (already divided by its block's power of two) as k steps of its binade, k rounded up where the 16 random bits ask
-// for it: MANTISSA bits after the point, binades from 2^LOWEST on (below it the step stays, as in the format).
+// ---- states in 8 bits ------------------------------------------------------------------------------------------------
+// |x| >= 0 (already divided by its block's power of two) rounded up or down by 16 random bits to MANTISSA bits after the point,
+// below 2^LOWEST to a multiple of 2^(LOWEST - MANTISSA).  A normal number takes the random bits below its last kept one, a
+// carry going into the exponent as it should; a smaller one does the same as a fixed-point number.
 template <int MANTISSA, int LOWEST>
-__device__ __forceinline__ float round_at_random(float x, unsigned int random, bool never_zero) {
-    const float a = fabsf(x);
-    int e = (int)(__float_as_uint(a) >> 23) - 127;
-    if (e < LOWEST) e = LOWEST;
-    // a / 2^(e - 23): a whole number for a normal number of the format, cut to one below
-    const unsigned int whole = (unsigned int)(a * __uint_as_float((unsigned int)(23 - e + 127) << 23));
-    unsigned int k = (whole + (random << (7 - MANTISSA))) >> (23 - MANTISSA);
+__device__ __forceinline__ float round_at_random(float a, unsigned int random, bool never_zero) {
+    const unsigned int add = random << (7 - MANTISSA);
+    const float normal = __uint_as_float((__float_as_uint(a) + add) & ~((1u << (23 - MANTISSA)) - 1u));
+    unsigned int k = ((unsigned int)(a * __uint_as_float((unsigned int)(23 - LOWEST + 127) << 23)) + add) >> (23 - MANTISSA);
     if (never_zero && k == 0 && a > 0.0f) k = 1;
-    return copysignf((float)k * __uint_as_float((unsigned int)(e - MANTISSA + 127) << 23), x);
+    const float small = (float)k * __uint_as_float((unsigned int)(LOWEST - MANTISSA + 127) << 23);
+    return a < __uint_as_float((unsigned int)(LOWEST + 127) << 23) ? small : normal;
 }
 
 // The scale byte of a block whose largest finite magnitude has the bits `top`.
@@ -121,104 +184,118 @@ __device__ __forceinline__ unsigned int scale_code(unsigned int top, int room) {
     return e < 1 ? 1u : (unsigned int)e;
 }
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((unsigned int)(e + 127) << 23); }
-// bits of |x|, 0 where it is not finite
-__device__ __forceinline__ unsigned int magnitude(float x) {
+// bits of |x|; 0 where it is not finite and that is asked for
+__device__ __forceinline__ unsigned int magnitude(float x, bool finite_only) {
     const unsigned int b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
+    return finite_only && b >= 0x7f800000u ? 0u : b;
+}
+// the largest over the wavefront
+template <int ROTATE>
+__device__ __forceinline__ unsigned int max_rotated(unsigned int v) {
+    const unsigned int o = (unsigned int)__builtin_amdgcn_update_dpp(0, (int)v, 0x120 + ROTATE, 0xf, 0xf, false);
+    return v > o ? v : o;
+}
+__device__ __forceinline__ unsigned int wave64_max(unsigned int v) {
+    v = max_rotated<1>(max_rotated<2>(max_rotated<4>(max_rotated<8>(v))));
+    const unsigned int a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+    const unsigned int c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+    const unsigned int ab = a > b ? a : b, cd = c > d ? c : d;
+    return ab > cd ? ab : cd;
 }
 
-// A wavefront takes blocks of 256 elements, four to a lane: the block's largest magnitudes meet by shuffles, the moments
-// go back to 8 bits in the registers they were computed in.
-template <bool ONCE>
+// The new states of a block: its elements' moments in the lanes (zeros behind the tensor's end).
+template <bool FULL>
+__device__ __forceinline__ void store_states(const AdamwEntry& t, long long from, unsigned int i, int left, const f32x4& mm, const f32x4& vv,
+                                             int tensor, const AdamwScalars& s) {
+    unsigned int m_top = 0, v_top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const unsigned int a = magnitude(mm[j], false), b = magnitude(vv[j], false);
+        m_top = a > m_top ? a : m_top, v_top = b > v_top ? b : v_top;
+    }
+    m_top = wave64_max(m_top), v_top = wave64_max(v_top);
+    const bool broken = m_top >= 0x7f800000u || v_top >= 0x7f800000u;  // (of the wavefront)
+    if (broken) {
+        m_top = v_top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const unsigned int a = magnitude(mm[j], true), b = magnitude(vv[j], true);
+            m_top = a > m_top ? a : m_top, v_top = b > v_top ? b : v_top;
+        }
+        m_top = wave64_max(m_top), v_top = wave64_max(v_top);
+    }
+    const unsigned int m_code = scale_code(m_top, 7), v_code = scale_code(v_top, 14);
+    const float m_inv = power_of_two(127 - (int)m_code), v_inv = power_of_two(127 - (int)v_code);
+    const unsigned long long quad = (unsigned long long)(from + i) >> 2;
+    const Philox4 r = philox4x32_10((unsigned int)quad, (unsigned int)(quad >> 32), (unsigned int)tensor, s.step, s.key0, s.key1);
+    f32x4 m_out, v_out;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float a = fabsf(mm[j] * m_inv), b = vv[j] * v_inv;
+        if (broken) a = a < __builtin_inff() ? a : 0.0f, b = b < __builtin_inff() ? b : 0.0f;
+        m_out[j] = copysignf(round_at_random<3, -6>(a, r.v[j] & 0xffffu, false), mm[j]);
+        v_out[j] = round_at_random<2, -14>(b, r.v[j] >> 16, true);
+    }
+    // (the values are exact in their formats: the conversions round nothing)
+    unsigned int m_word = 0, v_word = 0;
+    m_word = __builtin_amdgcn_cvt_pk_fp8_f32(m_out[0], m_out[1], m_word, false);
+    m_word = __builtin_amdgcn_cvt_pk_fp8_f32(m_out[2], m_out[3], m_word, true);
+    v_word = __builtin_amdgcn_cvt_pk_bf8_f32(v_out[0], v_out[1], v_word, false);
+    v_word = __builtin_amdgcn_cvt_pk_bf8_f32(v_out[2], v_out[3], v_word, true);
+    if (broken) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {  // 0x7f: NaN in both formats
+            if (magnitude(mm[j], false) >= 0x7f800000u) m_word = (m_word & ~(0xffu << (8 * j))) | 0x7fu << (8 * j);
+            if (magnitude(vv[j], false) >= 0x7f800000u) v_word = (v_word & ~(0xffu << (8 * j))) | 0x7fu << (8 * j);
+        }
+    }
+    give_bytes<FULL>(static_cast<unsigned char*>(t.m) + from, i, left, m_word);
+    give_bytes<FULL>(static_cast<unsigned char*>(t.v) + from, i, left, v_word);
+    const long long block = from / kAdamwBlock;
+    if ((threadIdx.x & 63) == 0) t.m_scale[block] = (unsigned char)m_code, t.v_scale[block] = (unsigned char)v_code;
+}
+
+// A wavefront's block of 256 elements: the block's largest magnitudes meet by rotations, the moments go back to 8 bits in the
+// registers they were computed in.
+template <bool ONCE, bool FULL>
+__device__ __forceinline__ void adamw8_block(const AdamwEntry& t, long long from, int tensor, float keep, const AdamwScalars& s) {
+    if (!FULL && from >= t.count) return;
+    const unsigned int i = (threadIdx.x & 63) * 4;
+    const int left = FULL || t.count - from - i >= 4 ? 4 : (int)(t.count - from - i);  // <= 0: behind the tensor's end
+    const long long block = from / kAdamwBlock;
+    const RawGradient raw = take_gradient<ONCE, FULL>(t, from, i, left);
+    f32x4 pp = take4<float, ONCE, FULL>(t.p + from, i, left), mm, vv;
+    const unsigned int mbits = take_bytes<FULL>(static_cast<const unsigned char*>(t.m) + from, i, left);
+    const unsigned int vbits = take_bytes<FULL>(static_cast<const unsigned char*>(t.v) + from, i, left);
+    const float m_unit = power_of_two((int)t.m_scale[block] - 127), v_unit = power_of_two((int)t.v_scale[block] - 127);
+    const f32x4 g = gradient_of(t, raw, s.grad_scale);
+    mm[0] = __builtin_amdgcn_cvt_f32_fp8(mbits, 0), mm[1] = __builtin_amdgcn_cvt_f32_fp8(mbits, 1);
+    mm[2] = __builtin_amdgcn_cvt_f32_fp8(mbits, 2), mm[3] = __builtin_amdgcn_cvt_f32_fp8(mbits, 3);
+    vv[0] = __builtin_amdgcn_cvt_f32_bf8(vbits, 0), vv[1] = __builtin_amdgcn_cvt_f32_bf8(vbits, 1);
+    vv[2] = __builtin_amdgcn_cvt_f32_bf8(vbits, 2), vv[3] = __builtin_amdgcn_cvt_f32_bf8(vbits, 3);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        mm[j] = moment1(mm[j] * m_unit, g[j], s);
+        vv[j] = moment2(vv[j] * v_unit, g[j], s);
+        pp[j] = new_parameter(pp[j], mm[j], vv[j], keep, s);
+    }
+    give4<float, ONCE, FULL>(t.p + from, i, left, pp);
+    if (t.copy != nullptr) give4<__bf16, ONCE, FULL>(t.copy + from, i, left, pp);
+    store_states<FULL>(t, from, i, left, mm, vv, tensor, s);
+}
+
+template <bool MANY>
 __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
                                                      AdamwScalars s) {
-    const int tensor = owner[blockIdx.x];
+    const int tensor = owner[blockIdx.x], w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AdamwEntry t = entries[tensor];
-    const long long base = (blockIdx.x - t.first_chunk) * kAdamwChunk;
+    const long long base = (blockIdx.x - t.first_chunk) * (kAdamwTurns<MANY> * kAdamwTurn) + w * kAdamwBlock;
     const float keep = 1.0f - s.rate * t.decay;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    unsigned char *m8 = static_cast<unsigned char*>(t.m), *v8 = static_cast<unsigned char*>(t.v);
+    if (base + (kAdamwTurns<MANY> - 1) * kAdamwTurn + kAdamwBlock <= t.count) {
 #pragma unroll
-    for (int k = 0; k < kAdamwChunk / 1024; ++k) {
-        const long long b0 = base + (4 * k + w) * kAdamwBlock;  // the wavefront's block
-        if (b0 >= t.count) break;
-        const long long i = b0 + lane * 4;
-        const int left = t.count - i < 4 ? (int)(t.count - i) : 4;  // <= 0: behind the tensor's end
-        unsigned int mbits = 0, vbits = 0;
-        RawGradient raw = {};
-        f32x4 pp = {0.0f, 0.0f, 0.0f, 0.0f}, mm, vv;
-        if (left > 0) {
-            raw = load_gradient<ONCE>(t, i, left);
-            pp = load4<float, ONCE>(t.p + i, left);
-            if (left == 4) {
-                mbits = *reinterpret_cast<const u32_any*>(m8 + i);
-                vbits = *reinterpret_cast<const u32_any*>(v8 + i);
-            } else {
-                for (int j = 0; j < left; ++j) {
-                    mbits |= (unsigned int)m8[i + j] << (8 * j);
-                    vbits |= (unsigned int)v8[i + j] << (8 * j);
-                }
-            }
-        }
-        const f32x4 g = gradient_of(t, raw, s.grad_scale);
-        const long long block = b0 / kAdamwBlock;
-        const float m_unit = power_of_two((int)t.m_scale[block] - 127), v_unit = power_of_two((int)t.v_scale[block] - 127);
-        mm[0] = __builtin_amdgcn_cvt_f32_fp8(mbits, 0), mm[1] = __builtin_amdgcn_cvt_f32_fp8(mbits, 1);
-        mm[2] = __builtin_amdgcn_cvt_f32_fp8(mbits, 2), mm[3] = __builtin_amdgcn_cvt_f32_fp8(mbits, 3);
-        vv[0] = __builtin_amdgcn_cvt_f32_bf8(vbits, 0), vv[1] = __builtin_amdgcn_cvt_f32_bf8(vbits, 1);
-        vv[2] = __builtin_amdgcn_cvt_f32_bf8(vbits, 2), vv[3] = __builtin_amdgcn_cvt_f32_bf8(vbits, 3);
-        unsigned int m_top = 0, v_top = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            mm[j] = moment1(mm[j] * m_unit, g[j], s);
-            vv[j] = moment2(vv[j] * v_unit, g[j], s);
-            pp[j] = new_parameter(pp[j], mm[j], vv[j], keep, s);
-            const unsigned int a = magnitude(mm[j]), b = magnitude(vv[j]);
-            m_top = a > m_top ? a : m_top;
-            v_top = b > v_top ? b : v_top;
-        }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const unsigned int a = (unsigned int)__shfl_xor((int)m_top, off, 64), b = (unsigned int)__shfl_xor((int)v_top, off, 64);
-            m_top = a > m_top ? a : m_top;
-            v_top = b > v_top ? b : v_top;
-        }
-        const unsigned int m_code = scale_code(m_top, 7), v_code = scale_code(v_top, 14);
-        const float m_inv = power_of_two(127 - (int)m_code), v_inv = power_of_two(127 - (int)v_code);
-        const Philox4 r = philox4x32_10((unsigned int)(i >> 2), (unsigned int)(i >> 34), (unsigned int)tensor, s.step, s.key0, s.key1);
-        unsigned int m_bytes[4], v_bytes[4];
-        float m_out[4], v_out[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const bool m_ok = fabsf(mm[j]) < __builtin_inff(), v_ok = fabsf(vv[j]) < __builtin_inff();
-            m_out[j] = round_at_random<3, -6>(m_ok ? mm[j] * m_inv : 0.0f, r.v[j] & 0xffffu, false);
-            v_out[j] = round_at_random<2, -14>(v_ok ? vv[j] * v_inv : 0.0f, r.v[j] >> 16, true);
-        }
-        // (the values are exact in their formats: the conversions round nothing)
-        unsigned int m_word = 0, v_word = 0;
-        m_word = __builtin_amdgcn_cvt_pk_fp8_f32(m_out[0], m_out[1], m_word, false);
-        m_word = __builtin_amdgcn_cvt_pk_fp8_f32(m_out[2], m_out[3], m_word, true);
-        v_word = __builtin_amdgcn_cvt_pk_bf8_f32(v_out[0], v_out[1], v_word, false);
-        v_word = __builtin_amdgcn_cvt_pk_bf8_f32(v_out[2], v_out[3], v_word, true);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m_bytes[j] = (m_word >> (8 * j)) & 0xffu, v_bytes[j] = (v_word >> (8 * j)) & 0xffu;
-            if (!(fabsf(mm[j]) < __builtin_inff())) m_bytes[j] = 0x7fu;  // NaN in both formats
-            if (!(fabsf(vv[j]) < __builtin_inff())) v_bytes[j] = 0x7fu;
-        }
-        if (left > 0) {
-            store4<float, ONCE>(t.p + i, left, pp);
-            if (t.copy != nullptr) store4<__bf16, ONCE>(t.copy + i, left, pp);
-            if (left == 4) {
-                *reinterpret_cast<u32_any*>(m8 + i) = m_bytes[0] | m_bytes[1] << 8 | m_bytes[2] << 16 | m_bytes[3] << 24;
-                *reinterpret_cast<u32_any*>(v8 + i) = v_bytes[0] | v_bytes[1] << 8 | v_bytes[2] << 16 | v_bytes[3] << 24;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (j < left) m8[i + j] = (unsigned char)m_bytes[j], v8[i + j] = (unsigned char)v_bytes[j];
-            }
-        }
-        if (lane == 0) t.m_scale[block] = (unsigned char)m_code, t.v_scale[block] = (unsigned char)v_code;
+        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw8_block<MANY, true>(t, base + k * kAdamwTurn, tensor, keep, s);
+    } else {
+        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw8_block<MANY, false>(t, base + k * kAdamwTurn, tensor, keep, s);
     }
 }
 

@@ -245,6 +245,7 @@ int block_norm_types(const snhip_block_norm_desc* d) {
 struct AdamwPlan {
     int device = 0, state_bits = 32;
     long long chunks = 0;
+    bool many = false;  // kAdamwMany elements or more
     void* table = nullptr;  // entries, then the owner of each chunk
     const int* owner = nullptr;
 };
@@ -268,14 +269,14 @@ bool overlapping(std::vector<Range>& ranges) {
 int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int state_bits, void** plan) {
     std::vector<AdamwEntry> entries((size_t)count);
     std::vector<Range> ranges;
-    long long chunks = 0;
+    long long elements = 0, chunks = 0;
     const size_t sb = state_bits == 32 ? 4 : 1;
     for (int k = 0; k < count; ++k) {
         const snhip_adamw_tensor& t = tensors[k];
         if (t.count < 0 || !is_storage_type(t.gradient_type) || !isfinite(t.weight_decay)) return SNHIP_STATUS_INVALID_VALUE;
         AdamwEntry& e = entries[(size_t)k];
         e = AdamwEntry{t.parameter, t.gradient, t.moment1, t.moment2, t.scale1, t.scale2, static_cast<__bf16*>(t.bf16_copy),
-                       t.count, chunks, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16};
+                       t.count, 0, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16};
         if (t.count == 0) continue;
         const size_t gb = type_bytes(t.gradient_type);
         if (t.parameter == nullptr || t.gradient == nullptr || t.moment1 == nullptr || t.moment2 == nullptr ||
@@ -295,7 +296,13 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
         add(t.bf16_copy, 2 * n, true);
         if (state_bits == 8) add(t.scale1, blocks, true), add(t.scale2, blocks, true);
         add(t.gradient, gb * n, false);
-        chunks += (t.count + kAdamwChunk - 1) / kAdamwChunk;
+        elements += t.count;
+    }
+    const bool many = elements >= kAdamwMany;
+    const long long chunk = kAdamwTurn * (many ? kAdamwTurns<true> : kAdamwTurns<false>);
+    for (AdamwEntry& e : entries) {
+        e.first_chunk = chunks;
+        chunks += (e.count + chunk - 1) / chunk;
     }
     if (chunks > 0x7fffffffLL) return SNHIP_STATUS_NOT_SUPPORTED;
     if (overlapping(ranges)) return SNHIP_STATUS_INVALID_VALUE;
@@ -303,11 +310,11 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
     if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
     std::vector<int> owner((size_t)chunks);
     for (int k = 0; k < count; ++k) {
-        const long long n = (entries[(size_t)k].count + kAdamwChunk - 1) / kAdamwChunk;
+        const long long n = (entries[(size_t)k].count + chunk - 1) / chunk;
         std::fill_n(owner.begin() + entries[(size_t)k].first_chunk, n, k);
     }
     std::unique_ptr<AdamwPlan> a(new AdamwPlan);
-    a->device = h->device, a->state_bits = state_bits, a->chunks = chunks;
+    a->device = h->device, a->state_bits = state_bits, a->chunks = chunks, a->many = many;
     if (chunks > 0) {
         const size_t entry_bytes = up256(entries.size() * sizeof(AdamwEntry));
         hipError_t e = hipMalloc(&a->table, entry_bytes + owner.size() * sizeof(int));
@@ -551,9 +558,8 @@ int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
     s.eps = (float)d->epsilon, s.grad_scale = d->gradient_scale;
     s.key0 = (unsigned int)d->seed, s.key1 = (unsigned int)(d->seed >> 32), s.step = (unsigned int)d->step;
     const AdamwEntry* entries = static_cast<const AdamwEntry*>(a->table);
-    const bool once = a->chunks * kAdamwChunk >= kAdamwOnce;
-    const auto kernel = a->state_bits == 32 ? (once ? adamw32_kernel<true> : adamw32_kernel<false>)
-                                            : (once ? adamw8_kernel<true> : adamw8_kernel<false>);
+    const auto kernel = a->state_bits == 8 ? (a->many ? adamw8_kernel<true> : adamw8_kernel<false>)
+                                           : (a->many ? adamw32_kernel<true> : adamw32_kernel<false>);
     hipLaunchKernelGGL(kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
     return hip_to_status(hipGetLastError());
 }
