@@ -2,9 +2,9 @@
 // Bound by HBM: 28 bytes an element with states in 32 bits, 16 with states in 8 (and an fp32 gradient), each read and
 // written once; the 8-bit form comes near the vector units' rate, too (some 90 instructions an element, a third of them the
 // random words).
-// A workgroup of 256 threads updates a chunk of a tensor, one or four turns of 1024 elements, four neighbours to a thread and
-// turn.  MANY: a plan of kAdamwMany elements or more, in chunks of four turns and around the caches.
-// FULL: all of a turn's elements exist; the tail of a tensor goes the other way.
+// A workgroup of 256 threads updates a chunk of a tensor, four neighbouring elements to a thread: longer chunks only put off
+// the next loads (66M elements, states in 32 / 8 bits: 315 / 178 us, chunks of four times the length 324 / 187 us).
+// FULL: all of a chunk's elements exist; the tail of a tensor goes the other way.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -15,14 +15,12 @@ namespace snhip {
 
 typedef unsigned int u32_any __attribute__((aligned(1)));  // four bytes at any address
 
-constexpr int kAdamwBlock = 256;  // elements that share a power of two (states in 8 bits)
-constexpr int kAdamwTurn = 1024;  // elements of a workgroup's turn
-// Elements from which on a chunk is four turns (2048 chunks, eight for each compute unit: below that one turn a chunk brings
-// more threads to work) and the data does not go through the caches: a step on 4 million (112 MB of fp32 states) finds some
-// of it in the 256 MB behind the L2s again, a step on more than they hold does not and runs at 5.45 instead of 5.15 TB/s.
-constexpr long long kAdamwMany = 1LL << 23;
-template <bool MANY>
-constexpr int kAdamwTurns = MANY ? 4 : 1;
+constexpr int kAdamwBlock = 256;              // elements that share a power of two (states in 8 bits)
+constexpr int kAdamwChunk = 4 * kAdamwBlock;  // elements of a workgroup
+// ONCE, from this many elements on: a plan's data does not go through the caches.  A step on less finds all of it in the 256 MB
+// behind the L2s again (3.2 million: 14.5 us both ways); one on more writes over what it would have found (7.1 million: 34.5 us
+// through the caches, 33.0 around them; 33 million: 170 us, 151).
+constexpr long long kAdamwOnce = 1LL << 22;
 
 struct AdamwEntry {
     float* p;
@@ -130,7 +128,7 @@ __device__ __forceinline__ f32x4 gradient_of(const AdamwEntry& t, const RawGradi
 
 // ---- states in 32 bits -----------------------------------------------------------------------------------------------
 template <bool ONCE, bool FULL>
-__device__ __forceinline__ void adamw32_turn(const AdamwEntry& t, long long from, float keep, const AdamwScalars& s) {
+__device__ __forceinline__ void adamw32_chunk(const AdamwEntry& t, long long from, float keep, const AdamwScalars& s) {
     const unsigned int i = threadIdx.x * 4;
     const int left = FULL || t.count - from - i >= 4 ? 4 : (int)(t.count - from - i);
     if (left <= 0) return;
@@ -150,18 +148,16 @@ __device__ __forceinline__ void adamw32_turn(const AdamwEntry& t, long long from
     if (t.copy != nullptr) give4<__bf16, ONCE, FULL>(t.copy + from, i, left, pp);
 }
 
-template <bool MANY>
+template <bool ONCE>
 __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
                                                       AdamwScalars s) {
     const AdamwEntry t = entries[owner[blockIdx.x]];
-    const long long base = (blockIdx.x - t.first_chunk) * (kAdamwTurns<MANY> * kAdamwTurn);
+    const long long from = (blockIdx.x - t.first_chunk) * kAdamwChunk;
     const float keep = 1.0f - s.rate * t.decay;
-    if (base + kAdamwTurns<MANY> * kAdamwTurn <= t.count) {
-#pragma unroll
-        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw32_turn<MANY, true>(t, base + k * kAdamwTurn, keep, s);
-    } else {
-        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw32_turn<MANY, false>(t, base + k * kAdamwTurn, keep, s);
-    }
+    if (from + kAdamwChunk <= t.count)
+        adamw32_chunk<ONCE, true>(t, from, keep, s);
+    else
+        adamw32_chunk<ONCE, false>(t, from, keep, s);
 }
 
 // ---- states in 8 bits ------------------------------------------------------------------------------------------------
@@ -259,7 +255,6 @@ __device__ __forceinline__ void store_states(const AdamwEntry& t, long long from
 // registers they were computed in.
 template <bool ONCE, bool FULL>
 __device__ __forceinline__ void adamw8_block(const AdamwEntry& t, long long from, int tensor, float keep, const AdamwScalars& s) {
-    if (!FULL && from >= t.count) return;
     const unsigned int i = (threadIdx.x & 63) * 4;
     const int left = FULL || t.count - from - i >= 4 ? 4 : (int)(t.count - from - i);  // <= 0: behind the tensor's end
     const long long block = from / kAdamwBlock;
@@ -284,19 +279,17 @@ __device__ __forceinline__ void adamw8_block(const AdamwEntry& t, long long from
     store_states<FULL>(t, from, i, left, mm, vv, tensor, s);
 }
 
-template <bool MANY>
+template <bool ONCE>
 __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
                                                      AdamwScalars s) {
     const int tensor = owner[blockIdx.x], w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AdamwEntry t = entries[tensor];
-    const long long base = (blockIdx.x - t.first_chunk) * (kAdamwTurns<MANY> * kAdamwTurn) + w * kAdamwBlock;
+    const long long from = (blockIdx.x - t.first_chunk) * kAdamwChunk + w * kAdamwBlock;
     const float keep = 1.0f - s.rate * t.decay;
-    if (base + (kAdamwTurns<MANY> - 1) * kAdamwTurn + kAdamwBlock <= t.count) {
-#pragma unroll
-        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw8_block<MANY, true>(t, base + k * kAdamwTurn, tensor, keep, s);
-    } else {
-        for (int k = 0; k < kAdamwTurns<MANY>; ++k) adamw8_block<MANY, false>(t, base + k * kAdamwTurn, tensor, keep, s);
-    }
+    if (from + kAdamwBlock <= t.count)
+        adamw8_block<ONCE, true>(t, from, tensor, keep, s);
+    else if (from < t.count)
+        adamw8_block<ONCE, false>(t, from, tensor, keep, s);
 }
 
 }  // namespace snhip

@@ -85,7 +85,8 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 // buckets ranked by i % 256 first.  The workgroup of a bucket finds its tokens in the order of their positions, a contiguous part to
 // each of its 16 wavefronts, and counts them by wavefront and id in LDS; after a scan over (id, wavefront) every wavefront
 // puts its tokens behind the earlier ones of their ids.  The order of all this is a function of the ids alone.
-// Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (6.6 us for 4000 tokens).
+// Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (8192 tokens
+// of 512: 29 us instead of 36 us).
 // With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup reads its own alone
 // (65536 tokens: 34 us the first way, 18 us the second).
 constexpr int kSortDirect = 8192; // tokens up to which every workgroup reads all ids
@@ -480,8 +481,8 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
 // The whole gradient in one launch, for few tokens (kSmallTokens) and few elements of dy (kSmallElements): the workgroup of a
 // bucket sorts its tokens in LDS as embedding_sort_kernel does and goes on to add up the rows of its ids.  A group of threads
 // takes an id at a time; ids with more than kLongRun tokens are left to all groups together, whose sums meet in LDS.  One
-// workgroup sums a frequent word's rows alone, which is what bounds the size (4000 x 100: 18 us in three launches, 10 us
-// in one; 1024 x 1024 into 32000 rows: 40 us in three, 51 us in one).
+// workgroup sums a frequent word's rows alone, which is what bounds the size (4000 x 100: 19 us in three launches, 11.5
+// us in one; 1024 x 1024 into 32000 rows: 37 us in three, 43 us in one).
 constexpr int kSmallTokens = 4096, kLongRun = 32;
 constexpr long long kSmallElements = 1LL << 19;
 
