@@ -150,9 +150,11 @@ __device__ __forceinline__ void adamw32_chunk(const AdamwEntry& t, long long fro
 
 template <bool ONCE>
 __global__ void __launch_bounds__(256) adamw32_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
-                                                      AdamwScalars s) {
-    const AdamwEntry t = entries[owner[blockIdx.x]];
-    const long long from = (blockIdx.x - t.first_chunk) * kAdamwChunk;
+                                                      long long chunks, AdamwScalars s) {
+    const long long chunk = block_number();
+    if (chunk >= chunks) return;
+    const AdamwEntry t = entries[owner[chunk]];
+    const long long from = (chunk - t.first_chunk) * kAdamwChunk;
     const float keep = 1.0f - s.rate * t.decay;
     if (from + kAdamwChunk <= t.count)
         adamw32_chunk<ONCE, true>(t, from, keep, s);
@@ -281,10 +283,12 @@ __device__ __forceinline__ void adamw8_block(const AdamwEntry& t, long long from
 
 template <bool ONCE>
 __global__ void __launch_bounds__(256) adamw8_kernel(const AdamwEntry* __restrict__ entries, const int* __restrict__ owner,
-                                                     AdamwScalars s) {
-    const int tensor = owner[blockIdx.x], w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+                                                     long long chunks, AdamwScalars s) {
+    const long long chunk = block_number();
+    if (chunk >= chunks) return;
+    const int tensor = owner[chunk], w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const AdamwEntry t = entries[tensor];
-    const long long from = (blockIdx.x - t.first_chunk) * kAdamwChunk + w * kAdamwBlock;
+    const long long from = (chunk - t.first_chunk) * kAdamwChunk + w * kAdamwBlock;
     const float keep = 1.0f - s.rate * t.decay;
     if (from + kAdamwBlock <= t.count)
         adamw8_block<ONCE, true>(t, from, tensor, keep, s);

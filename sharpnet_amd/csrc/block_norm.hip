@@ -29,7 +29,7 @@ namespace {
 template <int TPR, int N>
 void forward(const BlockNormParams& p, hipStream_t stream) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
-    const dim3 grid((unsigned)((p.rows + GROUPS - 1) / GROUPS));
+    const dim3 grid = many_blocks((p.rows + GROUPS - 1) / GROUPS);
     if (p.exact)
         hipLaunchKernelGGL((block_norm_forward_kernel<Stream, Block, TPR, N, true>), grid, dim3(NT), 0, stream, p);
     else

@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_forward_kern
     __shared__ float lds[2][2][TPR / 64 + 1];
     int turn = 0;
     const int lane = threadIdx.x % TPR, dim = p.dim;
-    const long long row = (long long)blockIdx.x * GROUPS + row_group<TPR>();
+    const long long row = block_number() * GROUPS + row_group<TPR>();
     if (row >= p.rows) return;  // (with a barrier ahead a workgroup has one row)
     f32x4 u[N];
     raw4<TS> x[N];

@@ -59,7 +59,7 @@ template <typename ID, typename TIN, typename TOUT, int ROWS>
 __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingParams p) {
     const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
     const int groups = 256 >> p.lanes_log2;
-    const long long t0 = ((long long)blockIdx.x * groups + group) * ROWS;
+    const long long t0 = (block_number() * groups + group) * ROWS;
     const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
     if (c >= p.dim) return;
     const bool ends = __ballot(p.dim - c < 4) != 0;

@@ -95,7 +95,7 @@ void embedding_forward_launch(const EmbeddingParams& p, hipStream_t stream) {
     const int groups = 256 >> p.lanes_log2;
     const long long blocks = (p.tokens + (long long)groups * ROWS - 1) / ((long long)groups * ROWS);
     hipLaunchKernelGGL((embedding_forward_kernel<ID, TIN, TOUT, ROWS>),
-                       dim3((unsigned)blocks, (unsigned)ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2)), dim3(256), 0, stream, p);
+                       many_blocks(blocks, (unsigned)ceil_div(ceil_div(p.dim, 4), 1 << p.lanes_log2)), dim3(256), 0, stream, p);
 }
 template <typename ID>
 void embedding_forward_types(const EmbeddingParams& p, int table_type, int output_type, hipStream_t stream) {
@@ -559,7 +559,7 @@ int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
     const AdamwEntry* entries = static_cast<const AdamwEntry*>(a->table);
     const auto kernel = a->state_bits == 8 ? (a->once ? adamw8_kernel<true> : adamw8_kernel<false>)
                                            : (a->once ? adamw32_kernel<true> : adamw32_kernel<false>);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a->chunks), dim3(256), 0, h->stream, entries, a->owner, s);
+    hipLaunchKernelGGL(kernel, many_blocks(a->chunks), dim3(256), 0, h->stream, entries, a->owner, a->chunks, s);
     return hip_to_status(hipGetLastError());
 }
 

@@ -120,4 +120,12 @@ __device__ __forceinline__ float wave64_sum(float v) {
     return (a + b) + (c + d);
 }
 
+// Launches that can have more workgroups than the 2^32 - 1 threads of a grid's x hold are spread over x and z, with up to 8 z
+// workgroups too many: a kernel looks at its number.
+inline dim3 many_blocks(long long blocks, unsigned int y = 1) {
+    const long long z = (blocks + 65535) >> 16, x = z > 1 ? ((blocks + z - 1) / z + 7) / 8 * 8 : blocks;
+    return dim3((unsigned int)x, y, (unsigned int)z);
+}
+__device__ __forceinline__ long long block_number() { return (long long)blockIdx.z * gridDim.x + blockIdx.x; }
+
 }  // namespace snhip
