@@ -40,8 +40,8 @@ def fused_attention_forward(Q, K, V, O, weights, *, batch, heads, tq, tkv, dk, d
     ldv, sv, sv2 = strides(tkv, dv)
     ldo, so, so2 = strides(tq, dv)
     d = hiplib.AttentionDesc(batch=batch * heads, batch_inner=heads, Tq=tq, Tk=tkv, dk=dk, dv=dv, scale=scale,
-                             causal=int(bool(is_causal)), Q=Q.Pointer, K=K.Pointer, V=V.Pointer, O=O.Pointer,
-                             weights=weights.Pointer if weights is not None else None, ldq=ldq, ldk=ldk, ldv=ldv, ldo=ldo,
+                             causal=int(bool(is_causal)), Q=Q.FloatPointer, K=K.FloatPointer, V=V.FloatPointer, O=O.FloatPointer,
+                             weights=weights.FloatPointer if weights is not None else None, ldq=ldq, ldk=ldk, ldv=ldv, ldo=ldo,
                              strideQ=sq, strideK=sk, strideV=sv, strideO=so, strideQ_outer=sq2, strideK_outer=sk2,
                              strideV_outer=sv2, strideO_outer=so2)
     st = Q._lib.snhip_attention_forward(Q.Wrapper.handle, ctypes.byref(d))
@@ -66,8 +66,8 @@ def attention_backward(dQ, dK, dV, Q, K, V, dO, weights, scores_gradients, *, ba
     ldv, sv, sv2 = strides(tkv, dv)
     ldo, so, so2 = strides(tq, dv)
     d = hiplib.AttentionBwdDesc(batch=batch * heads, batch_inner=heads, Tq=tq, Tk=tkv, dk=dk, dv=dv, scale=scale,
-                                Q=Q.Pointer, K=K.Pointer, V=V.Pointer, dO=dO.Pointer, weights=weights.Pointer,
-                                scores_gradients=scores_gradients.Pointer, dQ=dQ.Pointer, dK=dK.Pointer, dV=dV.Pointer,
+                                Q=Q.FloatPointer, K=K.FloatPointer, V=V.FloatPointer, dO=dO.FloatPointer, weights=weights.FloatPointer,
+                                scores_gradients=scores_gradients.FloatPointer, dQ=dQ.FloatPointer, dK=dK.FloatPointer, dV=dV.FloatPointer,
                                 ldq=ldq, ldk=ldk, ldv=ldv, ldo=ldo, strideQ=sq, strideK=sk, strideV=sv, strideO=so,
                                 strideQ_outer=sq2, strideK_outer=sk2, strideV_outer=sv2, strideO_outer=so2,
                                 causal=int(bool(is_causal)))

@@ -7,8 +7,9 @@ row of y is zeros and it adds nothing to the gradient.
 """
 import ctypes
 import math
+import threading
 
-from .gpu_tensor import GPUTensor
+from .gpu_tensor import LayerWorkspace, pointer_on
 from .hiplib import EmbeddingDesc, TYPES, check_status
 
 _ID_TYPES = {k: TYPES[k] for k in ("float32", "int32", "int64")}
@@ -24,11 +25,9 @@ class WordEmbedding:
         self.VocabularySize, self.EmbeddingDim = int(vocabularySize), int(embeddingDim)
         self.Scale, self.PaddingIndex = float(scale), int(paddingIndex)
         self.Wrapper = gpu_wrapper
-        self._workspace = None
-        self._workspaceBytes = 0
-        # a call fills in every field that is not of the layer itself
-        self._d = EmbeddingDesc(vocabulary=self.VocabularySize, dim=self.EmbeddingDim, padding_index=self.PaddingIndex, scale=self.Scale)
-        self._need = ctypes.c_size_t()
+        self._tableShape = [self.VocabularySize, self.EmbeddingDim]
+        self._workspace = LayerWorkspace()
+        self._mine = threading.local()  # a descriptor for each thread; a call fills in all but the sizes
 
     def _desc(self, x, rows, table_type):
         """rows: y or dy, (..., EmbeddingDim) with one row per id of x."""
@@ -39,23 +38,24 @@ class WordEmbedding:
         tokens = math.prod(x.Shape)
         if rows.Shape[-1] != self.EmbeddingDim or math.prod(rows.Shape) != tokens * self.EmbeddingDim:
             raise ValueError("%s ids and rows of %s do not fit an embedding dimension of %d" % (x.Shape, rows.Shape, self.EmbeddingDim))
-        d = self._d
+        try:
+            d = self._mine.desc
+        except AttributeError:
+            d = self._mine.desc = EmbeddingDesc(vocabulary=self.VocabularySize, dim=self.EmbeddingDim)
         d.id_type, d.table_type, d.output_type, d.tokens = _ID_TYPES[x.Type], _ROW_TYPES[table_type], _ROW_TYPES[rows.Type], tokens
+        d.padding_index, d.scale = self.PaddingIndex, self.Scale
         return d
 
     def _check_table(self, table):
-        if table.Shape != [self.VocabularySize, self.EmbeddingDim]:
-            raise ValueError("the table must be %s, not %s" % ([self.VocabularySize, self.EmbeddingDim], table.Shape))
+        if table.Shape != self._tableShape:
+            raise ValueError("the table must be %s, not %s" % (self._tableShape, table.Shape))
 
     def ForwardPropagation(self, y, x, wordEmbedding):
         """y (ids' shape + EmbeddingDim) = Scale * wordEmbedding[x]."""
         self._check_table(wordEmbedding)
-        d = self._desc(x, y, wordEmbedding.Type)
-        y.AssertIsNotDisposed()
-        x.AssertIsNotDisposed()
-        wordEmbedding.AssertIsNotDisposed()
-        check_status(y._lib.snhip_embedding_forward(y.Wrapper.handle, ctypes.byref(d), x.Pointer, wordEmbedding.Pointer,
-                                                    y.Pointer), "snhip_embedding_forward")
+        d, w = self._desc(x, y, wordEmbedding.Type), y.Wrapper
+        check_status(y._lib.snhip_embedding_forward(w.handle, ctypes.byref(d), pointer_on(w, x), pointer_on(w, wordEmbedding),
+                                                    pointer_on(w, y)), "snhip_embedding_forward")
 
     def BackwardWorkspaceSize(self, x, dy):
         nbytes = ctypes.c_size_t()
@@ -66,33 +66,21 @@ class WordEmbedding:
 
     def BackwardPropagation(self, dWordEmbedding, x, dy, accumulate=False, workspace=None):
         """dWordEmbedding (float32) = the table's gradient, or += it with ``accumulate``.  Without a ``workspace`` the layer
-        keeps one of its own, which grows when a longer batch comes (an allocation: size it with a first call before a
-        stream capture) and belongs to one stream at a time."""
+        keeps one of its own for each wrapper, which grows when a longer batch comes (an allocation: size it with a first call
+        before a stream capture).  It is one call's at a time: two captured graphs whose replays may overlap get one each."""
         self._check_table(dWordEmbedding)
         if dWordEmbedding.Type != "float32":
             raise ValueError("the table's gradient must be float32, not %s" % dWordEmbedding.Type)
-        d = self._desc(x, dy, "float32")
-        dWordEmbedding.AssertIsNotDisposed()
-        x.AssertIsNotDisposed()
-        dy.AssertIsNotDisposed()
-        need = self._need
+        d, need, w = self._desc(x, dy, "float32"), ctypes.c_size_t(), dy.Wrapper
+        pointers = pointer_on(w, x), pointer_on(w, dy), pointer_on(w, dWordEmbedding)
         check_status(dy._lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_embedding_backward_workspace_size")
-        if workspace is None and need.value:
-            if self._workspaceBytes < need.value:
-                if self._workspace is not None:
-                    self._workspace.Wrapper.synchronize()
-                    self._workspace.Dispose()
-                self._workspace = GPUTensor([need.value], None, dy.Wrapper, element_type="uint8")
-                self._workspaceBytes = need.value
-            workspace = self._workspace
-        check_status(dy._lib.snhip_embedding_backward(dy.Wrapper.handle, ctypes.byref(d), x.Pointer, dy.Pointer,
-                                                      dWordEmbedding.Pointer, int(bool(accumulate)),
-                                                      workspace.Pointer if workspace is not None else None,
+        if workspace is None:
+            workspace = self._workspace.Get(w, need.value)
+        check_status(dy._lib.snhip_embedding_backward(w.handle, ctypes.byref(d), *pointers, int(bool(accumulate)),
+                                                      pointer_on(w, workspace),
                                                       workspace.Count * workspace.ElementBytes if workspace is not None else 0),
                      "snhip_embedding_backward")
 
     def Dispose(self):
-        if self._workspace is not None:
-            self._workspace.Dispose()
-        self._workspace, self._workspaceBytes = None, 0
+        self._workspace.Dispose()

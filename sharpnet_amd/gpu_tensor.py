@@ -226,6 +226,13 @@ class GPUTensor:
         s = self.Shape
         return s[1] * self.MultDim1 if len(s) >= 2 else 1
 
+    @property
+    def FloatPointer(self):
+        """The address for entry points that compute with float32, which would read other types at the wrong places."""
+        if self.Type != "float32":
+            raise ValueError("a %s tensor where float32 is expected" % self.Type)
+        return self.Pointer
+
     def AssertIsNotDisposed(self):
         if self._disposed or (self._owner is not None and self._owner._disposed):
             raise RuntimeError("Tensor is disposed")  # GpuTensor.cs:1592-1598
@@ -342,7 +349,7 @@ class GPUTensor:
         # column-major library: compute B*A instead of A*B (GpuTensor.cs:1217-1218)
         al, be = ctypes.c_float(alpha), ctypes.c_float(beta)
         res = self._lib.snhip_sgemm(self.Wrapper.handle, transLeft, transRight, N, M, K, ctypes.byref(al),
-                                    b.Pointer, ldb, a.Pointer, lda, ctypes.byref(be), self.Pointer, ldc)
+                                    b.FloatPointer, ldb, a.FloatPointer, lda, ctypes.byref(be), self.FloatPointer, ldc)
         check_status(res, "snhip_sgemm")
 
     def BatchMatrixMultiplication(self, a_3D, transposeA, b_3D, transposeB, alpha, beta):
@@ -364,23 +371,24 @@ class GPUTensor:
         ldb, lda, ldc = bW, aW, N
         al, be = ctypes.c_float(alpha), ctypes.c_float(beta)
         res = self._lib.snhip_sgemm_strided_batched(self.Wrapper.handle, transLeft, transRight, N, M, K,
-                                                    ctypes.byref(al), b_3D.Pointer, ldb, bStride, a_3D.Pointer, lda,
-                                                    aStride, ctypes.byref(be), self.Pointer, ldc, cStride, batchCount)
+                                                    ctypes.byref(al), b_3D.FloatPointer, ldb, bStride, a_3D.FloatPointer, lda,
+                                                    aStride, ctypes.byref(be), self.FloatPointer, ldc, cStride, batchCount)
         check_status(res, "snhip_sgemm_strided_batched")
 
     # -- row-major convenience entry points (same numbers, fewer hops) ---------
     def DotRowMajor(self, a, transposeA, b, transposeB, alpha, beta, bias=None):
         """snhip_dot / snhip_dot_bias with BlasServices.DotMkl's parameter list."""
-        res = self._lib.snhip_dot_bias(self.Wrapper.handle, a.Pointer, a.Shape[0], a.MultDim0, int(transposeA),
-                                       b.Pointer, b.Shape[0], b.MultDim0, int(transposeB), self.Pointer, alpha, beta,
-                                       bias.Pointer if bias is not None else None)
+        res = self._lib.snhip_dot_bias(self.Wrapper.handle, a.FloatPointer, a.Shape[0], a.MultDim0, int(transposeA),
+                                       b.FloatPointer, b.Shape[0], b.MultDim0, int(transposeB), self.FloatPointer, alpha, beta,
+                                       bias.FloatPointer if bias is not None else None)
         check_status(res, "snhip_dot_bias")
 
     def GemmEx(self, **fields):
         """snhip_gemm_ex with this tensor as C: keyword arguments are snhip_gemm_desc fields; tensors may be passed
         for A, B, bias, D and colsum (their device pointers are used)."""
-        fields = {k: (v.Pointer if isinstance(v, GPUTensor) else v) for k, v in fields.items()}
-        desc = hiplib.GemmDesc(C=self.Pointer, **fields)
+        stored = ("A", "B") if fields.get("math") == GPUWrapper.MATH_BF16_STORED else ()
+        fields = {k: (v.Pointer if k in stored else v.FloatPointer) if isinstance(v, GPUTensor) else v for k, v in fields.items()}
+        desc = hiplib.GemmDesc(C=self.FloatPointer, **fields)
         check_status(self._lib.snhip_gemm_ex(self.Wrapper.handle, ctypes.byref(desc)), "snhip_gemm_ex")
 
     # -- lifetime ----------------------------------------------------------------
@@ -400,34 +408,69 @@ class GPUTensor:
 
 
 # -- element-wise / row helpers next to the GEMMs (same names as the reference's Tensor methods) -----------------
+class LayerWorkspace:
+    """Scratch memory of a layer, one buffer for each wrapper (device and stream) that it is used on.  A longer call gets a
+    longer buffer; the one before stays until Dispose, since a captured graph may still write to it."""
+
+    def __init__(self):
+        self._held = {}
+
+    def Get(self, wrapper, nbytes):
+        """A uint8 tensor of at least nbytes, or None for none."""
+        if nbytes == 0:
+            return None
+        held = self._held.setdefault(wrapper, [])
+        if not held or held[-1].Shape[0] < nbytes:
+            size = max(nbytes, held[-1].Shape[0] * 3 // 2) if held else nbytes  # (all together: at most three times the last)
+            held.append(GPUTensor([size], None, wrapper, element_type="uint8"))
+        return held[-1]
+
+    def Dispose(self):
+        held, self._held = self._held, {}
+        for buffers in held.values():
+            for t in buffers:
+                t.Dispose()
+
+
+def pointer_on(wrapper, t):
+    """The address of a live tensor on the wrapper's device, None for None."""
+    if t is None:
+        return None
+    if t._disposed or t._owner is not None:
+        t.AssertIsNotDisposed()
+    if t.Wrapper is not wrapper and t.Wrapper.device_id != wrapper.device_id:
+        raise ValueError("a tensor on device %d in a call on device %d" % (t.Wrapper.device_id, wrapper.device_id))
+    return t.Pointer
+
+
 def _add_tensor_methods():
     def Compute_BiasGradient_from_dy(self, biasGradient_1D):
         """biasGradient[c] = sum over rows of this[r][c]  (CpuTensor.cs:1736-1740)."""
         assert len(biasGradient_1D.Shape) == 1 and biasGradient_1D.Count == self.MultDim0
-        check_status(self._lib.snhip_bias_gradient(self.Wrapper.handle, self.Pointer, self.Shape[0], self.MultDim0,
-                                                   biasGradient_1D.Pointer), "snhip_bias_gradient")
+        check_status(self._lib.snhip_bias_gradient(self.Wrapper.handle, self.FloatPointer, self.Shape[0], self.MultDim0,
+                                                   biasGradient_1D.FloatPointer), "snhip_bias_gradient")
 
     def BroadcastAddVectorToOutput(self, y):
         """y[n, :] += this  (this = 1-D bias; CpuTensor.cs:1468-1487)."""
         assert y.Dimension >= 2 and y.MultDim0 == self.Count
-        check_status(self._lib.snhip_broadcast_add_vector(self.Wrapper.handle, self.Pointer, y.Pointer, y.Shape[0],
+        check_status(self._lib.snhip_broadcast_add_vector(self.Wrapper.handle, self.FloatPointer, y.FloatPointer, y.Shape[0],
                                                           y.MultDim0), "snhip_broadcast_add_vector")
 
     def Update_Adding_Alpha_X(self, alpha, x):
         """this += alpha * x  (Linear.cs:178)."""
         assert x.Count == self.Count
-        check_status(self._lib.snhip_axpy(self.Wrapper.handle, self.Count, alpha, x.Pointer, self.Pointer), "snhip_axpy")
+        check_status(self._lib.snhip_axpy(self.Wrapper.handle, self.Count, alpha, x.FloatPointer, self.FloatPointer), "snhip_axpy")
 
     def SoftmaxLastDimension(self, y):
         """y = softmax(this) over the last dimension (ActivationForward(SOFTMAX_LAST_DIMENSION))."""
         cols = self.Shape[-1]
-        check_status(self._lib.snhip_softmax_last_dim(self.Wrapper.handle, self.Pointer, y.Pointer,
+        check_status(self._lib.snhip_softmax_last_dim(self.Wrapper.handle, self.FloatPointer, y.FloatPointer,
                                                       self.Count // cols if cols else 0, cols), "snhip_softmax_last_dim")
 
     def SoftmaxLastDimensionBackward(self, dy, dx):
         """dx = softmax gradient given this = y (ActivationBackward(SOFTMAX_LAST_DIMENSION), cuDNN semantics)."""
         cols = self.Shape[-1]
-        check_status(self._lib.snhip_softmax_last_dim_backward(self.Wrapper.handle, self.Pointer, dy.Pointer, dx.Pointer,
+        check_status(self._lib.snhip_softmax_last_dim_backward(self.Wrapper.handle, self.FloatPointer, dy.FloatPointer, dx.FloatPointer,
                                                                self.Count // cols if cols else 0, cols),
                      "snhip_softmax_last_dim_backward")
 
@@ -435,7 +478,7 @@ def _add_tensor_methods():
         """CpuTensor.cs:3037-3052; 2-D or 3-D tensors."""
         assert len(self.Shape) in (2, 3)
         m, r, c = (self.Shape if len(self.Shape) == 3 else [1] + self.Shape)
-        check_status(self._lib.snhip_set_above_main_diagonal(self.Wrapper.handle, self.Pointer, m, r, c, value),
+        check_status(self._lib.snhip_set_above_main_diagonal(self.Wrapper.handle, self.FloatPointer, m, r, c, value),
                      "snhip_set_above_main_diagonal")
 
     def Transpose(self, transposed):
@@ -446,7 +489,7 @@ def _add_tensor_methods():
         M, N = self.Shape
         alpha, beta = ctypes.c_float(1.0), ctypes.c_float(0.0)
         check_status(self._lib.snhip_sgeam(self.Wrapper.handle, CUBLAS_OP_T, CUBLAS_OP_N, M, N, ctypes.byref(alpha),
-                                           self.Pointer, N, ctypes.byref(beta), None, M, transposed.Pointer, M), "snhip_sgeam")
+                                           self.FloatPointer, N, ctypes.byref(beta), None, M, transposed.FloatPointer, M), "snhip_sgeam")
 
     def MultiplyTensor(self, a, diagonalMatrix):
         """this = a * diagonalMatrix, element-wise when both have the same size, else every run of
@@ -455,8 +498,8 @@ def _add_tensor_methods():
         assert a.Count == self.Count and self.Count % diagonalMatrix.Count == 0
         n = diagonalMatrix.Count
         m = self.Count // n
-        check_status(self._lib.snhip_sdgmm(self.Wrapper.handle, 1, m, n, a.Pointer, m, diagonalMatrix.Pointer, 1,
-                                           self.Pointer, m), "snhip_sdgmm")
+        check_status(self._lib.snhip_sdgmm(self.Wrapper.handle, 1, m, n, a.FloatPointer, m, diagonalMatrix.FloatPointer, 1,
+                                           self.FloatPointer, m), "snhip_sdgmm")
 
     def TransposeSecondAndThirdDimension(self, target):
         """target[a][c][b][d] = this[a][b][c][d]; target is reshaped to the swapped shape (CpuTensor.cs:301-322)."""
@@ -464,7 +507,7 @@ def _add_tensor_methods():
         A, B, C = self.Shape[:3]
         D = self.Count // max(A * B * C, 1)
         target.Shape = [A, C, B] + list(self.Shape[3:])
-        check_status(self._lib.snhip_transpose_second_and_third_dimension(self.Wrapper.handle, self.Pointer, target.Pointer,
+        check_status(self._lib.snhip_transpose_second_and_third_dimension(self.Wrapper.handle, self.FloatPointer, target.FloatPointer,
                                                                           A, B, C, D),
                      "snhip_transpose_second_and_third_dimension")
 
@@ -472,15 +515,15 @@ def _add_tensor_methods():
         """y = act(this) for the RELU / LEAKY_RELU / SIGMOID / TANH modes (Tensor.ActivationForward);
         activationParameter is the leaky slope."""
         check_status(self._lib.snhip_activation_forward(self.Wrapper.handle, hiplib.activation_code(activationType),
-                                                        float(activationParameter or 0.0), self.Pointer, y.Pointer,
+                                                        float(activationParameter or 0.0), self.FloatPointer, y.FloatPointer,
                                                         self.Count), "snhip_activation_forward")
 
     def ActivationBackward(self, activationType, activationParameter, dy, dx):
         """dx = dy * act'(x) with this = y = act(x) (Tensor.ActivationBackward, CPU definitions
         CpuTensorActivationFunctions.cs:190-244)."""
         check_status(self._lib.snhip_activation_backward(self.Wrapper.handle, hiplib.activation_code(activationType),
-                                                         float(activationParameter or 0.0), self.Pointer, dy.Pointer,
-                                                         dx.Pointer, self.Count), "snhip_activation_backward")
+                                                         float(activationParameter or 0.0), self.FloatPointer, dy.FloatPointer,
+                                                         dx.FloatPointer, self.Count), "snhip_activation_backward")
 
     for f in (Compute_BiasGradient_from_dy, BroadcastAddVectorToOutput, Update_Adding_Alpha_X, SoftmaxLastDimension,
               SoftmaxLastDimensionBackward, SetAllElementsAboveMainDiagonal, Transpose, MultiplyTensor,

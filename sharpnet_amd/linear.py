@@ -24,8 +24,8 @@ def DenseForwardPropagation(y, x, weights, biasIfAny_1D, flattenInputTensorOnLas
         rows, in_features = xAs2DMatrix.Shape
         out_features = weights.Shape[0]
         assert weights.Shape[1] == in_features and yAs2DMatrix.Shape == [rows, out_features]
-        check_status(y._lib.snhip_dense_forward(y.Wrapper.handle, yAs2DMatrix.Pointer, xAs2DMatrix.Pointer,
-                                                weights.Pointer, biasIfAny_1D.Pointer if biasIfAny_1D is not None else None,
+        check_status(y._lib.snhip_dense_forward(y.Wrapper.handle, yAs2DMatrix.FloatPointer, xAs2DMatrix.FloatPointer,
+                                                weights.FloatPointer, biasIfAny_1D.FloatPointer if biasIfAny_1D is not None else None,
                                                 rows, in_features, out_features, act, float(activation_parameter)),
                      "snhip_dense_forward")
         return
@@ -58,10 +58,10 @@ def DenseBackwardPropagation(dx, weightGradients, biasGradients_1D, x, dy, weigh
         # weight decay on the bias gradient as well in the PyTorch mode (Linear.cs:178-181)
         bias_alpha = alpha if (alpha and compatibility_mode == "PyTorch" and biasGradients_1D is not None) else 0.0
         check_status(dy._lib.snhip_dense_backward_ex(
-            dy.Wrapper.handle, None if prevLayerIsInputLayer else dx.As2DTensor(flattenInputTensorOnLastDimension).Pointer,
-            weightGradients.Pointer, biasGradients_1D.Pointer if biasGradients_1D is not None else None,
-            xAs2DMatrix.Pointer, dyAs2DMatrix.Pointer, weights.Pointer, rows, in_features, out_features, multiplier, alpha,
-            bias_1D.Pointer if bias_alpha else None, bias_alpha), "snhip_dense_backward_ex")
+            dy.Wrapper.handle, None if prevLayerIsInputLayer else dx.As2DTensor(flattenInputTensorOnLastDimension).FloatPointer,
+            weightGradients.FloatPointer, biasGradients_1D.FloatPointer if biasGradients_1D is not None else None,
+            xAs2DMatrix.FloatPointer, dyAs2DMatrix.FloatPointer, weights.FloatPointer, rows, in_features, out_features, multiplier, alpha,
+            bias_1D.FloatPointer if bias_alpha else None, bias_alpha), "snhip_dense_backward_ex")
         return
     weightGradients.Dot(dyAs2DMatrix, True, xAs2DMatrix, False, multiplier, 0.0)
     if biasGradients_1D is not None:

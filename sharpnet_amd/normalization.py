@@ -7,8 +7,9 @@ what the next block reads.
 """
 import ctypes
 import math
+import threading
 
-from .gpu_tensor import GPUTensor
+from .gpu_tensor import LayerWorkspace, pointer_on
 from .hiplib import (ACT_NONE, ACT_SIGMOID, ACT_TANH, BlockNormDesc, NORM_LAYER, NORM_NONE, NORM_RMS, SharpNetHipError, CublasStatus,
                      TYPES, check_status)
 
@@ -16,14 +17,6 @@ _NORMS = {None: NORM_NONE, "none": NORM_NONE, "rms": NORM_RMS, "layer": NORM_LAY
 _GATES = {None: ACT_NONE, "none": ACT_NONE, "sigmoid": ACT_SIGMOID, "tanh": ACT_TANH,
           "CUDNN_ACTIVATION_IDENTITY": ACT_NONE, "CUDNN_ACTIVATION_SIGMOID": ACT_SIGMOID, "CUDNN_ACTIVATION_TANH": ACT_TANH}
 _ROW_TYPES = {k: TYPES[k] for k in ("float32", "bfloat16")}
-
-
-def _live(t):
-    """The address of a tensor that is there, None for None."""
-    if t is None:
-        return None
-    t.AssertIsNotDisposed()
-    return t.Pointer
 
 
 class BlockNorm:
@@ -41,12 +34,8 @@ class BlockNorm:
         self.PreNorm, self.PostNorm, self.GateActivation = _NORMS[preNorm], _NORMS[postNorm], _GATES[gateActivation]
         self.ResidualScale, self.Epsilon = float(residualScale), float(epsilon)
         self.Wrapper = gpu_wrapper
-        self._workspace = None
-        self._workspaceBytes = 0
-        # one descriptor for each direction; a call fills in every field that is not of the layer itself
-        layer = dict(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=self.EmbeddingDim,
-                     epsilon=self.Epsilon, residual_scale=self.ResidualScale)
-        self._forward, self._backward, self._need = BlockNormDesc(**layer), BlockNormDesc(**layer), ctypes.c_size_t()
+        self._workspace = LayerWorkspace()
+        self._mine = threading.local()  # a descriptor for each thread and direction; a call fills in what is not the layer's kind
 
     def _rows(self, t, name, shape, type_):
         """t is None or has rows like those of shape, in the given type."""
@@ -61,8 +50,8 @@ class BlockNorm:
         if t is not None and (t.Type != "float32" or (t.Shape != self._vectorShape and math.prod(t.Shape) != self.EmbeddingDim)):
             raise ValueError("%s is %s %s, expected %d float32" % (name, t.Type, t.Shape, self.EmbeddingDim))
 
-    def _fill(self, d, stream, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
-        """What both directions have: sizes and types, gate, weights, statistics."""
+    def _desc(self, direction, stream, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
+        """What both directions have: the layer itself, sizes and types, gate, weights, statistics."""
         if self.EmbeddingDim <= 0 or stream.Shape[-1] != self.EmbeddingDim:
             raise ValueError("rows of %s do not fit an embedding dimension of %d" % (stream.Shape, self.EmbeddingDim))
         if stream.Type not in _ROW_TYPES or block.Type not in _ROW_TYPES:
@@ -82,24 +71,31 @@ class BlockNorm:
                 self._vector(gate, "gate")
             else:
                 self._rows(gate, "gate", [-(-rows // gateRows), self.EmbeddingDim], block.Type)
+        w, mine = stream.Wrapper, self._mine.__dict__
+        d = mine.get(direction)
+        if d is None:
+            d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation,
+                                                dim=self.EmbeddingDim)
+        d.epsilon, d.residual_scale = self.Epsilon, self.ResidualScale
         d.rows, d.gate_rows = rows, gateRows
         d.stream_type, d.block_type = _ROW_TYPES[stream.Type], _ROW_TYPES[block.Type]
-        d.gate, d.pre_weight, d.pre_bias = _live(gate), _live(preWeight), _live(preBias)
-        d.post_weight, d.post_bias = _live(postWeight), _live(postBias)
-        d.pre_statistics, d.post_statistics = _live(preStatistics), _live(postStatistics)
+        d.gate, d.pre_weight, d.pre_bias = pointer_on(w, gate), pointer_on(w, preWeight), pointer_on(w, preBias)
+        d.post_weight, d.post_bias = pointer_on(w, postWeight), pointer_on(w, postBias)
+        d.pre_statistics, d.post_statistics = pointer_on(w, preStatistics), pointer_on(w, postStatistics)
+        return d
 
     def ForwardPropagation(self, x, h, y=None, u=None, gate=None, gateRows=0, preWeight=None, preBias=None, postWeight=None,
                            postBias=None, preStatistics=None, postStatistics=None):
         """h and u from x and y; h is None for a join without a norm ahead of the next block, y and u for a norm without a
         block.  gateRows: rows that share a row of the gate (0: the gate is one vector)."""
-        d, shape = self._forward, x.Shape
+        shape, w = x.Shape, x.Wrapper
         block = h if h is not None else y if y is not None else x
-        self._fill(d, x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
+        d = self._desc("forward", x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
         self._rows(y, "y", shape, block.Type)
         self._rows(h, "h", shape, block.Type)
         self._rows(u, "u", shape, x.Type)
-        d.x, d.y, d.u, d.h = _live(x), _live(y), _live(u), _live(h)
-        check_status(x._lib.snhip_block_norm_forward(x.Wrapper.handle, ctypes.byref(d)), "snhip_block_norm_forward")
+        d.x, d.y, d.u, d.h = pointer_on(w, x), pointer_on(w, y), pointer_on(w, u), pointer_on(w, h)
+        check_status(x._lib.snhip_block_norm_forward(w.handle, ctypes.byref(d)), "snhip_block_norm_forward")
 
     def BackwardPropagation(self, dx, u, dh, du=None, y=None, dy=None, gate=None, dGate=None, gateRows=0, preWeight=None,
                             preStatistics=None, dPreWeight=None, dPreBias=None, postWeight=None, postBias=None, postStatistics=None,
@@ -107,9 +103,9 @@ class BlockNorm:
         """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics; gradients that are
         None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
-        d, shape = self._backward, dx.Shape
+        shape, w = dx.Shape, dx.Wrapper
         block = next((t for t in (dh, y, dy) if t is not None), dx)
-        self._fill(d, dx, block, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
+        d = self._desc("backward", dx, block, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
         for t, name in ((y, "y"), (dh, "dh"), (dy, "dy")):
             self._rows(t, name, shape, block.Type)
         for t, name in ((u, "u"), (du, "du")):
@@ -118,26 +114,18 @@ class BlockNorm:
             self._vector(t, name)
         if dGate is not None and (gate is None or dGate.Shape != gate.Shape or dGate.Type != gate.Type):
             raise ValueError("dGate must have the gate's shape and type")
-        d.y, d.u, d.dx, d.dh, d.du, d.dy = _live(y), _live(u), _live(dx), _live(dh), _live(du), _live(dy)
-        d.d_gate, d.d_pre_weight, d.d_pre_bias = _live(dGate), _live(dPreWeight), _live(dPreBias)
-        d.d_post_weight, d.d_post_bias = _live(dPostWeight), _live(dPostBias)
+        d.y, d.u, d.dx, d.dh, d.du, d.dy = (pointer_on(w, t) for t in (y, u, dx, dh, du, dy))
+        d.d_gate, d.d_pre_weight, d.d_pre_bias = pointer_on(w, dGate), pointer_on(w, dPreWeight), pointer_on(w, dPreBias)
+        d.d_post_weight, d.d_post_bias = pointer_on(w, dPostWeight), pointer_on(w, dPostBias)
         d.accumulate = 1 if accumulate else 0
-        need, lib = self._need, dx._lib
+        need, lib = ctypes.c_size_t(), dx._lib
         check_status(lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_block_norm_backward_workspace_size")
-        if workspace is None and need.value:
-            if self._workspaceBytes < need.value:
-                if self._workspace is not None:
-                    self._workspace.Wrapper.synchronize()
-                    self._workspace.Dispose()
-                self._workspace = GPUTensor([need.value], None, dx.Wrapper, element_type="uint8")
-                self._workspaceBytes = need.value
-            workspace = self._workspace
+        if workspace is None:
+            workspace = self._workspace.Get(w, need.value)
         nbytes = workspace.Count * workspace.ElementBytes if workspace is not None else 0
-        check_status(lib.snhip_block_norm_backward(dx.Wrapper.handle, ctypes.byref(d), _live(workspace), nbytes),
+        check_status(lib.snhip_block_norm_backward(w.handle, ctypes.byref(d), pointer_on(w, workspace), nbytes),
                      "snhip_block_norm_backward")
 
     def Dispose(self):
-        if self._workspace is not None:
-            self._workspace.Dispose()
-        self._workspace, self._workspaceBytes = None, 0
+        self._workspace.Dispose()

@@ -2,7 +2,7 @@
 Prod/GPU/Kernels/SinglePrecision.cu:19, one launch per tensor, with decoupled weight decay) on GPUTensor."""
 import ctypes
 
-from .gpu_tensor import GPUTensor
+from .gpu_tensor import GPUTensor, pointer_on
 from .hiplib import AdamwStepDesc, AdamwTensor, TYPES, check_status
 
 
@@ -26,7 +26,7 @@ class AdamW:
             raise ValueError("stateBits is 8 or 32, not %r" % (stateBits,))
         self.LearningRate, self.Beta1, self.Beta2, self.Epsilon = learningRate, beta1, beta2, epsilon
         self.StateBits, self.Seed, self.StepCount = stateBits, int(seed), int(step)
-        self._plan = None
+        self._plan, self._disposed = None, False
         for p, g, c in zip(parameters, gradients, copies):
             if p.Type != "float32" or g.Type not in ("float32", "bfloat16") or (c is not None and c.Type != "bfloat16"):
                 raise ValueError("parameters are float32, gradients float32 or bfloat16, copies bfloat16")
@@ -38,18 +38,18 @@ class AdamW:
             self._check_states(p, s)
         # the plan holds addresses: everything it points at stays alive with it
         self.Parameters, self.Gradients, self.States, self.Copies = list(parameters), list(gradients), [list(s) for s in states], list(copies)
-        self._step = AdamwStepDesc()
+        self._held = [t for tensors in zip(self.Parameters, self.Gradients, self.Copies, *zip(*self.States)) for t in tensors if t is not None]
         if not count:
             return
         self._lib, self._wrapper = parameters[0]._lib, parameters[0].Wrapper
+        w = self._wrapper
         table = (AdamwTensor * count)()
         for e, p, g, s, c, d in zip(table, parameters, gradients, self.States, copies, decay):
-            for t in [p, g] + s:
-                t.AssertIsNotDisposed()
-            e.parameter, e.gradient, e.moment1, e.moment2 = p.Pointer, g.Pointer, s[0].Pointer, s[1].Pointer
+            e.parameter, e.gradient = pointer_on(w, p), pointer_on(w, g)
+            e.moment1, e.moment2 = pointer_on(w, s[0]), pointer_on(w, s[1])
             if stateBits == 8:
-                e.scale1, e.scale2 = s[2].Pointer, s[3].Pointer
-            e.bf16_copy = c.Pointer if c is not None else None
+                e.scale1, e.scale2 = pointer_on(w, s[2]), pointer_on(w, s[3])
+            e.bf16_copy = pointer_on(w, c)
             e.count, e.gradient_type, e.weight_decay = p.Count, TYPES[g.Type], d
         plan = ctypes.c_void_p()
         check_status(self._lib.snhip_adamw_create(self._wrapper.handle, table, count, stateBits, ctypes.byref(plan)), "snhip_adamw_create")
@@ -75,17 +75,23 @@ class AdamW:
 
     def Step(self, learningRate=None, gradientScale=1.0):
         """One step with the gradients as they are, times gradientScale (1 / loss scale, or a clipping factor)."""
+        if self._disposed:
+            raise RuntimeError("AdamW is disposed")
+        for t in self._held:
+            if t._disposed:
+                raise RuntimeError("a tensor of the optimizer is disposed")
         if learningRate is not None:
             self.LearningRate = learningRate
         if self._plan is not None:
-            d = self._step
+            d = AdamwStepDesc()
             d.step, d.learning_rate, d.beta1, d.beta2 = self.StepCount + 1, self.LearningRate, self.Beta1, self.Beta2
             d.epsilon, d.gradient_scale, d.seed = self.Epsilon, gradientScale, self.Seed
             check_status(self._lib.snhip_adamw_step(self._wrapper.handle, self._plan, ctypes.byref(d)), "snhip_adamw_step")
         self.StepCount += 1
 
     def Dispose(self):
-        """Ends the plan; tensors stay with whoever holds them."""
+        """Ends the plan (and with it a captured graph's steps); tensors stay with whoever holds them."""
+        self._disposed = True
         plan, self._plan = self._plan, None
         if plan is not None:
             self._wrapper.synchronize()

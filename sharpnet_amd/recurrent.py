@@ -124,11 +124,11 @@ class RecurrentLayer:
             hy = hyAll
         cyAll = GPUTensor([self.K * self.num_layers, batchSize, self.hidden_size], None, self.Wrapper) if cy is not None else None
         check_status(self._lib.snhip_rnn_forward(
-            self.Wrapper.handle, ctypes.byref(self.desc), int(isTraining), batchSize, timeSteps, x.Pointer, ySeq.Pointer,
-            hx.Pointer if hx is not None else None, hy.Pointer if hy is not None else None,
-            cx.Pointer if cx is not None else None, cyAll.Pointer if cyAll is not None else None,
-            self._weightsAndBiases.Pointer, workSpace.Pointer, ws_bytes,
-            self._reserveSpace.Pointer if isTraining else None, rs_bytes), "snhip_rnn_forward")
+            self.Wrapper.handle, ctypes.byref(self.desc), int(isTraining), batchSize, timeSteps, x.FloatPointer, ySeq.FloatPointer,
+            hx.FloatPointer if hx is not None else None, hy.FloatPointer if hy is not None else None,
+            cx.FloatPointer if cx is not None else None, cyAll.FloatPointer if cyAll is not None else None,
+            self._weightsAndBiases.FloatPointer, workSpace.FloatPointer, ws_bytes,
+            self._reserveSpace.FloatPointer if isTraining else None, rs_bytes), "snhip_rnn_forward")
         if not self._returnSequences:
             top = hyAll.Slice((self.num_layers - 1) * self.K * batchSize * self.hidden_size,
                               [self.K, batchSize, self.hidden_size])
@@ -174,7 +174,7 @@ class RecurrentLayer:
                     dy.Slice(batchId * K * H + H, [H]).CopyTo(dySeq.Slice(batchId * timeSteps * K * H + H, [H]))
         ws_bytes, rs_bytes = self._buffers(True, batchSize, timeSteps)
         workSpace = GPUTensor([ws_bytes // 4], None, self.Wrapper)
-        ptr = lambda t: t.Pointer if t is not None else None
+        ptr = lambda t: t.FloatPointer if t is not None else None
         # cell-state gradients travel as (K * layers, batch, hidden); with one layer that is the block itself
         dcyAll = None
         if dcy is not None:
@@ -182,13 +182,13 @@ class RecurrentLayer:
             dcyAll.ZeroMemory()
             dcy.CopyTo(dcyAll.Slice((self.num_layers - 1) * K * batchSize * H, [K, batchSize, H]))
         check_status(self._lib.snhip_rnn_backward_data(
-            self.Wrapper.handle, ctypes.byref(self.desc), batchSize, timeSteps, ySeq.Pointer, dySeq.Pointer,
-            ptr(dx), ptr(hx), None, ptr(dhx), ptr(cx), ptr(dcyAll), ptr(dcx), self._weightsAndBiases.Pointer,
-            workSpace.Pointer, ws_bytes, self._reserveSpace.Pointer, rs_bytes), "snhip_rnn_backward_data")
+            self.Wrapper.handle, ctypes.byref(self.desc), batchSize, timeSteps, ySeq.FloatPointer, dySeq.FloatPointer,
+            ptr(dx), ptr(hx), None, ptr(dhx), ptr(cx), ptr(dcyAll), ptr(dcx), self._weightsAndBiases.FloatPointer,
+            workSpace.FloatPointer, ws_bytes, self._reserveSpace.FloatPointer, rs_bytes), "snhip_rnn_backward_data")
         self._weightsAndBiasesGradients.ZeroMemory()
         check_status(self._lib.snhip_rnn_backward_weights(
-            self.Wrapper.handle, ctypes.byref(self.desc), batchSize, timeSteps, x.Pointer, ptr(hx), ySeq.Pointer,
-            self._weightsAndBiasesGradients.Pointer, workSpace.Pointer, ws_bytes, self._reserveSpace.Pointer, rs_bytes),
+            self.Wrapper.handle, ctypes.byref(self.desc), batchSize, timeSteps, x.FloatPointer, ptr(hx), ySeq.FloatPointer,
+            self._weightsAndBiasesGradients.FloatPointer, workSpace.FloatPointer, ws_bytes, self._reserveSpace.FloatPointer, rs_bytes),
             "snhip_rnn_backward_weights")
         workSpace.Dispose()
         if dcyAll is not None:

@@ -630,6 +630,88 @@ def test_training_operators_on_two_streams_at_once(gpu_wrapper):
         check_status(w.lib.snhip_stream_destroy(s))
 
 
+def test_launches_of_more_workgroups_than_a_grid_row(gpu_wrapper):
+    """Launches of over 65536 workgroups are spread over two dimensions of the grid: inputs that repeat every few rows give
+    outputs that do, bit for bit."""
+    from sharpnet_amd import embedding, normalization, optimizer
+    w, rng = gpu_wrapper, np.random.default_rng(8)
+    # one row of 520 elements to a workgroup of 256 threads, four in turn
+    tokens, dim, period = 4 * 65536 + 4 * 8 + 3, 520, 71
+    W = rounded(rng.normal(0, 1, (period, dim)), "bfloat16")
+    y = empty(w, (tokens, dim), "bfloat16")
+    embedding.WordEmbedding(period, dim).ForwardPropagation(y, tensor(w, (np.arange(tokens) % period).astype(np.int32), "int32"),
+                                                            tensor(w, W, "bfloat16"))
+    y = y.ToNumpy().reshape(tokens, dim)
+    for k in range(0, tokens, period):
+        assert np.array_equal(y[k:k + period], W[:tokens - k]), k
+    del y
+    # four rows of 68 elements to a workgroup
+    rows, dim, period = 4 * 65536 + 1, 68, 64
+    x = np.resize(rng.normal(0, 1, (period, dim)).astype(np.float32), (rows, dim))
+    h, first = empty(w, (rows, dim)), empty(w, (period, dim))
+    layer = normalization.BlockNorm(dim, "layer")
+    layer.ForwardPropagation(tensor(w, x), h)
+    layer.ForwardPropagation(tensor(w, x[:period]), first)
+    h, first = h.ToNumpy(), first.ToNumpy()
+    assert np.all(np.isfinite(first)) and np.array_equal(h, np.resize(first, (rows, dim)))
+    # 1024 elements to a workgroup
+    sizes = [65535 * 1024 + 5, 3, 2048]
+    short = [2048, 3, 2048]
+    g = rng.normal(0, 1, 2048).astype(np.float32)
+    result = []
+    for lengths in (sizes, short):
+        parameters = [tensor(w, np.resize(np.float32(0.5) * g, n)) for n in lengths]
+        opt = optimizer.AdamW(parameters, [tensor(w, np.resize(g, n)) for n in lengths], **ADAM)
+        opt.Step()
+        result.append([t.ToNumpy() for tensors in [parameters] + opt.States for t in tensors])
+        opt.Dispose()
+    for a, b in zip(*result):
+        assert np.array_equal(a, np.resize(b, a.size))
+
+
+def test_scratch_memory_that_has_grown_after_a_capture(gpu_wrapper):
+    """A graph goes on using the scratch memory it was captured with when a longer batch has come along."""
+    from sharpnet_amd import embedding
+    from sharpnet_amd.hiplib import check_status
+    w, rng = gpu_wrapper, np.random.default_rng(9)
+    hip, vp = hip_runtime(), ctypes.c_void_p
+    layer = embedding.WordEmbedding(300, 40)
+
+    def batch(tokens):
+        x, dy = make_ids(rng, tokens, 300, "int32"), rng.normal(0, 1, (tokens, 40)).astype(np.float32)
+        return tensor(w, x, "int32"), tensor(w, dy), empty(w, (300, 40))
+    x, dy, dW = batch(5000)
+    layer.BackwardPropagation(dW, x, dy)
+    want = dW.ToNumpy().copy()
+    stream, graph, graph_exec = vp(), vp(), vp()
+    check_status(w.lib.snhip_stream_create(ctypes.byref(stream)), "snhip_stream_create")
+    check_status(w.lib.snhip_set_stream(w.handle, stream), "snhip_set_stream")
+    try:
+        assert hip.hipStreamBeginCapture(stream, 0) == 0
+        try:
+            layer.BackwardPropagation(dW, x, dy)
+        finally:
+            assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(graph_exec), graph, None, None, 0) == 0
+        for tokens in (9000, 30000):
+            longer = batch(tokens)
+            layer.BackwardPropagation(longer[2], longer[0], longer[1])
+            other = empty(w, (2 << 20,))  # where freed memory would go
+            dW.SetValue(float("nan"))
+            assert hip.hipGraphLaunch(graph_exec, stream) == 0
+            w.synchronize()
+            assert np.array_equal(dW.ToNumpy(), want), tokens
+            assert np.all(np.isnan(other.ToNumpy()))
+    finally:
+        check_status(w.lib.snhip_set_stream(w.handle, None), "snhip_set_stream")
+        if graph_exec:
+            hip.hipGraphExecDestroy(graph_exec)
+        if graph:
+            hip.hipGraphDestroy(graph)
+        check_status(w.lib.snhip_stream_destroy(stream), "snhip_stream_destroy")
+        layer.Dispose()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # together, as a training step uses them
 # ---------------------------------------------------------------------------------------------------------------

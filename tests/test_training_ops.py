@@ -189,14 +189,20 @@ def test_adamw_step_checks(lib, handle, change):
 
 class Stub:
     """Shape and type of a tensor, for the host side's checks."""
+    _disposed, _owner, handle = False, None, None
 
-    def __init__(self, shape, type_="float32"):
-        self.Shape, self.Type, self.Pointer = list(shape), type_, A
+    def __init__(self, shape, type_="float32", device=0):
+        self.Shape, self.Type, self.Pointer, self.device_id = list(shape), type_, A, device
         self.Count = int(np.prod(shape))
         self.lib = self._lib = self.Wrapper = self
 
     def AssertIsNotDisposed(self):
         pass
+
+    def __getattr__(self, name):  # as a library: calls that nothing was refused of
+        if not name.startswith("snhip_"):
+            raise AttributeError(name)
+        return lambda *args: 0
 
 
 def test_host_sides_refuse_what_does_not_fit():
@@ -234,6 +240,78 @@ def test_host_sides_refuse_what_does_not_fit():
         GPUTensor.FromPointer([4], A + 2, "float32", gpu_wrapper=p)
     t = GPUTensor.FromPointer([4], A + 2, "bfloat16", gpu_wrapper=p, owner=ids)
     assert t.ElementBytes == 2 and t.Slice(1, [2]).Pointer == A + 4 and t.Slice(1, [2]).Type == "bfloat16" and not t.IsOwnerOfMemory
+
+
+def test_host_sides_refuse_tensors_of_another_device():
+    from sharpnet_amd import embedding, normalization, optimizer
+    e, n = embedding.WordEmbedding(7, 6), normalization.BlockNorm(6, "rms")
+    ids, y, table, far = Stub((10,), "int32"), Stub((10, 6)), Stub((7, 6)), Stub((7, 6), device=1)
+    for call in (lambda: e.ForwardPropagation(y, ids, far), lambda: e.BackwardPropagation(far, ids, y),
+                 lambda: n.ForwardPropagation(y, Stub((10, 6), device=1)), lambda: n.BackwardPropagation(y, Stub((10, 6), device=1), y),
+                 lambda: optimizer.AdamW([table], [far], states=[[table, table]])):
+        with pytest.raises(ValueError, match="device 1"):
+            call()
+
+
+def test_entry_points_that_compute_with_float32_refuse_other_types():
+    from sharpnet_amd import GPUTensor, attention, linear
+    w = Stub((1,))
+    new = lambda type_, *shape: GPUTensor.FromPointer(list(shape), A, type_, gpu_wrapper=w)  # noqa: E731
+    f, b = new("float32", 4, 4), new("bfloat16", 4, 4)
+    f3, b3, v = new("float32", 2, 4, 4), new("bfloat16", 2, 4, 4), new("int32", 4)
+    for call in (lambda: f.Dot(f, False, b, False), lambda: b.Dot(f, f), lambda: f3.BatchMatrixMultiplication(b3, False, f3, False, 1.0, 0.0),
+                 lambda: f.DotRowMajor(f, False, f, False, 1.0, 0.0, bias=v), lambda: f.GemmEx(A=b, B=f), lambda: f.GemmEx(A=b, B=f, bias=b, math=2),
+                 lambda: b.Compute_BiasGradient_from_dy(new("float32", 4)), lambda: f.Update_Adding_Alpha_X(1.0, b),
+                 lambda: b.SoftmaxLastDimension(f), lambda: f.Transpose(b), lambda: f.ActivationForward("CUDNN_ACTIVATION_RELU", 0.0, b),
+                 lambda: b.SetValue(1.0), lambda: linear.DenseForwardPropagation(f, f, b, None, False),
+                 lambda: attention.fused_attention_forward(f3, f3, b3, f3, None, batch=2, heads=1, tq=4, tkv=4, dk=4, dv=4, scale=1.0,
+                                                           is_causal=False, packed=False)):
+        with pytest.raises(ValueError, match="float32"):
+            call()
+    assert f.FloatPointer == f.Pointer == A
+
+
+def test_workspace_of_a_layer():
+    """One for each wrapper; a longer one leaves the one before in place until Dispose."""
+    from sharpnet_amd.gpu_tensor import LayerWorkspace
+
+    class Wrapper:
+        def __init__(self):
+            self.lib, self.live = None, []
+
+        def allocate(self, nbytes):
+            self.live.append(nbytes)
+            return A + len(self.live)
+
+        def release(self, pointer, nbytes):
+            self.live.remove(nbytes)
+
+    a, b, held = Wrapper(), Wrapper(), LayerWorkspace()
+    assert held.Get(a, 0) is None and not a.live
+    first = held.Get(a, 1000)
+    assert held.Get(a, 800) is first and held.Get(b, 800) is not first
+    second = held.Get(a, 1001)
+    assert second.Count == 1500 and not first._disposed and a.live == [1000, 1500] and b.live == [800]
+    held.Dispose()
+    assert first._disposed and second._disposed and not a.live and not b.live
+
+
+def test_adamw_after_its_end():
+    from sharpnet_amd import optimizer
+    tensors = [Stub((3, 4)) for _ in range(4)]
+    opt = optimizer.AdamW([], [])
+    opt.Step()
+    assert opt.StepCount == 1
+    opt.Dispose()
+    with pytest.raises(RuntimeError):
+        opt.Step()
+    assert opt.StepCount == 1
+    opt = optimizer.AdamW.__new__(optimizer.AdamW)
+    opt._disposed, opt._plan, opt._held, opt.StepCount = False, None, tensors, 3
+    tensors[2]._disposed = True
+    with pytest.raises(RuntimeError):
+        opt.Step()
+    assert opt.StepCount == 3
 
 
 # ---- the plain forms ------------------------------------------------------------------------------------------------
