@@ -186,7 +186,7 @@ struct BlockNormPlan {
 };
 // How the rows are cut into chunks, one workgroup each: as many as are on the compute units at a time (two workgroups to a
 // unit for long rows, four for short ones).  More would only add column sums on their way to memory and back
-// (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us).
+// (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us, before they took 5.7).
 long long block_norm_chunks(int dim) { return dim > 1024 ? 512 : 1024; }
 BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     BlockNormPlan b{};
@@ -500,7 +500,7 @@ int snhip_block_norm_backward(void* handle, const snhip_block_norm_desc* desc, v
     // (a gate vector without rows has one group and no chunks: its gradient is cleared like the others)
     const long long gate_jobs = b.slots[4] < 0 ? 0 : desc->gate_rows == 0 ? 1 : b.groups;
     if (j.vectors + gate_jobs > 0)
-        hipLaunchKernelGGL(column_parts_kernel, dim3((unsigned)ceil_div(p.dim, 64), (unsigned)(j.vectors + gate_jobs)), dim3(1024), 0,
+        hipLaunchKernelGGL(column_parts_kernel, dim3((unsigned)ceil_div(p.dim, 32), (unsigned)(j.vectors + gate_jobs)), dim3(1024), 0,
                            h->stream, j);
     return hip_to_status(hipGetLastError());
 }
