@@ -6,7 +6,9 @@
 // Both are bound by HBM.  The gradient is built without float atomics, in an order that depends on the ids alone, so its
 // bits repeat: the tokens are sorted by id (embedding_sort_kernel), runs of equal ids are added up in chunks of the sorted
 // order (embedding_grad_kernel), and runs that cross a chunk's end are joined from their chunks' sums
-// (embedding_join_kernel, which also clears the rows that no token has).
+// (embedding_join_kernel, which also clears the rows that no token has).  65536 tokens x 1024 bf16 into 50000 rows: sort 5 and
+// 13 us, sums 45 us (4.3 TB/s of rows that lie anywhere), joins and clearing 31 us; together 95 us.  Clearing beside the sums
+// instead of beside the joins took 3 us more.  The lookup of 32768 x 2048, fp32 to bf16, 62 us.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -81,14 +83,13 @@ __global__ void __launch_bounds__(256) embedding_forward_kernel(const EmbeddingP
 
 // The sort.  Ids are dealt out to the workgroups of embedding_sort_kernel in turn (words come by frequency in most
 // vocabularies: neighbours would put half of all tokens into one workgroup): id i is number i / B of bucket i % B, its key
-// rank * bins + i / B with the
-// buckets ranked by i % 256 first.  The workgroup of a bucket finds its tokens in the order of their positions, a contiguous part to
-// each of its 16 wavefronts, and counts them by wavefront and id in LDS; after a scan over (id, wavefront) every wavefront
-// puts its tokens behind the earlier ones of their ids.  The order of all this is a function of the ids alone.
-// Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (8192 tokens
-// of 512: 29 us instead of 36 us).
-// With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup reads its own alone
-// (65536 tokens: 34 us the first way, 18 us the second).
+// rank * bins + i / B with the buckets ranked by i % 256 first.  The workgroup of a bucket finds its tokens in the order of
+// their positions, a contiguous part to each of its 16 wavefronts, and counts them by wavefront and id in LDS; after a scan
+// over (id, wavefront) every wavefront puts its tokens behind the earlier ones of their ids.  The order of all this is a
+// function of the ids alone.
+// Where the tokens come from: with few of them every workgroup reads all ids, which saves a launch (8192 tokens of 512: 29 us
+// instead of 36 us).  With many, embedding_bucket_kernel has sorted the tokens by bucket, in pieces, so that a workgroup
+// reads its own alone (65536 tokens: 34 us the first way, 18 us the second).
 constexpr int kSortDirect = 8192; // tokens up to which every workgroup reads all ids
 constexpr int kPiece = 512;       // tokens that a workgroup of embedding_bucket_kernel sorts
 constexpr int kBuckets = 256;     // ... by bucket (bucket modulo 256 if there are more)
@@ -313,7 +314,8 @@ __global__ void __launch_bounds__(1024) embedding_sort_pieces_kernel(const Embed
     if (lane == 0) below[w] = smaller;
     __syncthreads();
     start_ids(p, count, below, wave_total);
-    const bool held = begin < end && end - begin <= U && longest > 0 && longest <= 64;  // all of this wavefront's tokens are in its registers still
+    // all of this wavefront's tokens are in its registers still
+    const bool held = begin < end && end - begin <= U && longest > 0 && longest <= 64;
     auto put = [&](int j, int at) { p.order[at] = token[j], p.sorted[at] = rank * p.bins + (id[j] >> p.sort_log2); };
     if (held) {
 #pragma unroll
