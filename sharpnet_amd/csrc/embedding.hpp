@@ -45,7 +45,8 @@ struct EmbeddingParams {
     int fine_log2;               // ... over 256 of them: 2^fine_log2 times 256
     int bins, bins_log2;         // ids of each (at most 512), and the bits that number them
     int chunk;        // sorted tokens per group of threads of the gradient
-    long long chunk_blocks;  // workgroups that add up or join chunks; those behind them clear rows without tokens
+    unsigned int join_blocks, join_columns;  // workgroups that join chunks, and how many of them share one's columns
+    unsigned int clear_columns;              // the same of those behind them, which clear rows without tokens
     int* order;       // [tokens]: token numbers, sorted by key (see embedding_sort_kernel)
     int* sorted;      // [tokens]: their ids' keys
     int* offsets;     // [sort_blocks * bins + 1]: where each key's run starts in `order`
@@ -432,20 +433,25 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(const EmbeddingPara
 }
 
 constexpr int kClearRows = 8;  // that a group of threads looks at
+constexpr int kJoinLanes = 16, kJoinGroups = 256 / kJoinLanes, kJoinColumns = 4 * kJoinLanes;
+constexpr int kLongJoin = 16;  // parts that a group adds up by itself
 
-// The rows whose run crosses the end of a chunk: the group of the chunk where the run starts adds its part and those of the
-// chunks behind it, in their order, in 64 bits (a frequent word has thousands of parts).  The same launch clears the rows that
-// no token has: the few long sums wait for memory while the stores go out.
+// The rows whose run crosses the end of a chunk: the parts of the chunk where the run starts and of those behind it, added in
+// 64 bits (a frequent word has thousands of parts) in an order that depends on their number alone.  A group of 16 threads
+// takes 64 columns of a run, up to 16 parts, eight under way together; a longer run is all 16 groups' of the workgroup, every
+// 16th part each, whose sums meet in LDS (15920 tokens x 80, 131 parts to the most frequent word: 16 us one after the other,
+// 5 us).  The same launch clears the rows that no token has, while the sums wait for memory.
 __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingParams p) {
-    constexpr int U = 16;
-    const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
-    const int groups = 256 >> p.lanes_log2;
-    const int c = (blockIdx.y << (p.lanes_log2 + 2)) + 4 * lane;
-    if (c >= p.dim) return;
-    const int left = p.dim - c;
-    if (blockIdx.x >= p.chunk_blocks) {  // rows that no token has, in the order of their keys: neighbours in `offsets`
+    __shared__ double meet[kJoinGroups][4][kJoinLanes];
+    __shared__ int long_runs[kJoinGroups], n_long;
+    if (blockIdx.x >= p.join_blocks) {  // rows that no token has, in the order of their keys: neighbours in `offsets`
+        const int lane = threadIdx.x & ((1 << p.lanes_log2) - 1), group = threadIdx.x >> p.lanes_log2;
+        const int groups = 256 >> p.lanes_log2;
+        const unsigned int block = blockIdx.x - p.join_blocks, at_key = block / p.clear_columns;
+        const int c = (int)((block - at_key * p.clear_columns) << (p.lanes_log2 + 2)) + 4 * lane;
+        if (c >= p.dim) return;
         const int keys = p.sort_blocks * p.bins;
-        const long long k0 = ((blockIdx.x - p.chunk_blocks) * groups + group) * kClearRows;
+        const long long k0 = ((long long)at_key * groups + group) * kClearRows;
         if (k0 >= keys) return;
         const int first = (int)k0, here = keys - first < kClearRows ? keys - first : kClearRows;
         int at[kClearRows + 1];
@@ -455,29 +461,65 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
         for (int k = 0; k < kClearRows; ++k) {
             const int id = id_of_key(p, first + k);
             if (k < here && at[k] == at[k + 1] && id < p.vocabulary)
-                store4(static_cast<float*>(p.out) + (long long)id * p.ld_out + c, left, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                store4(static_cast<float*>(p.out) + (long long)id * p.ld_out + c, p.dim - c, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         }
         return;
     }
-    const long long k = (long long)blockIdx.x * groups + group;
-    if (k >= p.chunks) return;
-    const int key = p.crossing[2 * k], k_end = p.crossing[2 * k + 1];
-    if (key < 0) return;
-    const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim + c, left);
-    double sum[4] = {first[0], first[1], first[2], first[3]};
-    for (long long q = k + 1; q <= k_end; q += U) {
-        f32x4 v[U];
+    const int lane = threadIdx.x & (kJoinLanes - 1), group = threadIdx.x / kJoinLanes;
+    const unsigned int block = blockIdx.x / p.join_columns;
+    const int c = (int)(blockIdx.x - block * p.join_columns) * kJoinColumns + 4 * lane, left = p.dim - c;
+    const long long k = (long long)block * kJoinGroups + group;
+    int key = -1, k_end = 0;
+    if (k < p.chunks) key = p.crossing[2 * k], k_end = p.crossing[2 * k + 1];
+    if (threadIdx.x == 0) n_long = 0;
+    __syncthreads();
+    // sum += the parts of chunks q, q + step ... to the last
+    auto add_parts = [&](double (&sum)[4], long long q, long long last, int step) {
+        constexpr int U = 8;
+        for (; q <= last; q += U * step) {
+            f32x4 v[U];
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (q + j <= k_end) v[j] = load4(p.partial + 2 * (q + j) * p.dim + c, left);
+            for (int j = 0; j < U; ++j) {
+                v[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (q + j * step <= last) v[j] = load4(p.partial + 2 * (q + j * step) * p.dim + c, left);
+            }
+#pragma unroll
+            for (int j = 0; j < U; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += v[j][e];
         }
-#pragma unroll
-        for (int j = 0; j < U; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum[e] += v[j][e];
+    };
+    if (key >= 0 && k_end - k > kLongJoin) {
+        if (lane == 0) long_runs[atomicAdd(&n_long, 1)] = group;  // (in any order: their rows have nothing to do with each other)
+    } else if (key >= 0 && left > 0) {
+        const f32x4 first = load4(p.partial + (2 * k + 1) * p.dim + c, left);
+        double sum[4] = {first[0], first[1], first[2], first[3]};
+        add_parts(sum, k + 1, k_end, 1);
+        put_gradient(p, key, c, f32x4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
     }
-    put_gradient(p, key, c, f32x4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
+    __syncthreads();
+    for (int i = 0; i < n_long; ++i) {
+        const long long from = (long long)block * kJoinGroups + long_runs[i];
+        const int run_key = p.crossing[2 * from], last = p.crossing[2 * from + 1];
+        double sum[4] = {0.0, 0.0, 0.0, 0.0};
+        if (left > 0) {
+            if (group == 0) {
+                const f32x4 first = load4(p.partial + (2 * from + 1) * p.dim + c, left);
+                for (int e = 0; e < 4; ++e) sum[e] = first[e];
+            }
+            add_parts(sum, from + 1 + group, last, kJoinGroups);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) meet[group][e][lane] = sum[e];
+        __syncthreads();
+        if (group == 0 && left > 0) {
+            for (int g = 1; g < kJoinGroups; ++g)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += meet[g][e][lane];
+            put_gradient(p, run_key, c, f32x4{(float)sum[0], (float)sum[1], (float)sum[2], (float)sum[3]});
+        }
+    }
 }
 
 // The whole gradient in one launch, for few tokens (kSmallTokens) and few elements of dy (kSmallElements): the workgroup of a

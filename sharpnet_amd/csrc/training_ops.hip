@@ -406,7 +406,7 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
     p.piece_start = reinterpret_cast<int*>(ws + e.piece_start);
     p.crossing = reinterpret_cast<int*>(ws + e.crossing), p.chunks = e.chunks;
     const int groups = 256 >> p.lanes_log2;
-    p.chunk_blocks = (e.chunks + groups - 1) / groups;
+    const long long chunk_blocks = (e.chunks + groups - 1) / groups;
     if (desc->id_type == SNHIP_TYPE_F32)
         embedding_sort_launch<float>(p, sort_grid, lds, h->stream);
     else if (desc->id_type == SNHIP_TYPE_I32)
@@ -415,17 +415,17 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
         embedding_sort_launch<long long>(p, sort_grid, lds, h->stream);
     const long long keys = (long long)p.sort_blocks * p.bins;
     const long long clear_blocks = p.accumulate ? 0 : (keys + kClearRows * groups - 1) / (kClearRows * groups);
-    const dim3 chunk_grid((unsigned)p.chunk_blocks, (unsigned)col_blocks);
-    if (p.chunk_blocks > 0) {
+    const dim3 chunk_grid((unsigned)chunk_blocks, (unsigned)col_blocks);
+    if (chunk_blocks > 0) {
         if (desc->output_type == SNHIP_TYPE_BF16)
             hipLaunchKernelGGL(embedding_grad_kernel<__bf16>, chunk_grid, dim3(256), 0, h->stream, p);
         else
             hipLaunchKernelGGL(embedding_grad_kernel<float>, chunk_grid, dim3(256), 0, h->stream, p);
     }
-    if (e.chunks <= 1) p.chunk_blocks = 0;  // nothing to join
-    if (p.chunk_blocks + clear_blocks > 0)
-        hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)(p.chunk_blocks + clear_blocks), (unsigned)col_blocks), dim3(256), 0,
-                           h->stream, p);
+    p.join_columns = (unsigned)ceil_div(p.dim, kJoinColumns), p.clear_columns = (unsigned)col_blocks;
+    p.join_blocks = e.chunks <= 1 ? 0 : (unsigned)((e.chunks + kJoinGroups - 1) / kJoinGroups * p.join_columns);
+    if (p.join_blocks + clear_blocks > 0)
+        hipLaunchKernelGGL(embedding_join_kernel, dim3((unsigned)(p.join_blocks + clear_blocks * col_blocks)), dim3(256), 0, h->stream, p);
     return hip_to_status(hipGetLastError());
 }
 
