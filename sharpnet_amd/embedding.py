@@ -27,24 +27,24 @@ class WordEmbedding:
         self.Wrapper = gpu_wrapper
         self._tableShape = [self.VocabularySize, self.EmbeddingDim]
         self._workspace = LayerWorkspace()
-        self._mine = threading.local()  # a descriptor for each thread; a call fills in all but the sizes
+        self._mine = threading.local()  # for each thread: its last call's sizes and types, and their descriptor
 
     def _desc(self, x, rows, table_type):
         """rows: y or dy, (..., EmbeddingDim) with one row per id of x."""
-        if x.Type not in _ID_TYPES:
-            raise ValueError("ids must be float32, int32 or int64, not %s" % x.Type)
-        if rows.Type not in _ROW_TYPES or table_type not in _ROW_TYPES:
-            raise ValueError("rows and table must be float32 or bfloat16, not %s and %s" % (rows.Type, table_type))
-        tokens = math.prod(x.Shape)
-        if rows.Shape[-1] != self.EmbeddingDim or math.prod(rows.Shape) != tokens * self.EmbeddingDim:
-            raise ValueError("%s ids and rows of %s do not fit an embedding dimension of %d" % (x.Shape, rows.Shape, self.EmbeddingDim))
-        try:
-            d = self._mine.desc
-        except AttributeError:
-            d = self._mine.desc = EmbeddingDesc(vocabulary=self.VocabularySize, dim=self.EmbeddingDim)
-        d.id_type, d.table_type, d.output_type, d.tokens = _ID_TYPES[x.Type], _ROW_TYPES[table_type], _ROW_TYPES[rows.Type], tokens
-        d.padding_index, d.scale = self.PaddingIndex, self.Scale
-        return d
+        tokens, mine, dim = math.prod(x.Shape), self._mine.__dict__, self.EmbeddingDim
+        if rows.Shape[-1] != dim or math.prod(rows.Shape) != tokens * dim:
+            raise ValueError("%s ids and rows of %s do not fit an embedding dimension of %d" % (x.Shape, rows.Shape, dim))
+        call = (x.Type, table_type, rows.Type, tokens, self.PaddingIndex, self.Scale)
+        if mine.get("call") != call:
+            if x.Type not in _ID_TYPES:
+                raise ValueError("ids must be float32, int32 or int64, not %s" % x.Type)
+            if rows.Type not in _ROW_TYPES or table_type not in _ROW_TYPES:
+                raise ValueError("rows and table must be float32 or bfloat16, not %s and %s" % (rows.Type, table_type))
+            mine["desc"] = EmbeddingDesc(id_type=_ID_TYPES[x.Type], table_type=_ROW_TYPES[table_type], output_type=_ROW_TYPES[rows.Type],
+                                         tokens=tokens, vocabulary=self.VocabularySize, dim=dim, padding_index=self.PaddingIndex,
+                                         scale=self.Scale)
+            mine["call"] = call
+        return mine["desc"]
 
     def _check_table(self, table):
         if table.Shape != self._tableShape:
