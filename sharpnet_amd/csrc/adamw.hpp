@@ -1,6 +1,6 @@
 // AdamW over the elements of many tensors in one launch (definitions: include/sharpnet_hip.h, snhip_adamw_create).
 // Bound by HBM: 28 bytes an element with states in 32 bits, 16 with states in 8 (and an fp32 gradient), each read and
-// written once: 153M elements with fp32 states and bf16 copies (4.28 GB) 700 to 740 us, 5.8 to 6.1 TB/s; 353M with states in 8
+// written once: 143M elements with fp32 states and bf16 copies (4.28 GB) 700 to 740 us, 5.8 to 6.1 TB/s; 353M with states in 8
 // bits, bf16 gradients and copies (5.66 GB) 960 to 985 us, 5.8 TB/s.  The 8-bit form is near the vector units' rate as well:
 // with a correctly rounded square root, maxima through LDS and 64-bit addresses it took 1120 us.
 // A workgroup of 256 threads updates a chunk of a tensor, four neighbouring elements to a thread: longer chunks only put off
