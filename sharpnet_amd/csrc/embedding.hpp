@@ -524,16 +524,17 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
 
 // The whole gradient in one launch, for few tokens (kSmallTokens) and few elements of dy (kSmallElements): the workgroup of a
 // bucket sorts its tokens in LDS as embedding_sort_kernel does and goes on to add up the rows of its ids.  A group of threads
-// takes an id at a time; ids with more than kLongRun tokens are left to all groups together, whose sums meet in LDS.  One
-// workgroup sums a frequent word's rows alone, which is what bounds the size (4000 x 100: 19 us in three launches, 11.5
-// us in one; 1024 x 1024 into 32000 rows: 37 us in three, 43 us in one).
-constexpr int kSmallTokens = 4096, kLongRun = 32;
+// takes an id at a time; ids with more than a group's share of the bucket's tokens (and than kLongRun) are left to all groups
+// together, whose sums meet in LDS (1024 x 512 into 32000 rows: 22 us with kLongRun = 32, 18 us with 8).  One workgroup sums a
+// frequent word's rows alone, which is what bounds the size (4000 x 100: 19 us in three launches, 11.5 us in one; 1024 x
+// 1024 into 32000 rows: 37 us in three, 43 us in one).
+constexpr int kSmallTokens = 4096, kLongRun = 8, kSmallGroups = 128;  // (most groups of a workgroup: 8 threads each)
 constexpr long long kSmallElements = 1LL << 19;
 
 template <typename ID, typename T>
 __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingParams p) {
     extern __shared__ int count[];  // [16][bins], then the cursors; at the end the groups' sums, 16 KB
-    __shared__ int wave_total[16], starts[513], long_runs[kSmallTokens / kLongRun], n_long;
+    __shared__ int wave_total[16], starts[513], long_runs[kSmallGroups], n_long;
     constexpr int PER = kSmallTokens / 1024, U = 8;
     if (threadIdx.x == 0) n_long = 0;
     __shared__ unsigned short notes[16][kSmallTokens / 16], order[kSmallTokens];
@@ -563,9 +564,14 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
     __syncthreads();
     int start, total;
     scan_counts<16>(count, bins, 0, wave_total, start, total);
+    const int glane = tid & ((1 << p.lanes_log2) - 1), group = tid >> p.lanes_log2, groups = 1024 >> p.lanes_log2;
+    int share = 0;  // of the bucket's tokens: fewer than `groups` runs are longer
+#pragma unroll
+    for (int k = 0; k < 16; ++k) share += wave_total[k];
+    share = share / groups > kLongRun ? share / groups : kLongRun;
     if (tid < bins) {
         starts[tid] = start;
-        if (total > kLongRun) long_runs[atomicAdd(&n_long, 1)] = tid;  // (in any order: their rows have nothing to do with each other)
+        if (total > share) long_runs[atomicAdd(&n_long, 1)] = tid;  // (in any order: their rows have nothing to do with each other)
     }
     if (tid == bins - 1) starts[bins] = start + total;
     for (int k = 0; k < noted; k += 64) {
@@ -576,7 +582,6 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
         if (in) order[at] = (unsigned short)t;
     }
     __syncthreads();
-    const int glane = tid & ((1 << p.lanes_log2) - 1), group = tid >> p.lanes_log2, groups = 1024 >> p.lanes_log2;
     f32x4* sums = reinterpret_cast<f32x4*>(count);
     for (int c0 = 0; c0 < p.dim; c0 += 4 << p.lanes_log2) {
         const int c = c0 + 4 * glane, left = p.dim - c;
@@ -601,7 +606,7 @@ __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingPa
         for (int number = group; number < bins; number += groups) {
             const int a = starts[number], b = starts[number + 1];
             const int row = (number << p.sort_log2) | rank;
-            if (b - a > kLongRun || row >= p.vocabulary || left <= 0) continue;
+            if (b - a > share || row >= p.vocabulary || left <= 0) continue;
             if (b > a)
                 put_gradient(p, rank * bins + number, c, add_up(a, b, 1));
             else if (!p.accumulate)

@@ -152,6 +152,20 @@ def test_embedding_backward(gpu_wrapper, tokens, vocabulary, dim, ids, rows):
         assert np.array_equal(into.ToNumpy()[absent], start[absent])
 
 
+@pytest.mark.parametrize("tokens,words,dim", [(4000, 10, 20), (2000, 20, 256), (4096, 400, 30), (3000, 1, 129), (9000, 700, 16), (20000, 900, 40)])
+def test_embedding_backward_of_ids_that_share_a_bucket(gpu_wrapper, tokens, words, dim):
+    """Ids that are all multiples of 512: whatever sorts them by their low bits has them in one place."""
+    from sharpnet_amd import embedding
+    w, rng = gpu_wrapper, np.random.default_rng(words)
+    vocabulary = 512 * words
+    x = (512 * rng.integers(0, words, tokens)).astype(np.int32)
+    x[: tokens // 3] = 512 * (words // 2)  # one of them is frequent
+    dy = rng.normal(0, 1, (tokens, dim)).astype(np.float32)
+    dW = empty(w, (vocabulary, dim))
+    embedding.WordEmbedding(vocabulary, dim).BackwardPropagation(dW, tensor(w, x, "int32"), tensor(w, dy))
+    within(dW.ToNumpy(), *ref.embedding_backward(x, dy, vocabulary, 1.0), "dW")
+
+
 def test_embedding_without_tokens_or_columns(gpu_wrapper):
     from sharpnet_amd import embedding
     w = gpu_wrapper
