@@ -526,10 +526,10 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(const EmbeddingPara
 // bucket sorts its tokens in LDS as embedding_sort_kernel does and goes on to add up the rows of its ids.  A group of threads
 // takes an id at a time; ids with more than a group's share of the bucket's tokens (and than kLongRun) are left to all groups
 // together, whose sums meet in LDS (1024 x 512 into 32000 rows: 22 us with kLongRun = 32, 18 us with 8).  One workgroup sums a
-// frequent word's rows alone, which is what bounds the size (4000 x 100: 19 us in three launches, 11.5 us in one; 1024 x
-// 1024 into 32000 rows: 37 us in three, 43 us in one).
+// frequent word's rows alone, which is what bounds the size (4000 x 100: 19 us in three launches, 11.5 us in one; 2048 x 512
+// 23 and 21 us; 2048 x 1024 38 and 49 us).
 constexpr int kSmallTokens = 4096, kLongRun = 8, kSmallGroups = 128;  // (most groups of a workgroup: 8 threads each)
-constexpr long long kSmallElements = 1LL << 19;
+constexpr long long kSmallElements = 1LL << 20;
 
 template <typename ID, typename T>
 __global__ void __launch_bounds__(1024) embedding_small_kernel(const EmbeddingParams p) {

@@ -118,7 +118,7 @@ BACKWARD = [(1, 1, 1, "int32", "float32"), (8, 3, 4, "int64", "float32"), (9, 3,
             (20000, 1, 12, "int32", "float32"), (8192, 600, 4, "int32", "float32"), (8193, 600, 4, "int64", "bfloat16"),
             (9000, 140001, 8, "float32", "float32"), (4096, 256, 256, "int32", "float32"), (4097, 256, 5, "int32", "float32"),
             (1000, 131072, 9, "int64", "bfloat16"), (900, 1, 1027, "int32", "float32"), (300, 2, 1030, "int32", "bfloat16"), (70000, 7, 3, "int64", "float32"),
-            (12000, 40, 150, "int32", "float32"), (17000, 30, 700, "int64", "bfloat16")]
+            (4096, 700, 256, "int64", "bfloat16"), (4096, 256, 257, "int32", "float32"), (12000, 40, 150, "int32", "float32"), (17000, 30, 700, "int64", "bfloat16")]
 
 
 @pytest.mark.parametrize("tokens,vocabulary,dim,ids,rows", BACKWARD)
