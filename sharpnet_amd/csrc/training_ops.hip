@@ -251,6 +251,8 @@ struct AdamwPlan {
     const int* owner = nullptr;
 };
 
+constexpr long long kAdamwMaxChunks = 0x7fffffff;  // their numbers are 32-bit integers
+
 struct Range {
     uintptr_t begin, end;
     bool written;
@@ -279,6 +281,10 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
         e = AdamwEntry{t.parameter, t.gradient, t.moment1, t.moment2, t.scale1, t.scale2, static_cast<__bf16*>(t.bf16_copy),
                        t.count, 0, t.weight_decay, t.gradient_type == SNHIP_TYPE_BF16};
         if (t.count == 0) continue;
+        if (t.count > kAdamwMaxChunks * kAdamwChunk) return SNHIP_STATUS_NOT_SUPPORTED;
+        e.first_chunk = chunks;
+        chunks += (t.count + kAdamwChunk - 1) / kAdamwChunk;
+        if (chunks > kAdamwMaxChunks) return SNHIP_STATUS_NOT_SUPPORTED;
         const size_t gb = type_bytes(t.gradient_type);
         if (t.parameter == nullptr || t.gradient == nullptr || t.moment1 == nullptr || t.moment2 == nullptr ||
             (state_bits == 8 && (t.scale1 == nullptr || t.scale2 == nullptr)))
@@ -299,11 +305,6 @@ int adamw_build(Handle* h, const snhip_adamw_tensor* tensors, int count, int sta
         add(t.gradient, gb * n, false);
         elements += t.count;
     }
-    for (AdamwEntry& e : entries) {
-        e.first_chunk = chunks;
-        chunks += (e.count + kAdamwChunk - 1) / kAdamwChunk;
-    }
-    if (chunks > 0x7fffffffLL) return SNHIP_STATUS_NOT_SUPPORTED;
     if (overlapping(ranges)) return SNHIP_STATUS_INVALID_VALUE;
     DeviceScope scope(h->device);
     if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;

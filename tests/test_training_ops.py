@@ -166,6 +166,8 @@ def test_adamw_scales_several_tensors_and_arguments(lib, handle):
     assert create(adamw_tensors({}, {"parameter": A + 4000}), 2, 32) == OK_SO_FAR
     assert create(adamw_tensors({}, {"gradient": A + 0x10000}), 2, 32) == OK_SO_FAR   # gradients are only read
     assert create(adamw_tensors({}), 1, 16) == UNSUPPORTED
+    assert create(adamw_tensors({"count": 2 ** 62}), 1, 32) == create(adamw_tensors({"count": 2 ** 63 - 1}), 1, 8) == UNSUPPORTED
+    assert create(adamw_tensors({"count": 2 ** 40}, {"count": 2 ** 40}), 2, 8) == UNSUPPORTED   # 2^31 chunks
     assert create(None, 1, 32) == BAD and create(adamw_tensors({}), -1, 32) == BAD
     assert lib.snhip_adamw_create(handle, None, 0, 32, None) == BAD
     assert lib.snhip_adamw_create(None, None, 0, 32, ctypes.byref(plan)) == S.CUBLAS_STATUS_NOT_INITIALIZED
