@@ -62,14 +62,16 @@ void backward_kind(const BlockNormParams& p, BlockNormKind k, hipStream_t stream
 
 }  // namespace
 
-// A row of up to 1024 elements is one wavefront's (no barrier), a longer one a workgroup's: 16384 x 1024 bf16 31 us, with 256
-// threads to a row 34; 16384 x 2048 57 us, with a wavefront to a row 66, with 1024 threads 118.  With few rows to go round a row
-// is spread over as many threads as it has pieces of four: 8 x 1024 3.2 us instead of 4.0, 256 x 4096 4.4 instead of 5.2; rows of
-// 513 to 1024 elements keep that up to 4096 of them (1024 x 1024: 4.1 us instead of 4.9; 4096 x 1024 9.4 instead of 9.8).
+// A row of up to 1024 elements is one wavefront's or less (no barrier), a longer one a workgroup's: 16384 x 1024 bf16 31 us, with
+// 256 threads to a row 34; 16384 x 2048 57 us, with a wavefront to a row 66, with 1024 threads 118.  As many pieces to a thread as
+// the row needs: what lies behind it costs time, too (6000 x 5120 with five pieces 58 us, with eight 79).  With few rows to go
+// round a row is spread over as many threads as it has pieces of four: 8 x 1024 3.2 us instead of 4.0, 256 x 4096 4.4 instead
+// of 5.2; rows of 513 to 1024 elements keep that up to 4096 of them (1024 x 1024: 4.1 us instead of 4.9; 4096 x 1024 9.4
+// instead of 9.8).
 void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
     const int units = (p.dim + 3) / 4;
     if (units <= 16) return forward<16, 1>(p, stream);
-    if (units <= 32) return forward<16, 2>(p, stream);
+    if (units <= 32) return forward<32, 1>(p, stream);
     if (units <= 64) return forward<64, 1>(p, stream);
     if (p.rows <= 512) {
         if (units <= 256) return forward<256, 1>(p, stream);
@@ -77,17 +79,23 @@ void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
         return forward<1024, 2>(p, stream);
     }
     if (units <= 128) return forward<64, 2>(p, stream);
-    if (units <= 256) return p.rows <= 4096 ? forward<256, 1>(p, stream) : forward<64, 4>(p, stream);
+    if (units <= 256 && p.rows <= 4096) return forward<256, 1>(p, stream);
+    if (units <= 192) return forward<64, 3>(p, stream);
+    if (units <= 256) return forward<64, 4>(p, stream);
     if (units <= 512) return forward<256, 2>(p, stream);
+    if (units <= 768) return forward<256, 3>(p, stream);
     if (units <= 1024) return forward<256, 4>(p, stream);
+    if (units <= 1280) return forward<256, 5>(p, stream);
+    if (units <= 1536) return forward<256, 6>(p, stream);
     forward<256, 8>(p, stream);
 }
 
-// (the groups of threads per workgroup: block_norm_backward_groups)
+// One or two pieces to a thread: more took registers that the column sums need.  (32 threads to rows of up to 128: 30000 x 128
+// bf16 21 us, with 16 and two pieces 26.  The groups of threads per workgroup: block_norm_backward_groups.)
 void SNHIP_BACKWARD(const BlockNormParams& p, BlockNormKind kind, hipStream_t stream) {
     const int units = (p.dim + 3) / 4;
     if (units <= 16) return backward_kind<16, 1>(p, kind, stream);
-    if (units <= 32) return backward_kind<16, 2>(p, kind, stream);
+    if (units <= 32) return backward_kind<32, 1>(p, kind, stream);
     if (units <= 64) return backward_kind<64, 1>(p, kind, stream);
     if (units <= 128) return backward_kind<64, 2>(p, kind, stream);
     if (units <= 256) return backward_kind<256, 1>(p, kind, stream);

@@ -38,8 +38,8 @@ struct BlockNormParams {
 // ---- pieces of a row -----------------------------------------------------------------------------------------------
 // Exact rows are read and written as buffers of their own length: the base is scalar, the place in the row a 32-bit offset
 // (64-bit addresses for every piece of every tensor took a third of the vector registers), what is read behind the row's end is
-// zero and what is written there is dropped, without a branch.  Other rows (a buffer counts in 32-bit elements), and 16 threads
-// to a row, which share a wavefront with rows of other bases: plain accesses, wide at any address, the end of the row checked
+// zero and what is written there is dropped, without a branch.  Other rows (a buffer counts in 32-bit elements), and 16 or 32
+// threads to a row, which share a wavefront with rows of other bases: plain accesses, wide at any address, the end of the row checked
 // (16384 x 1001: backward 110 us against 100 us for 1000 columns).
 typedef unsigned int u32x2 __attribute__((vector_size(8)));
 typedef unsigned int u32x4 __attribute__((vector_size(16)));
@@ -123,12 +123,14 @@ struct Piece {
 };
 
 // ---- sums over a row -----------------------------------------------------------------------------------------------
-// Over the TPR threads of a row, TPR = 16 or a multiple of 64.  Beyond a wavefront the wavefronts' sums meet in LDS; `turn`
+// Over the TPR threads of a row, TPR = 16, 32 or a multiple of 64.  Beyond a wavefront the wavefronts' sums meet in LDS; `turn`
 // alternates between two places, so that one barrier a sum is enough.
 template <int TPR>
 __device__ __forceinline__ float lanes_sum(float a) {
     if constexpr (TPR == 16)
         return row16_sum(a);
+    else if constexpr (TPR == 32)
+        return half32_sum(a);
     else
         return wave64_sum(a);
 }
@@ -311,7 +313,7 @@ template <typename TS, typename TB, int TPR, int N, int MODE, bool BIAS, bool GA
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_kernel(const BlockNormParams p) {
     constexpr int NT = TPR > 256 ? TPR : 256, GROUPS = NT / TPR;
     typedef Piece<TPR, EXACT> P;
-    constexpr bool HAS_Y = MODE == 2 || GATE, BOTH = N == 1 || TPR == 16;
+    constexpr bool HAS_Y = MODE == 2 || GATE, BOTH = N == 1;
     __shared__ float lds[2][2][TPR / 64 + 1];
     constexpr int VECTORS = 1 + (BIAS ? 1 : 0) + (MODE == 2 ? 1 + (BIAS ? 1 : 0) : 0) + (GATE ? 1 : 0);  // of column sums
     __shared__ f32x4 meet[GROUPS > 1 ? VECTORS * GROUPS * TPR * N : 1];
@@ -348,8 +350,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
     const bool gate_in_rows = p.gate_rows != 0;
 
     // what the norm ahead of the next block needs of a row, and what the norm behind this one needs: the first part of the
-    // next row and the second part of this one are under way while the other is worked on.  (BOTH: with a piece or two to a
-    // thread the work on the first is over too soon for that, and there are registers for the next row's second part, too.)
+    // next row and the second part of this one are under way while the other is worked on.  (BOTH: with one piece to a thread the
+    // work on the first is over too soon for that, and there are registers for the next row's second part, too.)
     struct Ahead {
         raw4<TS> u[N], du[N];
         raw4<TB> dh[N];

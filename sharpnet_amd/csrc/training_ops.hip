@@ -184,10 +184,22 @@ struct BlockNormPlan {
     int groups_per_chunk, chunks_per_group, rows_per_chunk, chunks;
     size_t bytes;
 };
-// How the rows are cut into chunks, one workgroup each: as many as are on the compute units at a time (two workgroups to a
-// unit for long rows, four for short ones).  More would only add column sums on their way to memory and back
-// (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us, before they took 5.7).
-long long block_norm_chunks(int dim) { return dim > 1024 ? 512 : 1024; }
+// How the rows are cut into chunks, one workgroup each: as many as the compute units hold at a time.  More would only add
+// column sums on their way to memory and back (16384 x 4096, two vectors: 1024 chunks 13 us for them, 512 8 us, before they took
+// 5.7); with few rows fewer are enough.
+long long block_norm_chunks(const snhip_block_norm_desc* d) {
+    const bool gated = d->gate != nullptr, normed = d->post_norm != SNHIP_NORM_NONE, narrow = d->stream_type == SNHIP_TYPE_BF16;
+    // 16 wavefronts: one of a compute unit, two of the smallest kind (4096 x 8192 bf16: 512 chunks 131 us, 256 124 us; the norm
+    // alone 6000 x 5120 71 us and 79 us)
+    if (d->dim > 4096) return gated || normed || !narrow ? 256 : 512;
+    if (d->dim > 2048) return 512;
+    if (d->dim <= 1024) return 1024;
+    // four of a compute unit, or three with a gate and a norm to undo (12000 x 1280 bf16: 512 chunks 88 us, 1024 71 us; fp32 768
+    // 92 us instead of 101 us), if that leaves eight rows to each (2048 x 2048 fp32: 512 chunks 29 us, 1024 33 us)
+    const bool three = gated && normed && (!narrow || d->dim % 4 != 0);
+    const long long most = three ? 768 : 1024;
+    return d->rows >= 8 * most ? most : 512;
+}
 BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     BlockNormPlan b{};
     const bool gate_rows = d->gate != nullptr && d->gate_rows > 0;
@@ -195,7 +207,7 @@ BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     if (b.rows_per_group < 1) b.rows_per_group = 1;
     b.groups = (d->rows + b.rows_per_group - 1) / b.rows_per_group;
     const int at_once = block_norm_backward_groups(d->dim);
-    const long long wanted = block_norm_chunks(d->dim);
+    const long long wanted = block_norm_chunks(d);
     long long c = (d->rows + wanted - 1) / wanted;
     if (c < at_once) c = at_once;
     b.flush = gate_rows && b.rows_per_group <= c;

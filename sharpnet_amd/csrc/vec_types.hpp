@@ -100,7 +100,7 @@ __device__ __forceinline__ f32x4 existing(f32x4 v, int left, bool ends) {
     return r;
 }
 
-// Sums over 16 neighbouring lanes / over the wavefront, in every lane of them, without going through LDS: rotations within
+// Sums over 16 or 32 neighbouring lanes / over the wavefront, in every lane of them, without going through LDS: rotations within
 // rows of 16 lanes are free operands of the additions (ds_bpermute, what a shuffle becomes, is a round trip each).
 template <int ROTATE>
 __device__ __forceinline__ float add_rotated(float v) {
@@ -118,6 +118,12 @@ __device__ __forceinline__ float wave64_sum(float v) {
     const float a = __int_as_float(__builtin_amdgcn_readlane(r, 0)), b = __int_as_float(__builtin_amdgcn_readlane(r, 16));
     const float c = __int_as_float(__builtin_amdgcn_readlane(r, 32)), d = __int_as_float(__builtin_amdgcn_readlane(r, 48));
     return (a + b) + (c + d);
+}
+__device__ __forceinline__ float half32_sum(float v) {
+    const int r = __float_as_int(row16_sum(v));
+    const float a = __int_as_float(__builtin_amdgcn_readlane(r, 0)), b = __int_as_float(__builtin_amdgcn_readlane(r, 16));
+    const float c = __int_as_float(__builtin_amdgcn_readlane(r, 32)), d = __int_as_float(__builtin_amdgcn_readlane(r, 48));
+    return threadIdx.x & 32 ? c + d : a + b;
 }
 
 // Launches that can have more workgroups than the 2^32 - 1 threads of a grid's x hold are spread over x and z, with up to 8 z

@@ -202,7 +202,12 @@ NORMS = [(1, 1, "layer", None, None, None, True, "float32", "float32"),
          (513, 8190, "rms", "layer", 0, None, True, "float32", "bfloat16"),
          (5000, 12, "layer", "layer", 2, "sigmoid", True, "float32", "float32"),
          (2100, 40, "rms", "rms", 1000, None, False, "float32", "float32"),
-         (4100, 128, "layer", None, 0, "sigmoid", True, "bfloat16", "bfloat16")]
+         (4100, 128, "layer", None, 0, "sigmoid", True, "bfloat16", "bfloat16"),
+         (3001, 127, "layer", "rms", 5, "tanh", True, "float32", "bfloat16"), (37, 97, "rms", "layer", 0, None, False, "bfloat16", "bfloat16"),
+         (4200, 700, "layer", "rms", 0, None, False, "bfloat16", "bfloat16"), (4150, 1023, "rms", "layer", 9, "sigmoid", True, "float32", "float32"),
+         (600, 2600, "layer", "layer", 0, None, False, "float32", "bfloat16"), (550, 5001, "rms", None, 1, "tanh", True, "bfloat16", "bfloat16"),
+         (520, 6140, "layer", "rms", None, None, False, "float32", "float32"), (6200, 1028, "rms", "layer", 0, "sigmoid", False, "float32", "bfloat16"),
+         (8195, 1032, "layer", None, 4, None, True, "bfloat16", "bfloat16")]
 
 
 def norm_case(rng, rows, dim, pre, post, gate_rows, bias, stream, block):
