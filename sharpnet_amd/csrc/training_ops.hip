@@ -193,12 +193,14 @@ long long block_norm_chunks(const snhip_block_norm_desc* d) {
     // alone 6000 x 5120 71 us and 79 us)
     if (d->dim > 4096) return gated || normed || !narrow ? 256 : 512;
     if (d->dim > 2048) return 512;
-    if (d->dim <= 1024) return 1024;
-    // four of a compute unit, or three with a gate and a norm to undo (12000 x 1280 bf16: 512 chunks 88 us, 1024 71 us; fp32 768
-    // 92 us instead of 101 us), if that leaves eight rows to each (2048 x 2048 fp32: 512 chunks 29 us, 1024 33 us)
+    if (d->dim <= 256 || (d->dim > 512 && d->dim <= 1024)) return 1024;
+    // Two pieces to a thread: four of a compute unit, or three with a gate and a norm to undo (12000 x 1280 bf16: 512 chunks 88
+    // us, 1024 71 us; fp32 768 92 us instead of 101 us; 20000 x 300 fp32 1024 chunks 52 us, 512 45 us), if that leaves eight
+    // turns to each (2048 x 2048 fp32: 512 chunks 29 us, 1024 33 us).
     const bool three = gated && normed && (!narrow || d->dim % 4 != 0);
+    if (d->dim <= 512 && !three) return 1024;
     const long long most = three ? 768 : 1024;
-    return d->rows >= 8 * most ? most : 512;
+    return d->rows >= 8 * most * block_norm_backward_groups(d->dim) ? most : 512;
 }
 BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     BlockNormPlan b{};
@@ -209,7 +211,9 @@ BlockNormPlan block_norm_plan(const snhip_block_norm_desc* d) {
     const int at_once = block_norm_backward_groups(d->dim);
     const long long wanted = block_norm_chunks(d);
     long long c = (d->rows + wanted - 1) / wanted;
-    if (c < at_once) c = at_once;
+    // (a turn each would give the column sums more to do than the rows: 1024 x 1024 bf16 13.2 us, two turns 11.8)
+    const int least = d->rows > 512LL * at_once ? 2 * at_once : at_once;
+    if (c < least) c = least;
     b.flush = gate_rows && b.rows_per_group <= c;
     if (b.flush) {
         b.groups_per_chunk = (int)((c / b.rows_per_group + at_once - 1) / at_once * at_once);
