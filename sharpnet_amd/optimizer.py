@@ -38,7 +38,8 @@ class AdamW:
             self._check_states(p, s)
         # the plan holds addresses: everything it points at stays alive with it
         self.Parameters, self.Gradients, self.States, self.Copies = list(parameters), list(gradients), [list(s) for s in states], list(copies)
-        self._held = [t for tensors in zip(self.Parameters, self.Gradients, self.Copies, *zip(*self.States)) for t in tensors if t is not None]
+        memory = (t._owner or t for tensors in zip(self.Parameters, self.Gradients, self.Copies, *zip(*self.States)) for t in tensors if t is not None)
+        self._memory = list({id(t): t for t in memory}.values())
         if not count:
             return
         self._lib, self._wrapper = parameters[0]._lib, parameters[0].Wrapper
@@ -77,9 +78,9 @@ class AdamW:
         """One step with the gradients as they are, times gradientScale (1 / loss scale, or a clipping factor)."""
         if self._disposed:
             raise RuntimeError("AdamW is disposed")
-        for t in self._held:
+        for t in self._memory:
             if t._disposed:
-                raise RuntimeError("a tensor of the optimizer is disposed")
+                raise RuntimeError("memory of the optimizer's tensors is disposed")
         if learningRate is not None:
             self.LearningRate = learningRate
         if self._plan is not None:

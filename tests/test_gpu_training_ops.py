@@ -512,6 +512,24 @@ def test_adamw_gradients_that_are_not_finite_or_at_the_ends_of_the_range(gpu_wra
         p = got
 
 
+def test_adamw_of_memory_that_has_gone(gpu_wrapper):
+    """Parameters that are parts of one buffer: the step is refused once the buffer is disposed, not for a view of it."""
+    from sharpnet_amd import optimizer
+    w = gpu_wrapper
+    whole, grads = tensor(w, np.ones(300)), tensor(w, np.ones(300))
+    views = [whole.Slice(0, [100]), whole.Slice(100, [10, 20])]
+    opt = optimizer.AdamW(views, [grads.Slice(0, [100]), grads.Slice(100, [10, 20])])
+    opt.Step()
+    views[0].Dispose()
+    opt.Step()
+    before = whole.ToNumpy().copy()
+    assert np.all(before[:300] < 1)
+    whole.Dispose()
+    with pytest.raises(RuntimeError):
+        opt.Step()
+    assert opt.StepCount == 2
+
+
 def test_adamw_8_bit_states_follow_a_slow_mean(gpu_wrapper):
     """beta2 = 0.999 moves v by a thousandth of its distance a step, a hundredth of a step of e5m2.  From v = 0 and gradients
     of 1 the mean of v over n elements is 1 - 0.999^t; rounding at random keeps it: the rounding of a step moves an element

@@ -273,6 +273,33 @@ def test_entry_points_that_compute_with_float32_refuse_other_types():
     assert f.FloatPointer == f.Pointer == A
 
 
+def test_one_layer_called_by_two_threads():
+    """Every call's descriptor is its own, whatever another thread asks of the layer meanwhile."""
+    import threading
+    import time
+    from sharpnet_amd import embedding, normalization
+    e, n, wrong = embedding.WordEmbedding(7, 6), normalization.BlockNorm(6, "rms"), []
+
+    def run(rows):
+        def check(handle, d, *args):
+            time.sleep(1e-4)
+            got = d._obj.tokens if isinstance(d._obj, hiplib.EmbeddingDesc) else d._obj.rows
+            if got != rows:
+                wrong.append((got, rows))
+            return 0
+        y, ids, table = Stub((rows, 6)), Stub((rows,), "int32"), Stub((7, 6))
+        y.snhip_embedding_forward = y.snhip_block_norm_forward = check
+        for _ in range(100):
+            e.ForwardPropagation(y, ids, table)
+            n.ForwardPropagation(y, Stub((rows, 6)))
+    threads = [threading.Thread(target=run, args=(rows,)) for rows in (3, 4, 5)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_workspace_of_a_layer():
     """One for each wrapper; a longer one leaves the one before in place until Dispose."""
     from sharpnet_amd.gpu_tensor import LayerWorkspace
@@ -309,7 +336,7 @@ def test_adamw_after_its_end():
         opt.Step()
     assert opt.StepCount == 1
     opt = optimizer.AdamW.__new__(optimizer.AdamW)
-    opt._disposed, opt._plan, opt._held, opt.StepCount = False, None, tensors, 3
+    opt._disposed, opt._plan, opt._memory, opt.StepCount = False, None, tensors, 3
     tensors[2]._disposed = True
     with pytest.raises(RuntimeError):
         opt.Step()
