@@ -37,64 +37,66 @@ class BlockNorm:
         self._workspace = LayerWorkspace()
         self._mine = threading.local()  # a descriptor for each thread and direction; a call fills in what is not the layer's kind
 
-    def _rows(self, t, name, shape, type_):
-        """t is None or has rows like those of shape, in the given type."""
+    def _rows(self, w, t, name, shape, type_):
+        """The address of t, which is None or has rows like those of shape, in the given type, on the wrapper's device."""
         if t is None:
-            return
+            return None
         if t.Shape != shape and (t.Shape[-1] != self.EmbeddingDim or math.prod(t.Shape) != math.prod(shape)):
             raise ValueError("%s is %s, expected the rows of %s" % (name, t.Shape, shape))
         if t.Type != type_:
             raise ValueError("%s is %s, expected %s" % (name, t.Type, type_))
+        return pointer_on(w, t)
 
-    def _vector(self, t, name):
-        if t is not None and (t.Type != "float32" or (t.Shape != self._vectorShape and math.prod(t.Shape) != self.EmbeddingDim)):
+    def _vector(self, w, t, name):
+        if t is None:
+            return None
+        if t.Type != "float32" or (t.Shape != self._vectorShape and math.prod(t.Shape) != self.EmbeddingDim):
             raise ValueError("%s is %s %s, expected %d float32" % (name, t.Type, t.Shape, self.EmbeddingDim))
+        return pointer_on(w, t)
+
+    def _statistics(self, w, t, name, rows):
+        if t is None:
+            return None
+        if t.Type != "float32" or math.prod(t.Shape) != 2 * rows:
+            raise ValueError("%s is %s %s, expected (%d, 2) float32" % (name, t.Type, t.Shape, rows))
+        return pointer_on(w, t)
 
     def _desc(self, direction, stream, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
         """What both directions have: the layer itself, sizes and types, gate, weights, statistics."""
-        if self.EmbeddingDim <= 0 or stream.Shape[-1] != self.EmbeddingDim:
-            raise ValueError("rows of %s do not fit an embedding dimension of %d" % (stream.Shape, self.EmbeddingDim))
-        if stream.Type not in _ROW_TYPES or block.Type not in _ROW_TYPES:
-            raise ValueError("rows must be float32 or bfloat16, not %s and %s" % (stream.Type, block.Type))
-        rows = math.prod(stream.Shape) // self.EmbeddingDim
-        self._vector(preWeight, "preWeight")
-        self._vector(preBias, "preBias")
-        self._vector(postWeight, "postWeight")
-        self._vector(postBias, "postBias")
-        for t, name in ((preStatistics, "preStatistics"), (postStatistics, "postStatistics")):
-            if t is not None and (math.prod(t.Shape) != 2 * rows or t.Type != "float32"):
-                raise ValueError("%s is %s %s, expected (%d, 2) float32" % (name, t.Type, t.Shape, rows))
+        w, dim, stream_type, block_type = stream.Wrapper, self.EmbeddingDim, stream.Type, block.Type
+        if dim <= 0 or stream.Shape[-1] != dim:
+            raise ValueError("rows of %s do not fit an embedding dimension of %d" % (stream.Shape, dim))
+        if stream_type not in _ROW_TYPES or block_type not in _ROW_TYPES:
+            raise ValueError("rows must be float32 or bfloat16, not %s and %s" % (stream_type, block_type))
         if gateRows < 0:
             raise ValueError("gateRows is %d" % gateRows)
-        if gate is not None:
-            if gateRows == 0:
-                self._vector(gate, "gate")
-            else:
-                self._rows(gate, "gate", [-(-rows // gateRows), self.EmbeddingDim], block.Type)
-        w, mine = stream.Wrapper, self._mine.__dict__
+        rows, mine = math.prod(stream.Shape) // dim, self._mine.__dict__
         d = mine.get(direction)
         if d is None:
-            d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation,
-                                                dim=self.EmbeddingDim)
+            d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=dim)
         d.epsilon, d.residual_scale = self.Epsilon, self.ResidualScale
         d.rows, d.gate_rows = rows, gateRows
-        d.stream_type, d.block_type = _ROW_TYPES[stream.Type], _ROW_TYPES[block.Type]
-        d.gate, d.pre_weight, d.pre_bias = pointer_on(w, gate), pointer_on(w, preWeight), pointer_on(w, preBias)
-        d.post_weight, d.post_bias = pointer_on(w, postWeight), pointer_on(w, postBias)
-        d.pre_statistics, d.post_statistics = pointer_on(w, preStatistics), pointer_on(w, postStatistics)
+        d.stream_type, d.block_type = _ROW_TYPES[stream_type], _ROW_TYPES[block_type]
+        d.pre_weight, d.pre_bias = self._vector(w, preWeight, "preWeight"), self._vector(w, preBias, "preBias")
+        d.post_weight, d.post_bias = self._vector(w, postWeight, "postWeight"), self._vector(w, postBias, "postBias")
+        d.pre_statistics = self._statistics(w, preStatistics, "preStatistics", rows)
+        d.post_statistics = self._statistics(w, postStatistics, "postStatistics", rows)
+        if gateRows == 0:
+            d.gate = self._vector(w, gate, "gate")
+        else:
+            d.gate = self._rows(w, gate, "gate", [-(-rows // gateRows), dim], block_type)
         return d
 
     def ForwardPropagation(self, x, h, y=None, u=None, gate=None, gateRows=0, preWeight=None, preBias=None, postWeight=None,
                            postBias=None, preStatistics=None, postStatistics=None):
         """h and u from x and y; h is None for a join without a norm ahead of the next block, y and u for a norm without a
         block.  gateRows: rows that share a row of the gate (0: the gate is one vector)."""
-        shape, w = x.Shape, x.Wrapper
+        shape, w, stream_type = x.Shape, x.Wrapper, x.Type
         block = h if h is not None else y if y is not None else x
+        block_type = block.Type
         d = self._desc("forward", x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
-        self._rows(y, "y", shape, block.Type)
-        self._rows(h, "h", shape, block.Type)
-        self._rows(u, "u", shape, x.Type)
-        d.x, d.y, d.u, d.h = pointer_on(w, x), pointer_on(w, y), pointer_on(w, u), pointer_on(w, h)
+        d.x, d.u = pointer_on(w, x), self._rows(w, u, "u", shape, stream_type)
+        d.y, d.h = self._rows(w, y, "y", shape, block_type), self._rows(w, h, "h", shape, block_type)
         check_status(x._lib.snhip_block_norm_forward(w.handle, ctypes.byref(d)), "snhip_block_norm_forward")
 
     def BackwardPropagation(self, dx, u, dh, du=None, y=None, dy=None, gate=None, dGate=None, gateRows=0, preWeight=None,
@@ -103,26 +105,30 @@ class BlockNorm:
         """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics; gradients that are
         None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
-        shape, w = dx.Shape, dx.Wrapper
-        block = next((t for t in (dh, y, dy) if t is not None), dx)
+        shape, w, lib, stream_type = dx.Shape, dx.Wrapper, dx._lib, dx.Type
+        block = dh if dh is not None else y if y is not None else dy if dy is not None else dx
+        block_type = block.Type
         d = self._desc("backward", dx, block, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
-        for t, name in ((y, "y"), (dh, "dh"), (dy, "dy")):
-            self._rows(t, name, shape, block.Type)
-        for t, name in ((u, "u"), (du, "du")):
-            self._rows(t, name, shape, dx.Type)
-        for t, name in ((dPreWeight, "dPreWeight"), (dPreBias, "dPreBias"), (dPostWeight, "dPostWeight"), (dPostBias, "dPostBias")):
-            self._vector(t, name)
+        d.dx, d.u, d.du = pointer_on(w, dx), self._rows(w, u, "u", shape, stream_type), self._rows(w, du, "du", shape, stream_type)
+        d.dh, d.y = self._rows(w, dh, "dh", shape, block_type), self._rows(w, y, "y", shape, block_type)
+        d.dy = self._rows(w, dy, "dy", shape, block_type)
         if dGate is not None and (gate is None or dGate.Shape != gate.Shape or dGate.Type != gate.Type):
             raise ValueError("dGate must have the gate's shape and type")
-        d.y, d.u, d.dx, d.dh, d.du, d.dy = (pointer_on(w, t) for t in (y, u, dx, dh, du, dy))
-        d.d_gate, d.d_pre_weight, d.d_pre_bias = pointer_on(w, dGate), pointer_on(w, dPreWeight), pointer_on(w, dPreBias)
-        d.d_post_weight, d.d_post_bias = pointer_on(w, dPostWeight), pointer_on(w, dPostBias)
+        d.d_gate = pointer_on(w, dGate)
+        d.d_pre_weight, d.d_pre_bias = self._vector(w, dPreWeight, "dPreWeight"), self._vector(w, dPreBias, "dPreBias")
+        d.d_post_weight, d.d_post_bias = self._vector(w, dPostWeight, "dPostWeight"), self._vector(w, dPostBias, "dPostBias")
         d.accumulate = 1 if accumulate else 0
-        need, lib = ctypes.c_size_t(), dx._lib
-        check_status(lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
-                     "snhip_block_norm_backward_workspace_size")
         if workspace is None:
-            workspace = self._workspace.Get(w, need.value)
+            # what its size depends on
+            call = (shape, stream_type, block_type, gateRows, dh is None, gate is None, dGate is None, dPreWeight is None,
+                    dPreBias is None, dPostWeight is None, dPostBias is None)
+            mine = self._mine.__dict__
+            if mine.get("call") != call:
+                need = ctypes.c_size_t()
+                check_status(lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
+                             "snhip_block_norm_backward_workspace_size")
+                mine["call"], mine["need"] = (list(shape),) + call[1:], need.value
+            workspace = self._workspace.Get(w, mine["need"])
         nbytes = workspace.Count * workspace.ElementBytes if workspace is not None else 0
         check_status(lib.snhip_block_norm_backward(w.handle, ctypes.byref(d), pointer_on(w, workspace), nbytes),
                      "snhip_block_norm_backward")
