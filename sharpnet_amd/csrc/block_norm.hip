@@ -40,10 +40,12 @@ template <int TPR, int N, int MODE, bool BIAS, bool GATE>
 void backward(const BlockNormParams& p, hipStream_t stream) {
     constexpr int NT = TPR > 256 ? TPR : 256;
     const dim3 grid((unsigned)p.chunks);
-    if (p.exact)
-        hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, true>), grid, dim3(NT), 0, stream, p);
-    else
-        hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, false>), grid, dim3(NT), 0, stream, p);
+    if constexpr (TPR != 256 || N != 1)  // (those are rows of another width than a multiple of four)
+        if (p.exact) {
+            hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, true>), grid, dim3(NT), 0, stream, p);
+            return;
+        }
+    hipLaunchKernelGGL((block_norm_backward_kernel<Stream, Block, TPR, N, MODE, BIAS, GATE, false>), grid, dim3(NT), 0, stream, p);
 }
 
 template <int TPR, int N>
@@ -90,14 +92,18 @@ void SNHIP_FORWARD(const BlockNormParams& p, hipStream_t stream) {
     forward<256, 8>(p, stream);
 }
 
-// One or two pieces to a thread: more took registers that the column sums need.  (32 threads to rows of up to 128: 30000 x 128
-// bf16 21 us, with 16 and two pieces 26.  The groups of threads per workgroup: block_norm_backward_groups.)
+// A row of up to 1024 elements is one wavefront's or less, as above (32 threads to rows of up to 128: 30000 x 128 bf16 19 us, with 16
+// and two pieces 23; 16384 x 768 with three pieces 46 us, with 256 threads to a row 57; 16384 x 1024 55 and 60 us), but not with
+// four pieces and ends to look at, which take too many registers (8000 x 1001 fp32: 78 us, 256 threads 59).  Beyond that two
+// pieces to a thread leave registers for the column sums.  (The groups of threads per workgroup: block_norm_backward_groups.)
 void SNHIP_BACKWARD(const BlockNormParams& p, BlockNormKind kind, hipStream_t stream) {
     const int units = (p.dim + 3) / 4;
     if (units <= 16) return backward_kind<16, 1>(p, kind, stream);
     if (units <= 32) return backward_kind<32, 1>(p, kind, stream);
     if (units <= 64) return backward_kind<64, 1>(p, kind, stream);
     if (units <= 128) return backward_kind<64, 2>(p, kind, stream);
+    if (units <= 192) return backward_kind<64, 3>(p, kind, stream);
+    if (units <= 256 && p.dim % 4 == 0) return backward_kind<64, 4>(p, kind, stream);
     if (units <= 256) return backward_kind<256, 1>(p, kind, stream);
     if (units <= 512) return backward_kind<256, 2>(p, kind, stream);
     if (units <= 1024) return backward_kind<512, 2>(p, kind, stream);

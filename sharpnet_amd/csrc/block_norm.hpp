@@ -316,7 +316,8 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
     constexpr bool HAS_Y = MODE == 2 || GATE, BOTH = N == 1;
     __shared__ float lds[2][2][TPR / 64 + 1];
     constexpr int VECTORS = 1 + (BIAS ? 1 : 0) + (MODE == 2 ? 1 + (BIAS ? 1 : 0) : 0) + (GATE ? 1 : 0);  // of column sums
-    __shared__ f32x4 meet[GROUPS > 1 ? VECTORS * GROUPS * TPR * N : 1];
+    constexpr bool TOGETHER = VECTORS * GROUPS * TPR * N * sizeof(f32x4) <= 48 << 10;  // in LDS (2000 x 64: 7.4 us, one by one 9.0)
+    __shared__ f32x4 meet[GROUPS > 1 ? (TOGETHER ? VECTORS : 1) * GROUPS * TPR * N : 1];
     int turn = 0;
     const int lane = threadIdx.x % TPR, group = row_group<TPR>(), dim = p.dim;
     constexpr f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -473,24 +474,36 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
     };
     if constexpr (GROUPS > 1) {
         constexpr int PIECES = TPR * N;
-        int v = 0;
-        every([&](const f32x4* acc, int) {
+        auto put = [&](const f32x4* acc, int v) {
 #pragma unroll
             for (int n = 0; n < N; ++n) meet[(v * GROUPS + group) * PIECES + n * TPR + lane] = acc[n];
-            ++v;
-        });
-        __syncthreads();
-        for (int k = threadIdx.x; k < VECTORS * PIECES; k += NT) {
-            const int piece = k % PIECES, vector = k / PIECES;
-            int slot = -1, at = 0;
-            every([&](const f32x4*, int s) {
-                if (at == vector) slot = p.slot[s];
-                ++at;
+        };
+        auto add_up = [&](int v, int piece, int slot) {
+            f32x4 sum = meet[v * GROUPS * PIECES + piece];
+            for (int g = 1; g < GROUPS; ++g) sum += meet[(v * GROUPS + g) * PIECES + piece];
+            store4(p.partial + ((long long)slot * p.chunks + chunk) * dim + 4 * piece, dim - 4 * piece, sum);
+        };
+        if constexpr (TOGETHER) {
+            int v = 0;
+            every([&](const f32x4* acc, int) { put(acc, v++); });
+            __syncthreads();
+            for (int k = threadIdx.x; k < VECTORS * PIECES; k += NT) {
+                const int piece = k % PIECES, vector = k / PIECES;
+                int slot = -1, at = 0;
+                every([&](const f32x4*, int s) {
+                    if (at == vector) slot = p.slot[s];
+                    ++at;
+                });
+                if (slot >= 0) add_up(vector, piece, slot);
+            }
+        } else {
+            every([&](const f32x4* acc, int s) {
+                if (p.slot[s] < 0) return;
+                __syncthreads();
+                put(acc, 0);
+                __syncthreads();
+                for (int piece = threadIdx.x; piece < PIECES; piece += NT) add_up(0, piece, p.slot[s]);
             });
-            if (slot < 0) continue;
-            f32x4 s = meet[vector * GROUPS * PIECES + piece];
-            for (int g = 1; g < GROUPS; ++g) s += meet[(vector * GROUPS + g) * PIECES + piece];
-            store4(p.partial + ((long long)slot * p.chunks + chunk) * dim + 4 * piece, dim - 4 * piece, s);
         }
     } else {
         every([&](const f32x4* acc, int s) {

@@ -10,7 +10,7 @@ namespace snhip {
 constexpr int kBlockNormMaxDim = 8192;
 
 // Rows that a workgroup of the backward kernel holds at a time.
-inline int block_norm_backward_groups(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 8 : dim <= 512 ? 4 : 1; }
+inline int block_norm_backward_groups(int dim) { return dim <= 64 ? 16 : dim <= 128 ? 8 : dim <= 768 || (dim <= 1024 && dim % 4 == 0) ? 4 : 1; }
 
 // mode, bias, gate: the template parameters of block_norm_backward_kernel
 struct BlockNormKind {

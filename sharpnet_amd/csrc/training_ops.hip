@@ -193,7 +193,8 @@ long long block_norm_chunks(const snhip_block_norm_desc* d) {
     // alone 6000 x 5120 71 us and 79 us)
     if (d->dim > 4096) return gated || normed || !narrow ? 256 : 512;
     if (d->dim > 2048) return 512;
-    if (d->dim <= 256 || (d->dim > 512 && d->dim <= 1024)) return 1024;
+    if (d->dim <= 256) return 1024;
+    if (d->dim > 512 && d->dim <= 1024) return block_norm_backward_groups(d->dim) > 1 ? 512 : 1024;
     // Two pieces to a thread: four of a compute unit, or three with a gate and a norm to undo (12000 x 1280 bf16: 512 chunks 88
     // us, 1024 71 us; fp32 768 92 us instead of 101 us; 20000 x 300 fp32 1024 chunks 52 us, 512 45 us), if that leaves eight
     // turns to each (2048 x 2048 fp32: 512 chunks 29 us, 1024 33 us).

@@ -207,7 +207,9 @@ NORMS = [(1, 1, "layer", None, None, None, True, "float32", "float32"),
          (4200, 700, "layer", "rms", 0, None, False, "bfloat16", "bfloat16"), (4150, 1023, "rms", "layer", 9, "sigmoid", True, "float32", "float32"),
          (600, 2600, "layer", "layer", 0, None, False, "float32", "bfloat16"), (550, 5001, "rms", None, 1, "tanh", True, "bfloat16", "bfloat16"),
          (520, 6140, "layer", "rms", None, None, False, "float32", "float32"), (6200, 1028, "rms", "layer", 0, "sigmoid", False, "float32", "bfloat16"),
-         (8195, 1032, "layer", None, 4, None, True, "bfloat16", "bfloat16")]
+         (8195, 1032, "layer", None, 4, None, True, "bfloat16", "bfloat16"),
+         (900, 900, "layer", "layer", 1, "sigmoid", True, "float32", "float32"), (801, 640, "layer", "layer", 0, "tanh", True, "float32", "bfloat16"),
+         (2050, 1024, "rms", "layer", 700, "tanh", True, "bfloat16", "bfloat16"), (5, 770, "rms", None, None, None, False, "float32", "bfloat16")]
 
 
 def norm_case(rng, rows, dim, pre, post, gate_rows, bias, stream, block):
@@ -377,7 +379,7 @@ def rows_of(t, rows, dim, ld, offset, fill=3.0):
     return got[:, :dim]
 
 
-@pytest.mark.parametrize("dim,ld,offset", [(12, 20, 0), (12, 20, 4), (12, 21, 0), (12, 20, 1), (300, 301, 3), (1500, 1504, 4)])
+@pytest.mark.parametrize("dim,ld,offset", [(12, 20, 0), (12, 20, 4), (12, 21, 0), (12, 20, 1), (300, 301, 3), (1500, 1504, 4), (900, 903, 1), (700, 702, 3)])
 def test_block_norm_rows_with_pitches_and_any_alignment(gpu_wrapper, dim, ld, offset):
     from sharpnet_amd.hiplib import ACT_SIGMOID, BlockNormDesc, NORM_LAYER, NORM_RMS, TYPES, check_status
     w, rng = gpu_wrapper, np.random.default_rng(ld)
