@@ -61,6 +61,9 @@ int snhip_get_workspace_size(void* handle, size_t* bytes);
  * GEMMs run on the legacy default stream); offered for callers with their own
  * hipStream_t.  stream == NULL selects the null stream again. */
 int snhip_set_stream(void* handle, void* stream);
+/* The stream that snhip_set_stream selected (NULL: the null stream), for callers whose scratch memory goes by it: calls before
+ * and after a change of streams are not ordered. */
+int snhip_get_stream(void* handle, void** stream);
 /* Replaces cublasGetVersion_v2 (CublasWrapper.cs:250): major*10000+minor*100+patch. */
 int snhip_get_version(void* handle, int* version);
 
@@ -580,7 +583,7 @@ int snhip_transpose_second_and_third_dimension(void* handle, const float* src, f
 /* Replace the nvcuda calls GPUTensor makes: cuMemAlloc_v2 (GpuTensor.cs:41),
  * cuMemFree_v2 (:1634), cuMemsetD32 (:1583), cuMemcpyHtoDAsync (:77),
  * cuMemcpyDtoH (:1668), cuMemcpyDtoDAsync (:1499), cuStreamSynchronize
- * (Prod/GPU/StreamWrapper.cs:20). */
+ * (Prod/GPU/StreamWrapper.cs:20).  snhip_malloc may be called while a stream is captured. */
 int snhip_malloc(void** dptr, size_t bytes);
 int snhip_free(void* dptr);
 int snhip_memset32(void* handle, void* dptr, unsigned int value, size_t count);

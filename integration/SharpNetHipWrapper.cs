@@ -11,6 +11,7 @@ namespace SharpNet.GPU
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_create(ref IntPtr handle);
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_destroy(IntPtr handle);
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_set_stream(IntPtr handle, IntPtr stream);
+        [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_get_stream(IntPtr handle, out IntPtr stream);
         [DllImport(DLL_NAME)] public static extern cublasStatus_t snhip_get_version(IntPtr handle, out int version);
 
         [DllImport(DLL_NAME)]

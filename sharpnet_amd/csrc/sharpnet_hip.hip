@@ -1316,6 +1316,13 @@ int snhip_set_stream(void* handle, void* stream) {
     return SNHIP_STATUS_SUCCESS;
 }
 
+int snhip_get_stream(void* handle, void** stream) {
+    if (handle == nullptr) return SNHIP_STATUS_NOT_INITIALIZED;
+    if (stream == nullptr) return SNHIP_STATUS_INVALID_VALUE;
+    *stream = static_cast<Handle*>(handle)->stream;
+    return SNHIP_STATUS_SUCCESS;
+}
+
 int snhip_get_version(void* handle, int* version) {
     (void)handle;
     if (version == nullptr) return SNHIP_STATUS_INVALID_VALUE;
@@ -1970,7 +1977,11 @@ int snhip_malloc(void** dptr, size_t bytes) {
     if (dptr == nullptr) return SNHIP_STATUS_INVALID_VALUE;
     *dptr = nullptr;
     if (bytes < 8) bytes = 8;  // GPUTensor never allocates less (GpuTensor.cs:38)
+    // an allocation has no place in a graph and disturbs none: allowed while a stream is captured
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
     hipError_t e = hipMalloc(dptr, bytes);
+    (void)hipThreadExchangeStreamCaptureMode(&mode);
     if (e != hipSuccess) {
         (void)hipGetLastError();
         return SNHIP_STATUS_ALLOC_FAILED;

@@ -9,7 +9,7 @@ import ctypes
 import math
 import threading
 
-from .gpu_tensor import LayerWorkspace, pointer_on
+from .gpu_tensor import LayerWorkspace, pointer_on, stream_of
 from .hiplib import EmbeddingDesc, TYPES, check_status
 
 _ID_TYPES = {k: TYPES[k] for k in ("float32", "int32", "int64")}
@@ -66,8 +66,8 @@ class WordEmbedding:
 
     def BackwardPropagation(self, dWordEmbedding, x, dy, accumulate=False, workspace=None):
         """dWordEmbedding (float32) = the table's gradient, or += it with ``accumulate``.  Without a ``workspace`` the layer
-        keeps one of its own for each wrapper, which grows when a longer batch comes (an allocation: size it with a first call
-        before a stream capture).  It is one call's at a time: two captured graphs whose replays may overlap get one each."""
+        keeps one of its own for each wrapper and stream that it is called on, which grows when a longer batch comes.  It is one
+        call's at a time: graphs whose replays may overlap one another, or calls on the stream they were captured on, get one each."""
         self._check_table(dWordEmbedding)
         if dWordEmbedding.Type != "float32":
             raise ValueError("the table's gradient must be float32, not %s" % dWordEmbedding.Type)
@@ -75,8 +75,8 @@ class WordEmbedding:
         pointers = pointer_on(w, x), pointer_on(w, dy), pointer_on(w, dWordEmbedding)
         check_status(dy._lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                      "snhip_embedding_backward_workspace_size")
-        if workspace is None:
-            workspace = self._workspace.Get(w, need.value)
+        if workspace is None and need.value > 0:
+            workspace = self._workspace.Get(w, need.value, stream_of(w))
         check_status(dy._lib.snhip_embedding_backward(w.handle, ctypes.byref(d), *pointers, int(bool(accumulate)),
                                                       pointer_on(w, workspace),
                                                       workspace.Count * workspace.ElementBytes if workspace is not None else 0),

@@ -408,18 +408,25 @@ class GPUTensor:
 
 
 # -- element-wise / row helpers next to the GEMMs (same names as the reference's Tensor methods) -----------------
+def stream_of(wrapper):
+    """The address of the stream that the wrapper's calls go to (0: the null stream)."""
+    stream = ctypes.c_void_p()
+    check_status(wrapper.lib.snhip_get_stream(wrapper.handle, ctypes.byref(stream)), "snhip_get_stream")
+    return stream.value or 0
+
+
 class LayerWorkspace:
-    """Scratch memory of a layer, one buffer for each wrapper (device and stream) that it is used on.  A longer call gets a
-    longer buffer; the one before stays until Dispose, since a captured graph may still write to it."""
+    """Scratch memory of a layer, one buffer for each wrapper and stream (stream_of) that it is used on: calls on two streams may
+    overlap.  A longer call gets a longer buffer; the one before stays until Dispose, since a captured graph may still write to it."""
 
     def __init__(self):
         self._held = {}
 
-    def Get(self, wrapper, nbytes):
+    def Get(self, wrapper, nbytes, stream=0):
         """A uint8 tensor of at least nbytes, or None for none."""
         if nbytes == 0:
             return None
-        held = self._held.setdefault(wrapper, [])
+        held = self._held.setdefault((wrapper, stream), [])
         if not held or held[-1].Shape[0] < nbytes:
             size = max(nbytes, held[-1].Shape[0] * 3 // 2) if held else nbytes  # (all together: at most three times the last)
             held.append(GPUTensor([size], None, wrapper, element_type="uint8"))

@@ -220,6 +220,7 @@ SIGNATURES = {
     "snhip_create": [_vpp],
     "snhip_destroy": [_vp],
     "snhip_set_stream": [_vp, _vp],
+    "snhip_get_stream": [_vp, _vpp],
     "snhip_reserve_workspace": [_vp, _sz],
     "snhip_get_workspace_size": [_vp, ctypes.POINTER(_sz)],
     "snhip_get_version": [_vp, _c_int_p],

@@ -9,7 +9,7 @@ import ctypes
 import math
 import threading
 
-from .gpu_tensor import LayerWorkspace, pointer_on
+from .gpu_tensor import LayerWorkspace, pointer_on, stream_of
 from .hiplib import (ACT_NONE, ACT_SIGMOID, ACT_TANH, BlockNormDesc, NORM_LAYER, NORM_NONE, NORM_RMS, SharpNetHipError, CublasStatus,
                      TYPES, check_status)
 
@@ -128,7 +128,7 @@ class BlockNorm:
                 check_status(lib.snhip_block_norm_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
                              "snhip_block_norm_backward_workspace_size")
                 mine["call"], mine["need"] = (list(shape),) + call[1:], need.value
-            workspace = self._workspace.Get(w, mine["need"])
+            workspace = self._workspace.Get(w, mine["need"], stream_of(w)) if mine["need"] > 0 else None
         nbytes = workspace.Count * workspace.ElementBytes if workspace is not None else 0
         check_status(lib.snhip_block_norm_backward(w.handle, ctypes.byref(d), pointer_on(w, workspace), nbytes),
                      "snhip_block_norm_backward")

@@ -752,6 +752,79 @@ def test_scratch_memory_that_has_grown_after_a_capture(gpu_wrapper):
         layer.Dispose()
 
 
+def test_one_layer_on_two_streams_of_a_handle(gpu_wrapper):
+    """Gradients of a long and a short batch in turn on two streams of one handle, without waiting: each stream's calls have
+    scratch memory of their own (the sums of a call do not depend on the other's).  Then the same under a capture on a stream
+    that the layers have not been used on, replayed beside eager calls."""
+    from sharpnet_amd import embedding, normalization
+    from sharpnet_amd.hiplib import check_status
+    w, rng = gpu_wrapper, np.random.default_rng(12)
+    hip, vp = hip_runtime(), ctypes.c_void_p
+    vocabulary, dim = 3000, 64
+    e, n = embedding.WordEmbedding(vocabulary, dim), normalization.BlockNorm(dim, "rms")
+
+    def job(tokens):
+        x, dy = tensor(w, make_ids(rng, tokens, vocabulary, "int32"), "int32"), tensor(w, rng.normal(0, 1, (tokens, dim)))
+        s = tensor(w, np.concatenate(ref.statistics(dy.ToNumpy(), "rms", 1e-5), 1))
+        dW, dx, dw = empty(w, (vocabulary, dim)), empty(w, (tokens, dim)), empty(w, (dim,))
+
+        def work():
+            e.BackwardPropagation(dW, x, dy)
+            n.BackwardPropagation(dx, dy, dy, preStatistics=s, dPreWeight=dw)
+        return work, (dW, dx, dw)
+    jobs = [job(40000), job(9000)]
+    want = []
+    for work, outs in jobs:
+        work()
+        want.append([t.ToNumpy().copy() for t in outs])
+
+    def check():
+        for (_, outs), expected in zip(jobs, want):
+            for t, value in zip(outs, expected):
+                assert np.array_equal(t.ToNumpy(), value)
+                t.SetValue(float("nan"))
+        w.synchronize()
+    streams, graph, graph_exec = [vp(), vp(), vp()], vp(), vp()
+    for s in streams:
+        check_status(w.lib.snhip_stream_create(ctypes.byref(s)), "snhip_stream_create")
+    try:
+        for _ in range(4):
+            for _ in range(5):
+                for (work, _), s in zip(jobs, streams):
+                    check_status(w.lib.snhip_set_stream(w.handle, s), "snhip_set_stream")
+                    work()
+            for s in streams[:2]:
+                check_status(w.lib.snhip_set_stream(w.handle, s), "snhip_set_stream")
+                w.synchronize()
+            check()
+        check_status(w.lib.snhip_set_stream(w.handle, streams[2]), "snhip_set_stream")
+        assert hip.hipStreamBeginCapture(streams[2], 0) == 0
+        try:
+            jobs[0][0]()
+        finally:
+            assert hip.hipStreamEndCapture(streams[2], ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(graph_exec), graph, None, None, 0) == 0
+        for _ in range(4):
+            check_status(w.lib.snhip_set_stream(w.handle, streams[1]), "snhip_set_stream")
+            for _ in range(3):
+                jobs[1][0]()
+                assert hip.hipGraphLaunch(graph_exec, streams[2]) == 0
+            for s in streams[1:]:
+                check_status(w.lib.snhip_set_stream(w.handle, s), "snhip_set_stream")
+                w.synchronize()
+            check()
+    finally:
+        check_status(w.lib.snhip_set_stream(w.handle, None), "snhip_set_stream")
+        if graph_exec:
+            hip.hipGraphExecDestroy(graph_exec)
+        if graph:
+            hip.hipGraphDestroy(graph)
+        for s in streams:
+            check_status(w.lib.snhip_stream_destroy(s), "snhip_stream_destroy")
+        e.Dispose()
+        n.Dispose()
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # together, as a training step uses them
 # ---------------------------------------------------------------------------------------------------------------

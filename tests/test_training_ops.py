@@ -325,6 +325,59 @@ def test_workspace_of_a_layer():
     assert first._disposed and second._disposed and not a.live and not b.live
 
 
+def test_scratch_memory_goes_by_stream(lib, handle):
+    """Calls on two streams of one handle may overlap: each has its own scratch memory, the same one when it comes again."""
+    from sharpnet_amd import embedding, normalization
+    stream, allocated, given = [0], [], []
+
+    class Wrapper:
+        lib, device_id, handle = None, 0, None
+
+        def allocate(self, nbytes):
+            allocated.append(nbytes)
+            return A + (len(allocated) << 24)
+
+        def release(self, pointer, nbytes):
+            pass
+
+        def snhip_get_stream(self, handle, out):
+            out._obj.value = stream[0]
+            return 0
+
+        def snhip_embedding_backward_workspace_size(self, desc, out):
+            return lib.snhip_embedding_backward_workspace_size(desc, out)
+
+        def snhip_block_norm_backward_workspace_size(self, desc, out):
+            return lib.snhip_block_norm_backward_workspace_size(desc, out)
+
+        def snhip_embedding_backward(self, handle, desc, ids, dy, table, accumulate, workspace, nbytes):
+            given.append(workspace)
+            return 0
+
+        def snhip_block_norm_backward(self, handle, desc, workspace, nbytes):
+            given.append(workspace)
+            return 0
+    w = Wrapper()
+    w.lib = w
+
+    def on(shape, type_="float32"):
+        t = Stub(shape, type_)
+        t.Wrapper = t._lib = w
+        return t
+    e, n = embedding.WordEmbedding(7, 6), normalization.BlockNorm(6, "rms")
+    ids, dy, dW, stats, dw = on((9000,), "int32"), on((9000, 6)), on((7, 6)), on((9000, 2)), on((6,))
+    for call in (lambda: e.BackwardPropagation(dW, ids, dy),
+                 lambda: n.BackwardPropagation(dy, dy, dy, preStatistics=stats, dPreWeight=dw)):
+        given.clear()
+        for stream[0] in (0, 0x1000, 0x2000, 0x1000, 0):
+            call()
+        null, first, second = given[:3]
+        assert len({null, first, second}) == 3 and None not in given and given[3:] == [first, null]
+    p, q = ctypes.c_void_p(1), ctypes.byref(ctypes.c_void_p())
+    assert lib.snhip_get_stream(None, q) == S.CUBLAS_STATUS_NOT_INITIALIZED and lib.snhip_get_stream(handle, None) == BAD
+    assert lib.snhip_get_stream(handle, ctypes.byref(p)) == 0 and not p.value
+
+
 def test_adamw_after_its_end():
     from sharpnet_amd import optimizer
     tensors = [Stub((3, 4)) for _ in range(4)]
