@@ -172,7 +172,7 @@ __device__ __forceinline__ float round_at_random(float a, unsigned int random, b
     const unsigned int add = random << (7 - MANTISSA);
     const float normal = __uint_as_float((__float_as_uint(a) + add) & ~((1u << (23 - MANTISSA)) - 1u));
     unsigned int k = ((unsigned int)(a * __uint_as_float((unsigned int)(23 - LOWEST + 127) << 23)) + add) >> (23 - MANTISSA);
-    if (never_zero && k == 0 && a > 0.0f) k = 1;
+    if (never_zero && k == 0) k = 1;
     const float small = (float)k * __uint_as_float((unsigned int)(LOWEST - MANTISSA + 127) << 23);
     return a < __uint_as_float((unsigned int)(LOWEST + 127) << 23) ? small : normal;
 }
@@ -233,7 +233,7 @@ __device__ __forceinline__ void store_states(const AdamwEntry& t, long long from
         float a = fabsf(mm[j] * m_inv), b = vv[j] * v_inv;
         if (broken) a = a < __builtin_inff() ? a : 0.0f, b = b < __builtin_inff() ? b : 0.0f;
         m_out[j] = copysignf(round_at_random<3, -6>(a, r.v[j] & 0xffffu, false), mm[j]);
-        v_out[j] = round_at_random<2, -14>(b, r.v[j] >> 16, true);
+        v_out[j] = round_at_random<2, -14>(b, r.v[j] >> 16, vv[j] > 0.0f);  // (b may have underflowed)
     }
     // (the values are exact in their formats: the conversions round nothing)
     unsigned int m_word = 0, v_word = 0;

@@ -514,6 +514,24 @@ def test_adamw_gradients_that_are_not_finite_or_at_the_ends_of_the_range(gpu_wra
         p = got
 
 
+def test_adamw_8_bit_v_is_never_zero_beside_a_huge_one(gpu_wrapper):
+    """A block's elements of 1e-20 beside one of 1e32: what scaling by the block's power of two leaves of them is below the
+    smallest fp32 number, stored they are the smallest code, not zero."""
+    from sharpnet_amd import optimizer
+    w, n = gpu_wrapper, 600
+    g = np.zeros(n, np.float32)
+    g[0], g[1], g[2:200:3], g[256:512], g[512] = 1e17, 1e-9, -1e-9, 1e-9, 1e17
+    opt = optimizer.AdamW([tensor(w, np.ones(n, np.float32))], [tensor(w, g)], weightDecay=0.0, stateBits=8, seed=4, **ADAM)
+    opt.Step()
+    z = np.zeros(n, np.float32)
+    m, v = ref.moments(z, z, g, 0.9, 0.99)
+    code, scale = ref.store_v(v, ref.random_words(n, 0, 1, 4))
+    assert np.array_equal(opt.States[0][3].ToNumpy(), scale)
+    below = (v > 0) & (v * np.repeat(ref.power(127 - scale.astype(np.int64)), 256)[:n] == 0)
+    assert below.sum() == 67
+    assert np.array_equal(opt.States[0][1].ToNumpy(), np.where(below, 1, code))
+
+
 def test_adamw_of_memory_that_has_gone(gpu_wrapper):
     """Parameters that are parts of one buffer: the step is refused once the buffer is disposed, not for a view of it."""
     from sharpnet_amd import optimizer
