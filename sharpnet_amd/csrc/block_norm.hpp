@@ -182,10 +182,26 @@ __device__ __forceinline__ f32x4 gate_values(f32x4 g, int act) {
     }
     return g;
 }
-__device__ __forceinline__ f32x4 gate_slopes(f32x4 q, int act) {  // in terms of q = act(g)
-    if (act == GATE_SIGMOID) return q - q * q;
-    if (act == GATE_TANH) return 1.0f - q * q;
-    return f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+// act(g) in place of g, and its slope: from e = exp(-|g|) or exp(-2 |g|), e / (1 + e)^2 and 4 e / (1 + e)^2.  (q - q q and 1 - q q of
+// the rounded q lose the digits of a gate near its limit: a sigmoid's slope off by 6 % at g = 16 and zero from 18 on.)
+__device__ __forceinline__ f32x4 gate_slopes(f32x4& g, int act) {
+    f32x4 slope = {1.0f, 1.0f, 1.0f, 1.0f};
+    if (act == GATE_SIGMOID) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e = __builtin_amdgcn_exp2f(fabsf(g[j]) * -1.44269504088896341f), r = __builtin_amdgcn_rcpf(1.0f + e), q = e * r;
+            slope[j] = q * r;
+            g[j] = g[j] < 0.0f ? q : r;
+        }
+    } else if (act == GATE_TANH) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float e = __builtin_amdgcn_exp2f(fabsf(g[j]) * -2.88539008177792681f), r = __builtin_amdgcn_rcpf(1.0f + e);
+            slope[j] = 4.0f * e * r * r;
+        }
+        g = gate_values(g, act);
+    }
+    return slope;
 }
 
 // which row of the workgroup's rows this thread works on: the same for a wavefront where a row takes one or more
@@ -436,9 +452,9 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
                         g = P::value(now.g[n], n, lane, dim);
                     else
                         g = P::vector(static_cast<const float*>(p.gate), n, lane, dim, 1.0f);
-                    const f32x4 q = gate_values(g, p.act);
-                    acc_g[n] += t[n] * v * gate_slopes(q, p.act);
-                    t[n] *= q;
+                    const f32x4 slope = gate_slopes(g, p.act);  // (g: the gate's values from here on)
+                    acc_g[n] += t[n] * v * slope;
+                    t[n] *= g;
                 }
                 if constexpr (MODE == 2) {
                     acc_pw[n] += t[n] * hat[n];

@@ -318,6 +318,28 @@ def test_block_norm_backward(gpu_wrapper, rows, dim, pre, post, gate_rows, activ
         assert np.array_equal(o2["d_gate"].ToNumpy(), first["d_gate"])
 
 
+@pytest.mark.parametrize("activation", ["sigmoid", "tanh"])
+@pytest.mark.parametrize("gate_rows", [0, 1])
+def test_block_norm_gradient_of_a_saturated_gate(gpu_wrapper, activation, gate_rows):
+    """The gate's gradient keeps its digits where the activation has run into its limit, the same on both sides.  With
+    e = exp(-k |g|) (k = 1, 2) the slope is e / (1 + e)^2 or four times that: the exponent's product and its constant are off by
+    u each, 2 u k |g| of e; the hardware's exponential and reciprocal (twice) by 2 u each, 1 + e (twice) and three products by u;
+    what the slope is multiplied with by 3 u more: (16 + 2 k |g|) u."""
+    from sharpnet_amd import normalization
+    w, rng = gpu_wrapper, np.random.default_rng(21)
+    k = 2 if activation == "tanh" else 1
+    g = np.concatenate((np.linspace(-20, 20, 161), [-38.0, -30.0, 30.0, 38.0, 1e-3, -1e-3, 0.2499, 0.25, 0.0])).astype(np.float32)
+    dim, rows = g.size, 1 if gate_rows == 0 else 3
+    gate = np.broadcast_to(g, (rows, dim)) if gate_rows else g
+    y, du = rng.normal(0, 1, (rows, dim)).astype(np.float32), rng.normal(0, 1, (rows, dim)).astype(np.float32)
+    dgate, dx, dy = empty(w, gate.shape), empty(w, (rows, dim)), empty(w, (rows, dim))
+    layer = normalization.BlockNorm(dim, "rms", None, residualScale=0.5, gateActivation=activation)
+    layer.BackwardPropagation(dx, None, None, du=tensor(w, du), y=tensor(w, y), dy=dy, gate=tensor(w, gate), dGate=dgate, gateRows=gate_rows)
+    e = np.exp(-k * np.abs(g.astype(np.float64)))
+    want = 0.5 * du.astype(np.float64) * y * (k * k * e / (1 + e) ** 2)
+    within(dgate.ToNumpy().reshape(want.shape), want, (16 + 2 * k * np.abs(g)) * ref.U * np.abs(want) + ref.TINY, "d_gate")
+
+
 def test_block_norm_rows_without_spread_and_missing_parts(gpu_wrapper):
     """Rows of one value (variance 0: 1 / deviation = 1 / sqrt(epsilon)), rows of zeros, a backward call without du and one
     without dh, gradients that are not wanted."""
