@@ -43,7 +43,7 @@ class WordEmbedding:
             mine["desc"] = EmbeddingDesc(id_type=_ID_TYPES[x.Type], table_type=_ROW_TYPES[table_type], output_type=_ROW_TYPES[rows.Type],
                                          tokens=tokens, vocabulary=self.VocabularySize, dim=dim, padding_index=self.PaddingIndex,
                                          scale=self.Scale)
-            mine["call"] = call
+            mine["call"], mine["need"] = call, None
         return mine["desc"]
 
     def _check_table(self, table):
@@ -71,12 +71,12 @@ class WordEmbedding:
         self._check_table(dWordEmbedding)
         if dWordEmbedding.Type != "float32":
             raise ValueError("the table's gradient must be float32, not %s" % dWordEmbedding.Type)
-        d, need, w = self._desc(x, dy, "float32"), ctypes.c_size_t(), dy.Wrapper
+        d, w, mine = self._desc(x, dy, "float32"), dy.Wrapper, self._mine.__dict__
         pointers = pointer_on(w, x), pointer_on(w, dy), pointer_on(w, dWordEmbedding)
-        check_status(dy._lib.snhip_embedding_backward_workspace_size(ctypes.byref(d), ctypes.byref(need)),
-                     "snhip_embedding_backward_workspace_size")
-        if workspace is None and need.value > 0:
-            workspace = self._workspace.Get(w, need.value, stream_of(w))
+        if workspace is None:
+            if mine["need"] is None:
+                mine["need"] = self.BackwardWorkspaceSize(x, dy)
+            workspace = self._workspace.Get(w, mine["need"], stream_of(w)) if mine["need"] > 0 else None
         check_status(dy._lib.snhip_embedding_backward(w.handle, ctypes.byref(d), *pointers, int(bool(accumulate)),
                                                       pointer_on(w, workspace),
                                                       workspace.Count * workspace.ElementBytes if workspace is not None else 0),

@@ -18,6 +18,7 @@ stage host data for the H2D / D2H copies.
 """
 import ctypes
 import math
+import threading
 
 import numpy as np
 
@@ -408,11 +409,19 @@ class GPUTensor:
 
 
 # -- element-wise / row helpers next to the GEMMs (same names as the reference's Tensor methods) -----------------
+_mine = threading.local()  # where each thread's calls of snhip_get_stream put their answer
+
+
 def stream_of(wrapper):
     """The address of the stream that the wrapper's calls go to (0: the null stream)."""
-    stream = ctypes.c_void_p()
-    check_status(wrapper.lib.snhip_get_stream(wrapper.handle, ctypes.byref(stream)), "snhip_get_stream")
-    return stream.value or 0
+    answer = _mine.__dict__.get("answer")
+    if answer is None:
+        stream = ctypes.c_void_p()
+        answer = _mine.answer = stream, ctypes.byref(stream)
+    status = wrapper.lib.snhip_get_stream(wrapper.handle, answer[1])
+    if status:
+        check_status(status, "snhip_get_stream")
+    return answer[0].value or 0
 
 
 class LayerWorkspace:
@@ -426,7 +435,9 @@ class LayerWorkspace:
         """A uint8 tensor of at least nbytes, or None for none."""
         if nbytes == 0:
             return None
-        held = self._held.setdefault((wrapper, stream), [])
+        held = self._held.get((wrapper, stream))
+        if held is None:
+            held = self._held.setdefault((wrapper, stream), [])
         if not held or held[-1].Shape[0] < nbytes:
             size = max(nbytes, held[-1].Shape[0] * 3 // 2) if held else nbytes  # (all together: at most three times the last)
             held.append(GPUTensor([size], None, wrapper, element_type="uint8"))

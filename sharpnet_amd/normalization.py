@@ -129,7 +129,9 @@ class BlockNorm:
                              "snhip_block_norm_backward_workspace_size")
                 mine["call"], mine["need"] = (list(shape),) + call[1:], need.value
             workspace = self._workspace.Get(w, mine["need"], stream_of(w)) if mine["need"] > 0 else None
-        nbytes = workspace.Count * workspace.ElementBytes if workspace is not None else 0
+            nbytes = workspace.Shape[0] if workspace is not None else 0
+        else:
+            nbytes = workspace.Count * workspace.ElementBytes
         check_status(lib.snhip_block_norm_backward(w.handle, ctypes.byref(d), pointer_on(w, workspace), nbytes),
                      "snhip_block_norm_backward")
 
