@@ -415,7 +415,8 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
  * weights and biases are fp32 vectors of dim elements, NULL for ones and zeros; post_weight / post_bias belong to
  * post_norm and are ignored without it.
  * statistics: (mean, rstd) per row as the backward call wants them, NULL to skip; sums are taken in fp32 over the row in
- * registers, the variance around the mean.
+ * registers, the variance around the mean (its squares leave fp32 for deviations beyond 1e19; below 1e-19, which matter
+ * with next to no epsilon, they lose digits and at 1e-23 vanish).
  * Backward, from dh and du (the gradients that reach h and u; either may be NULL = zeros, not both):
  *     t = du + dN_pre(dh);  dx = t;  dy = dN_post(residual_scale * act(gate) * t)
  * and the gradients of gate, weights and biases (each NULL to skip) summed over the rows in a fixed order: bits repeat.

@@ -231,7 +231,10 @@ __device__ __forceinline__ void row_statistics(const f32x4 (&z)[N], int lane, in
         const f32x4 d = Piece<TPR, EXACT>::cut(z[n] - mean, n, lane, p.dim);
         s += (d[0] * d[0] + d[1] * d[1]) + (d[2] * d[2] + d[3] * d[3]);
     }
-    rstd = __builtin_amdgcn_rsqf(row_sum<TPR>(s, lds, turn) * p.inv_dim + p.eps);
+    // (the hardware's reciprocal root takes numbers below the normal ones for zeros: a small one goes in times 2^96)
+    const float variance = row_sum<TPR>(s, lds, turn) * p.inv_dim + p.eps;
+    const bool tiny = variance < 0x1p-96f;
+    rstd = __builtin_amdgcn_rsqf(tiny ? variance * 0x1p+96f : variance) * (tiny ? 0x1p+48f : 1.0f);
 }
 
 template <typename TS, typename TB, int TPR, int N, bool EXACT>

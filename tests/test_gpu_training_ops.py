@@ -373,6 +373,23 @@ def test_block_norm_rows_without_spread_and_missing_parts(gpu_wrapper):
     within(dpw.ToNumpy(), *back["d_post_weight"], "d_post_weight")
 
 
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("dim", [36, 260, 1001, 4096])
+def test_block_norm_of_tiny_rows_without_epsilon(gpu_wrapper, kind, dim):
+    """Rows whose mean square is below the normal numbers, epsilon = 0.  A square there and the mean are off by 2^-150 each
+    besides their relative rounding: the variance by 2^-149 / variance, 1 / deviation by half of that."""
+    from sharpnet_amd import normalization
+    w, rng = gpu_wrapper, np.random.default_rng(dim)
+    x = (rng.normal(0, 1, (5, dim)) * np.array([[1.0], [1e-18], [1e-19], [5e-20], [2e-20]])).astype(np.float32)
+    h, s = empty(w, x.shape), empty(w, (5, 2))
+    normalization.BlockNorm(dim, kind, epsilon=0.0).ForwardPropagation(tensor(w, x), h, preStatistics=s)
+    mean, rstd = ref.statistics(x, kind, 0.0)
+    rel = ref.C * ref.U + 2.0 ** -150 * rstd ** 2
+    want = (x - mean) * rstd
+    within(h.ToNumpy(), want, rel * (np.abs(x) + np.abs(x).mean(1, keepdims=True)) * rstd, "h")
+    within(s.ToNumpy()[:, 1:], rstd, rel * rstd, "1 / deviation")
+
+
 def test_block_norm_without_rows(gpu_wrapper):
     from sharpnet_amd import normalization
     w = gpu_wrapper
