@@ -472,7 +472,8 @@ int snhip_block_norm_backward(void* handle, const snhip_block_norm_desc* desc, v
  *     g = gradient_scale * gradient;  m' = beta1 m + (1 - beta1) g;  v' = beta2 v + (1 - beta2) g g
  *     p' = p (1 - learning_rate weight_decay) - learning_rate / (1 - beta1^step) * m' / (sqrt(v') / sqrt(1 - beta2^step) + epsilon)
  * in fp32, each product and sum of m' and v' rounded by itself, and writes a bf16 copy of p' for the bf16-stored products
- * where a tensor has one.  (With epsilon = 0 an element whose gradients have all been zero is 0 / 0, NaN.)
+ * where a tensor has one.  (With epsilon = 0 an element whose gradients have all been zero is 0 / 0, NaN.)  Status 7 for an
+ * epsilon between 0 and 2^-126, and for a learning rate that fp32 does not hold (divided by 1 - beta1^step, too).
  * state_bits = 32: moment1 and moment2 are fp32.  state_bits = 8: blocks of 256 consecutive elements of a tensor (the last
  * one shorter) keep m in e4m3 and v in e5m2 with a power of two per block and moment, 2^(scale - 127): scale1 / scale2 hold
  * one byte a block, max(e - 7, 1) for m and max(e - 14, 1) for v, where e is the biased exponent of the block's largest

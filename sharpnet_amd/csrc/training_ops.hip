@@ -2,6 +2,7 @@
 // launch shape, launches.  Declarations are in include/sharpnet_hip.h.
 #include "../../include/sharpnet_hip.h"
 
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -563,6 +564,11 @@ int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
     if (d->step < 1 || !isfinite(d->learning_rate) || !(d->beta1 >= 0.0 && d->beta1 < 1.0) || !(d->beta2 >= 0.0 && d->beta2 < 1.0) ||
         !(d->epsilon >= 0.0) || !isfinite(d->epsilon) || !isfinite(d->gradient_scale))
         return SNHIP_STATUS_INVALID_VALUE;
+    // What the kernels are given in fp32 has to fit: an epsilon below the normal numbers would be a zero to the reciprocal, a rate
+    // beyond the largest one times nothing not a number.
+    const double step_size = d->learning_rate / (1.0 - pow(d->beta1, d->step));
+    if ((d->epsilon > 0.0 && d->epsilon < FLT_MIN) || fabs(d->learning_rate) > FLT_MAX || fabs(step_size) > FLT_MAX)
+        return SNHIP_STATUS_INVALID_VALUE;
     if (a->chunks == 0) return SNHIP_STATUS_SUCCESS;
     DeviceScope scope(h->device);
     if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
@@ -570,7 +576,7 @@ int snhip_adamw_step(void* handle, void* plan, const snhip_adamw_step_desc* d) {
     s.beta1 = (float)d->beta1, s.rest1 = (float)(1.0 - d->beta1);
     s.beta2 = (float)d->beta2, s.rest2 = (float)(1.0 - d->beta2);
     s.rate = (float)d->learning_rate;
-    s.step_size = (float)(d->learning_rate / (1.0 - pow(d->beta1, d->step)));
+    s.step_size = (float)step_size;
     s.root_scale = (float)(1.0 / sqrt(1.0 - pow(d->beta2, d->step)));
     s.eps = (float)d->epsilon, s.grad_scale = d->gradient_scale;
     s.key0 = (unsigned int)d->seed, s.key1 = (unsigned int)(d->seed >> 32), s.step = (unsigned int)d->step;

@@ -189,6 +189,16 @@ def test_adamw_step_checks(lib, handle, change):
     assert lib.snhip_adamw_step(handle, ctypes.addressof(plan), None) == BAD
 
 
+@pytest.mark.parametrize("change,status", [({"epsilon": 1e-40}, BAD), ({"epsilon": 1e-300}, BAD), ({"epsilon": 0.0}, 0), ({"epsilon": 2.0 ** -126}, 0),
+                                           ({"learning_rate": 1e39}, BAD), ({"learning_rate": -1e39}, BAD), ({"learning_rate": 1e38}, BAD),
+                                           ({"learning_rate": 1e38, "beta1": 0.0}, 0), ({"learning_rate": 0.0}, 0)])
+def test_adamw_scalars_that_fp32_does_not_hold(lib, handle, change, status):
+    """1e38 / (1 - 0.9) is beyond fp32's largest number; an epsilon below its normal numbers would be a division by zero."""
+    plan = ctypes.create_string_buffer(256)      # a plan of no chunks on device 0
+    d = hiplib.AdamwStepDesc(**{"learning_rate": 1e-3, **change})
+    assert lib.snhip_adamw_step(handle, ctypes.addressof(plan), ctypes.byref(d)) == status
+
+
 class Stub:
     """Shape and type of a tensor, for the host side's checks."""
     _disposed, _owner, handle = False, None, None
