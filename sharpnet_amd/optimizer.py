@@ -33,7 +33,9 @@ class AdamW:
             if g.Count != p.Count or (c is not None and c.Count != p.Count):
                 raise ValueError("a gradient or copy of %s does not fit its parameters of %s" % (g.Shape, p.Shape))
         if states is None:
-            states = [self._zero_states(p) for p in parameters]
+            states = [self._zero_states(p, parameters[0].Wrapper) for p in parameters]
+            if count:
+                parameters[0].Wrapper.synchronize()  # (the steps may go to another stream)
         for p, s in zip(parameters, states):
             self._check_states(p, s)
         # the plan holds addresses: everything it points at stays alive with it
@@ -56,11 +58,11 @@ class AdamW:
         check_status(self._lib.snhip_adamw_create(self._wrapper.handle, table, count, stateBits, ctypes.byref(plan)), "snhip_adamw_create")
         self._plan = plan
 
-    def _zero_states(self, p):
+    def _zero_states(self, p, wrapper):
         if self.StateBits == 32:
-            made = [GPUTensor(p.Shape, None, p.Wrapper) for _ in range(2)]
+            made = [GPUTensor(p.Shape, None, wrapper) for _ in range(2)]
         else:
-            made = [GPUTensor([n], None, p.Wrapper, element_type="uint8") for n in (p.Count, p.Count, -(-p.Count // 256), -(-p.Count // 256))]
+            made = [GPUTensor([n], None, wrapper, element_type="uint8") for n in (p.Count, p.Count, -(-p.Count // 256), -(-p.Count // 256))]
         for t in made:
             t.ZeroMemory()
         return made

@@ -388,6 +388,46 @@ def test_scratch_memory_goes_by_stream(lib, handle):
     assert lib.snhip_get_stream(handle, ctypes.byref(p)) == 0 and not p.value
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_clears_its_states_where_its_steps_go(bits):
+    """Parameters of two wrappers of a device: the states are cleared by the one that the steps are issued by, and are clear
+    before the plan is made."""
+    from sharpnet_amd import optimizer
+    log = []
+
+    class Wrapper:
+        device_id = 0
+
+        def __init__(self, name):
+            self.lib, self.handle, self.made = self, name, 0
+
+        def allocate(self, nbytes):
+            self.made += 1
+            return A + (self.made << 20)
+
+        def release(self, pointer, nbytes):
+            pass
+
+        def synchronize(self):
+            log.append(("wait", self.handle))
+
+        def snhip_memset32(self, handle, *args):
+            log.append(("clear", handle))
+            return 0
+
+        def snhip_adamw_create(self, handle, *args):
+            log.append(("create", handle))
+            return 0
+    first, second = Wrapper("first"), Wrapper("second")
+    tensors = [Stub((300,)) for _ in range(4)]
+    for t, w in zip(tensors, (first, second, first, second)):
+        t.Wrapper = t._lib = w
+    opt = optimizer.AdamW(tensors[:2], tensors[2:], stateBits=bits)
+    clears = 2 * (2 if bits == 32 else 4)
+    assert log == [("clear", "first")] * clears + [("wait", "first"), ("create", "first")]
+    opt._plan = None  # (nothing to destroy)
+
+
 def test_adamw_after_its_end():
     from sharpnet_amd import optimizer
     tensors = [Stub((3, 4)) for _ in range(4)]
