@@ -25,7 +25,6 @@ class WordEmbedding:
         self.VocabularySize, self.EmbeddingDim = int(vocabularySize), int(embeddingDim)
         self.Scale, self.PaddingIndex = float(scale), int(paddingIndex)
         self.Wrapper = gpu_wrapper
-        self._tableShape = [self.VocabularySize, self.EmbeddingDim]
         self._workspace = LayerWorkspace()
         self._mine = threading.local()  # for each thread: its last call's sizes and types, and their descriptor
 
@@ -34,7 +33,7 @@ class WordEmbedding:
         tokens, mine, dim = math.prod(x.Shape), self._mine.__dict__, self.EmbeddingDim
         if rows.Shape[-1] != dim or math.prod(rows.Shape) != tokens * dim:
             raise ValueError("%s ids and rows of %s do not fit an embedding dimension of %d" % (x.Shape, rows.Shape, dim))
-        call = (x.Type, table_type, rows.Type, tokens, self.PaddingIndex, self.Scale)
+        call = (x.Type, table_type, rows.Type, tokens, self.VocabularySize, dim, self.PaddingIndex, self.Scale)
         if mine.get("call") != call:
             if x.Type not in _ID_TYPES:
                 raise ValueError("ids must be float32, int32 or int64, not %s" % x.Type)
@@ -47,8 +46,8 @@ class WordEmbedding:
         return mine["desc"]
 
     def _check_table(self, table):
-        if table.Shape != self._tableShape:
-            raise ValueError("the table must be %s, not %s" % (self._tableShape, table.Shape))
+        if table.Shape != [self.VocabularySize, self.EmbeddingDim]:
+            raise ValueError("the table must be %s, not %s" % ([self.VocabularySize, self.EmbeddingDim], table.Shape))
 
     def ForwardPropagation(self, y, x, wordEmbedding):
         """y (ids' shape + EmbeddingDim) = Scale * wordEmbedding[x]."""

@@ -71,6 +71,10 @@ class BlockNorm:
         if gateRows < 0:
             raise ValueError("gateRows is %d" % gateRows)
         rows, mine = math.prod(stream.Shape) // dim, self._mine.__dict__
+        kind = self.PreNorm, self.PostNorm, self.GateActivation, dim
+        if mine.get("kind") != kind:  # (the first call, or the layer has been changed)
+            mine.clear()
+            mine["kind"], self._vectorShape = kind, [dim]
         d = mine.get(direction)
         if d is None:
             d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=dim)

@@ -310,6 +310,46 @@ def test_one_layer_called_by_two_threads():
     assert not wrong
 
 
+def test_layers_that_are_changed_between_calls():
+    """The next call goes by the norms, the activation and the sizes that the layer has by then, its scratch size included."""
+    from sharpnet_amd import embedding, normalization
+    seen, sizes = [], []
+    kind = lambda d: (d.pre_norm, d.post_norm, d.gate_activation, d.dim, d.epsilon, d.residual_scale)  # noqa: E731
+
+    def tensor(*shape, type_="float32"):
+        t = Stub(shape, type_)
+        t.snhip_block_norm_forward = t.snhip_block_norm_backward = lambda handle, d, *rest: seen.append(kind(d._obj)) or 0
+        t.snhip_block_norm_backward_workspace_size = lambda d, out: sizes.append(kind(d._obj)) or 0
+        t.snhip_embedding_forward = lambda handle, d, *rest: seen.append((d._obj.vocabulary, d._obj.dim)) or 0
+        return t
+    n = normalization.BlockNorm(8, "layer", "rms", 0.5, epsilon=0.25)
+    x, v, s = tensor(5, 8), tensor(8), tensor(5, 2)
+
+    def both(x, v):
+        n.ForwardPropagation(x, x, y=x, u=x, gate=v, preWeight=v)
+        n.BackwardPropagation(x, x, x, y=x, dy=x, gate=v, preWeight=v, preStatistics=s, postStatistics=s)
+        return seen[-2:], sizes[-1:]
+    want = (hiplib.NORM_LAYER, hiplib.NORM_RMS, hiplib.ACT_NONE, 8, 0.25, 0.5)
+    assert both(x, v) == ([want] * 2, [want])
+    n.PreNorm, n.PostNorm, n.GateActivation, n.Epsilon, n.ResidualScale = hiplib.NORM_RMS, hiplib.NORM_LAYER, hiplib.ACT_TANH, 0.5, 2.0
+    want = (hiplib.NORM_RMS, hiplib.NORM_LAYER, hiplib.ACT_TANH, 8, 0.5, 2.0)
+    assert both(x, v) == ([want] * 2, [want])
+    n.EmbeddingDim = 4
+    with pytest.raises(ValueError):
+        both(x, v)
+    with pytest.raises(ValueError):
+        both(tensor(10, 4), v)
+    s = tensor(10, 2)
+    assert both(tensor(10, 4), tensor(4))[0] == [want[:3] + (4,) + want[4:]] * 2
+    e = embedding.WordEmbedding(7, 6)
+    e.ForwardPropagation(tensor(10, 6), tensor(10, type_="int32"), tensor(7, 6))
+    e.VocabularySize = 9
+    with pytest.raises(ValueError):
+        e.ForwardPropagation(tensor(10, 6), tensor(10, type_="int32"), tensor(7, 6))
+    e.ForwardPropagation(tensor(10, 6), tensor(10, type_="int32"), tensor(9, 6))
+    assert seen[-2:] == [(7, 6), (9, 6)]
+
+
 def test_workspace_of_a_layer():
     """One for each wrapper; a longer one leaves the one before in place until Dispose."""
     from sharpnet_amd.gpu_tensor import LayerWorkspace
