@@ -40,8 +40,8 @@ class WordEmbedding:
             if rows.Type not in _ROW_TYPES or table_type not in _ROW_TYPES:
                 raise ValueError("rows and table must be float32 or bfloat16, not %s and %s" % (rows.Type, table_type))
             mine["desc"] = EmbeddingDesc(id_type=_ID_TYPES[x.Type], table_type=_ROW_TYPES[table_type], output_type=_ROW_TYPES[rows.Type],
-                                         tokens=tokens, vocabulary=self.VocabularySize, dim=dim, padding_index=self.PaddingIndex,
-                                         scale=self.Scale)
+                                         tokens=tokens, vocabulary=self.VocabularySize, dim=dim, scale=self.Scale,
+                                         padding_index=self.PaddingIndex if self.PaddingIndex < self.VocabularySize else -1)
             mine["call"], mine["need"] = call, None
         return mine["desc"]
 

@@ -133,6 +133,17 @@ class RnnDesc(ctypes.Structure):
             setattr(self, k, float(v) if k == "dropout" else int(v))
 
 
+def _fill(desc, name, fields):
+    """Sets fields of a descriptor; a number that its field does not hold is refused (ctypes would cut it off)."""
+    types = dict(desc._fields_)
+    for k, v in fields.items():
+        if k not in types:
+            raise TypeError("%s has no field %r" % (name, k))
+        setattr(desc, k, v)
+        if types[k] in (_i, _ll) and getattr(desc, k) != v:
+            raise ValueError("%s.%s does not hold %d" % (name, k, v))
+
+
 class EmbeddingDesc(ctypes.Structure):
     """snhip_embedding_desc of include/sharpnet_hip.h (field for field)."""
     _fields_ = [("struct_size", _i), ("id_type", _i), ("table_type", _i), ("output_type", _i), ("tokens", _ll),
@@ -143,10 +154,7 @@ class EmbeddingDesc(ctypes.Structure):
         super().__init__()
         self.struct_size = ctypes.sizeof(EmbeddingDesc)
         self.padding_index, self.scale = -1, 1.0
-        for k, v in kw.items():
-            if k not in dict(self._fields_):
-                raise TypeError("snhip_embedding_desc has no field %r" % k)
-            setattr(self, k, v)
+        _fill(self, "snhip_embedding_desc", kw)
 
 
 class BlockNormDesc(ctypes.Structure):
@@ -163,10 +171,7 @@ class BlockNormDesc(ctypes.Structure):
         super().__init__()
         self.struct_size = ctypes.sizeof(BlockNormDesc)
         self.epsilon, self.residual_scale = 1e-5, 1.0
-        for k, v in kw.items():
-            if k not in dict(self._fields_):
-                raise TypeError("snhip_block_norm_desc has no field %r" % k)
-            setattr(self, k, v)
+        _fill(self, "snhip_block_norm_desc", kw)
 
 
 class AdamwTensor(ctypes.Structure):
@@ -184,10 +189,7 @@ class AdamwStepDesc(ctypes.Structure):
         super().__init__()
         self.struct_size = ctypes.sizeof(AdamwStepDesc)
         self.step, self.beta1, self.beta2, self.epsilon, self.gradient_scale = 1, 0.9, 0.999, 1e-8, 1.0
-        for k, v in kw.items():
-            if k not in dict(self._fields_):
-                raise TypeError("snhip_adamw_step_desc has no field %r" % k)
-            setattr(self, k, v)
+        _fill(self, "snhip_adamw_step_desc", kw)
 
 
 # SNHIP_NORM_*

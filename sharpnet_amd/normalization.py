@@ -79,7 +79,7 @@ class BlockNorm:
         if d is None:
             d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=dim)
         d.epsilon, d.residual_scale = self.Epsilon, self.ResidualScale
-        d.rows, d.gate_rows = rows, gateRows
+        d.rows, d.gate_rows = rows, min(gateRows, 0x7FFFFFFF)  # (there are no more rows)
         d.stream_type, d.block_type = _ROW_TYPES[stream_type], _ROW_TYPES[block_type]
         d.pre_weight, d.pre_bias = self._vector(w, preWeight, "preWeight"), self._vector(w, preBias, "preBias")
         d.post_weight, d.post_bias = self._vector(w, postWeight, "postWeight"), self._vector(w, postBias, "postBias")

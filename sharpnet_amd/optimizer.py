@@ -86,6 +86,8 @@ class AdamW:
         if learningRate is not None:
             self.LearningRate = learningRate
         if self._plan is not None:
+            if self.StepCount + 1 > 0x7FFFFFFF:
+                raise ValueError("step %d" % (self.StepCount + 1))
             d = AdamwStepDesc()
             d.step, d.learning_rate, d.beta1, d.beta2 = self.StepCount + 1, self.LearningRate, self.Beta1, self.Beta2
             d.epsilon, d.gradient_scale, d.seed = self.Epsilon, gradientScale, self.Seed

@@ -350,6 +350,43 @@ def test_layers_that_are_changed_between_calls():
     assert seen[-2:] == [(7, 6), (9, 6)]
 
 
+def test_sizes_beyond_32_bits_are_not_cut_off():
+    """Numbers that the descriptors' 32-bit fields do not hold: refused, or what they mean where they mean something."""
+    from sharpnet_amd import embedding, normalization, optimizer
+    seen = []
+
+    def tensor(*shape, type_="float32"):
+        t = Stub(shape, type_)
+        t.snhip_embedding_forward = lambda handle, d, *rest: seen.append((d._obj.vocabulary, d._obj.dim, d._obj.padding_index)) or 0
+        t.snhip_block_norm_forward = lambda handle, d: seen.append(d._obj.gate_rows) or 0
+        t.snhip_adamw_step = lambda handle, plan, d: seen.append(d._obj.step) or 0
+        return t
+    large, ids = 2 ** 32 + 5, tensor(10, type_="int32")
+    for vocabulary, dim in ((large, 1), (7, large), (2 ** 31, 1)):
+        with pytest.raises(ValueError):
+            embedding.WordEmbedding(vocabulary, dim).ForwardPropagation(tensor(10, dim), ids, tensor(vocabulary, dim))
+    for padding in (large, 2 ** 31, 2 ** 32 - 1, 7):  # beyond the vocabulary: no token's
+        embedding.WordEmbedding(7, 6, paddingIndex=padding).ForwardPropagation(tensor(10, 6), ids, tensor(7, 6))
+    embedding.WordEmbedding(7, 6, paddingIndex=6).ForwardPropagation(tensor(10, 6), ids, tensor(7, 6))
+    assert seen == [(7, 6, -1)] * 4 + [(7, 6, 6)]
+    seen.clear()
+    with pytest.raises(ValueError):
+        normalization.BlockNorm(large).ForwardPropagation(tensor(1, large), tensor(1, large))
+    x = tensor(10, 6)
+    for rows in (2 ** 32, large, 2 ** 31):  # one row of the gate for all
+        normalization.BlockNorm(6).ForwardPropagation(x, x, y=x, u=x, gate=tensor(1, 6), gateRows=rows)
+    assert seen == [2 ** 31 - 1] * 3
+    seen.clear()
+    opt = optimizer.AdamW([x], [x], states=[[x, x]], step=2 ** 31 - 2)
+    opt._plan = ctypes.c_void_p(A)
+    opt.Step()
+    for opt.StepCount in (2 ** 31 - 1, 2 ** 32, large):
+        with pytest.raises(ValueError):
+            opt.Step()
+    assert seen == [2 ** 31 - 1]
+    opt._plan = None
+
+
 def test_workspace_of_a_layer():
     """One for each wrapper; a longer one leaves the one before in place until Dispose."""
     from sharpnet_amd.gpu_tensor import LayerWorkspace
