@@ -410,7 +410,8 @@ int snhip_embedding_backward(void* handle, const snhip_embedding_desc* desc, con
  * rstd = 1 / sqrt(mean of (z - mean)^2 + epsilon) with mean = 0 for RMS, over the `dim` elements of a row: the reference's
  * StandardizeRowsInPlaceBroadcastGammasBetas / RMSStandardizeRowsInPlaceBroadcastGammas and the LayerNormalizationBackward
  * / RMSNormalizationBackward kernels (Prod/GPU/Kernels/SinglePrecision.cu:82,108,158-236).
- * Without y the call is the norm alone (u is not written and may be NULL); with pre_norm = SNHIP_NORM_NONE there is no h.
+ * Without y the call is the norm alone (u and dy are not written and may be NULL; a backward call takes y as the sign that there
+ * is a block, also where it needs none of its values); with pre_norm = SNHIP_NORM_NONE there is no h.
  * gate: NULL; one fp32 vector of dim elements (gate_rows = 0); or rows of block_type, row r / gate_rows for row r.
  * weights and biases are fp32 vectors of dim elements, NULL for ones and zeros; post_weight / post_bias belong to
  * post_norm and are ignored without it.

@@ -98,6 +98,9 @@ class BlockNorm:
         shape, w, stream_type = x.Shape, x.Wrapper, x.Type
         block = h if h is not None else y if y is not None else x
         block_type = block.Type
+        if (u is not None and y is None) or (self.PreNorm == NORM_NONE and (h is not None or preStatistics is not None)) or \
+                (self.PostNorm == NORM_NONE and postStatistics is not None):
+            raise ValueError("there is no u without y, and neither h nor statistics without their norm")
         d = self._desc("forward", x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
         d.x, d.u = pointer_on(w, x), self._rows(w, u, "u", shape, stream_type)
         d.y, d.h = self._rows(w, y, "y", shape, block_type), self._rows(w, h, "h", shape, block_type)
@@ -106,12 +109,14 @@ class BlockNorm:
     def BackwardPropagation(self, dx, u, dh, du=None, y=None, dy=None, gate=None, dGate=None, gateRows=0, preWeight=None,
                             preStatistics=None, dPreWeight=None, dPreBias=None, postWeight=None, postBias=None, postStatistics=None,
                             dPostWeight=None, dPostBias=None, accumulate=False, workspace=None):
-        """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics; gradients that are
-        None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
+        """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics (y also where its values
+        do not matter: without it there is no block and no dy); gradients that are None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
         shape, w, lib, stream_type = dx.Shape, dx.Wrapper, dx._lib, dx.Type
         block = dh if dh is not None else y if y is not None else dy if dy is not None else dx
         block_type = block.Type
+        if dy is not None and y is None:
+            raise ValueError("dy is wanted without y")
         d = self._desc("backward", dx, block, gate, gateRows, preWeight, None, postWeight, postBias, preStatistics, postStatistics)
         d.dx, d.u, d.du = pointer_on(w, dx), self._rows(w, u, "u", shape, stream_type), self._rows(w, du, "du", shape, stream_type)
         d.dh, d.y = self._rows(w, dh, "dh", shape, block_type), self._rows(w, y, "y", shape, block_type)

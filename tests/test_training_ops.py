@@ -387,6 +387,21 @@ def test_sizes_beyond_32_bits_are_not_cut_off():
     opt._plan = None
 
 
+def test_block_norm_outputs_that_would_stay_as_they_are_are_refused():
+    from sharpnet_amd import normalization
+    x, s = Stub((5, 8)), Stub((5, 2))
+    norm, join, bare = normalization.BlockNorm(8), normalization.BlockNorm(8, None, "rms"), normalization.BlockNorm(8, None)
+    for call in (lambda: norm.ForwardPropagation(x, x, u=x), lambda: join.ForwardPropagation(x, x, y=x, u=x),
+                 lambda: bare.ForwardPropagation(x, x, y=x, u=x), lambda: norm.BackwardPropagation(x, x, x, dy=x, preStatistics=s),
+                 lambda: bare.BackwardPropagation(x, None, None, du=x, dy=x),
+                 lambda: join.ForwardPropagation(x, None, y=x, u=x, preStatistics=s), lambda: norm.ForwardPropagation(x, x, postStatistics=s)):
+        with pytest.raises(ValueError):
+            call()
+    norm.ForwardPropagation(x, x, preStatistics=s)
+    join.ForwardPropagation(x, None, y=x, u=x, postStatistics=s)
+    bare.BackwardPropagation(x, None, None, du=x, y=x, dy=x)
+
+
 def test_workspace_of_a_layer():
     """One for each wrapper; a longer one leaves the one before in place until Dispose."""
     from sharpnet_amd.gpu_tensor import LayerWorkspace
