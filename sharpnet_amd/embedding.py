@@ -17,7 +17,8 @@ _ROW_TYPES = {k: TYPES[k] for k in ("float32", "bfloat16")}
 
 
 class WordEmbedding:
-    """The layer: sizes, scale and the scratch memory of its backward pass."""
+    """The layer: sizes, scale and the scratch memory of its backward pass.  Its calls go to gpu_wrapper, without one to the wrapper
+    of the rows they are given."""
 
     def __init__(self, vocabularySize, embeddingDim, scale=1.0, paddingIndex=-1, gpu_wrapper=None):
         if vocabularySize < 0 or embeddingDim < 0 or paddingIndex < -1:
@@ -52,7 +53,7 @@ class WordEmbedding:
     def ForwardPropagation(self, y, x, wordEmbedding):
         """y (ids' shape + EmbeddingDim) = Scale * wordEmbedding[x]."""
         self._check_table(wordEmbedding)
-        d, w = self._desc(x, y, wordEmbedding.Type), y.Wrapper
+        d, w = self._desc(x, y, wordEmbedding.Type), self.Wrapper or y.Wrapper
         check_status(y._lib.snhip_embedding_forward(w.handle, ctypes.byref(d), pointer_on(w, x), pointer_on(w, wordEmbedding),
                                                     pointer_on(w, y)), "snhip_embedding_forward")
 
@@ -70,7 +71,7 @@ class WordEmbedding:
         self._check_table(dWordEmbedding)
         if dWordEmbedding.Type != "float32":
             raise ValueError("the table's gradient must be float32, not %s" % dWordEmbedding.Type)
-        d, w, mine = self._desc(x, dy, "float32"), dy.Wrapper, self._mine.__dict__
+        d, w, mine = self._desc(x, dy, "float32"), self.Wrapper or dy.Wrapper, self._mine.__dict__
         pointers = pointer_on(w, x), pointer_on(w, dy), pointer_on(w, dWordEmbedding)
         if workspace is None:
             if mine["need"] is None:

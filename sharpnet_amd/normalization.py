@@ -22,7 +22,8 @@ _ROW_TYPES = {k: TYPES[k] for k in ("float32", "bfloat16")}
 class BlockNorm:
     """The join between two blocks: kinds of the two norms ("rms", "layer" or None), the factor of the block's output and
     the activation of its gate.  Tensors of the stream (x, u and their gradients) have one type, those of the blocks (y, h, a
-    gate in rows and their gradients) another or the same; weights, biases and a gate vector are float32."""
+    gate in rows and their gradients) another or the same; weights, biases and a gate vector are float32.  Calls go to gpu_wrapper,
+    without one to the wrapper of the stream's tensors."""
 
     def __init__(self, embeddingDim, preNorm="rms", postNorm=None, residualScale=1.0, gateActivation=None, epsilon=1e-5, gpu_wrapper=None):
         if preNorm not in _NORMS or postNorm not in _NORMS:
@@ -63,7 +64,7 @@ class BlockNorm:
 
     def _desc(self, direction, stream, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics):
         """What both directions have: the layer itself, sizes and types, gate, weights, statistics."""
-        w, dim, stream_type, block_type = stream.Wrapper, self.EmbeddingDim, stream.Type, block.Type
+        w, dim, stream_type, block_type = self.Wrapper or stream.Wrapper, self.EmbeddingDim, stream.Type, block.Type
         if dim <= 0 or stream.Shape[-1] != dim:
             raise ValueError("rows of %s do not fit an embedding dimension of %d" % (stream.Shape, dim))
         if stream_type not in _ROW_TYPES or block_type not in _ROW_TYPES:
@@ -95,7 +96,7 @@ class BlockNorm:
                            postBias=None, preStatistics=None, postStatistics=None):
         """h and u from x and y; h is None for a join without a norm ahead of the next block, y and u for a norm without a
         block.  gateRows: rows that share a row of the gate (0: the gate is one vector)."""
-        shape, w, stream_type = x.Shape, x.Wrapper, x.Type
+        shape, w, stream_type = x.Shape, self.Wrapper or x.Wrapper, x.Type
         block = h if h is not None else y if y is not None else x
         block_type = block.Type
         if (u is not None and y is None) or (self.PreNorm == NORM_NONE and (h is not None or preStatistics is not None)) or \
@@ -112,7 +113,7 @@ class BlockNorm:
         """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics (y also where its values
         do not matter: without it there is no block and no dy); gradients that are None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
-        shape, w, lib, stream_type = dx.Shape, dx.Wrapper, dx._lib, dx.Type
+        shape, w, lib, stream_type = dx.Shape, self.Wrapper or dx.Wrapper, dx._lib, dx.Type
         block = dh if dh is not None else y if y is not None else dy if dy is not None else dx
         block_type = block.Type
         if dy is not None and y is None:

@@ -402,6 +402,33 @@ def test_block_norm_outputs_that_would_stay_as_they_are_are_refused():
     bare.BackwardPropagation(x, None, None, du=x, y=x, dy=x)
 
 
+def test_layers_call_the_wrapper_they_are_made_for():
+    from sharpnet_amd import embedding, normalization
+    used, own, far = [], Stub((1,)), Stub((1,), device=1)
+    own.handle = "own"
+
+    def tensor(*shape, type_="float32"):
+        t = Stub(shape, type_)
+        t.handle = "tensor's"
+        for name in ("embedding_forward", "embedding_backward", "block_norm_forward", "block_norm_backward"):
+            setattr(t, "snhip_" + name, lambda handle, *rest: used.append(handle) or 0)
+        return t
+    x, ids, table = tensor(10, 6), tensor(10, type_="int32"), tensor(7, 6)
+
+    def calls(w):
+        e, n = embedding.WordEmbedding(7, 6, gpu_wrapper=w), normalization.BlockNorm(6, gpu_wrapper=w)
+        return (lambda: e.ForwardPropagation(x, ids, table), lambda: e.BackwardPropagation(table, ids, x), lambda: n.ForwardPropagation(x, x),
+                lambda: n.BackwardPropagation(x, x, x, preStatistics=tensor(10, 2)))
+    for w, handle in ((own, "own"), (None, "tensor's")):
+        for call in calls(w):
+            call()
+        assert used == [handle] * 4
+        used.clear()
+    for call in calls(far):
+        with pytest.raises(ValueError, match="device 1"):
+            call()
+
+
 def test_workspace_of_a_layer():
     """One for each wrapper; a longer one leaves the one before in place until Dispose."""
     from sharpnet_amd.gpu_tensor import LayerWorkspace
