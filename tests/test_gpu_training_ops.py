@@ -152,6 +152,25 @@ def test_embedding_backward(gpu_wrapper, tokens, vocabulary, dim, ids, rows):
         assert np.array_equal(into.ToNumpy()[absent], start[absent])
 
 
+EXACT_TOKENS = [(70000, 7, 3, "int64"), (70000, 40, 36, "int32"), (20000, 1, 12, "int32"), (40000, 30000, 20, "float32"), (9000, 140001, 8, "int32"),
+                (8192, 600, 40, "int32"), (5000, 3, 300, "int64"), (4096, 1, 256, "int32"), (3000, 2000, 30, "int32"), (66000, 100, 200, "int32")]
+
+
+@pytest.mark.parametrize("tokens,vocabulary,dim,ids", EXACT_TOKENS)
+@pytest.mark.parametrize("rows", ["float32", "bfloat16"])
+def test_embedding_gradient_loses_and_doubles_no_token(gpu_wrapper, tokens, vocabulary, dim, ids, rows):
+    """Whole numbers of up to 15: every partial sum is below 2^24, so exact in whatever order, and so is the scale of 1/2: the
+    gradient has the formula's bits, and one token too few or too many would show."""
+    from sharpnet_amd import embedding
+    w, rng = gpu_wrapper, np.random.default_rng(tokens + dim)
+    x = make_ids(rng, tokens, vocabulary, ids)
+    dy = (rng.integers(1, 16, (tokens, dim)) * rng.choice([-1, 1], (1, dim))).astype(np.float32)
+    assert tokens * 15 < 2 ** 24
+    dW = empty(w, (vocabulary, dim))
+    embedding.WordEmbedding(vocabulary, dim, 0.5).BackwardPropagation(dW, tensor(w, x, ids), tensor(w, dy, rows))
+    assert np.array_equal(dW.ToNumpy().reshape(vocabulary, dim), ref.embedding_backward(x, dy, vocabulary, 0.5)[0])
+
+
 @pytest.mark.parametrize("tokens,words,dim", [(4000, 10, 20), (2000, 20, 256), (4096, 400, 30), (3000, 1, 129), (9000, 700, 16), (20000, 900, 40)])
 def test_embedding_backward_of_ids_that_share_a_bucket(gpu_wrapper, tokens, words, dim):
     """Ids that are all multiples of 512: whatever sorts them by their low bits has them in one place."""
@@ -338,6 +357,91 @@ def test_block_norm_gradient_of_a_saturated_gate(gpu_wrapper, activation, gate_r
     e = np.exp(-k * np.abs(g.astype(np.float64)))
     want = 0.5 * du.astype(np.float64) * y * (k * k * e / (1 + e) ** 2)
     within(dgate.ToNumpy().reshape(want.shape), want, (16 + 2 * k * np.abs(g)) * ref.U * np.abs(want) + ref.TINY, "d_gate")
+
+
+EXACT_ROWS = [(1, 5, None), (100, 60, 0), (4099, 64, 16), (3000, 100, 7), (5000, 128, 1), (2048, 512, 0), (1500, 516, 300), (6200, 700, 0),
+              (4100, 1024, 2), (4150, 1023, 9), (6200, 1028, 0), (2500, 2044, 1000), (1030, 4096, 1), (600, 5001, 50), (1300, 8192, 0), (9000, 33, 4000)]
+
+
+@pytest.mark.parametrize("rows,dim,gate_rows", EXACT_ROWS)
+@pytest.mark.parametrize("stream,block", [("float32", "float32"), ("float32", "bfloat16"), ("bfloat16", "bfloat16")])
+def test_block_norm_column_sums_lose_and_double_no_row(gpu_wrapper, rows, dim, gate_rows, stream, block):
+    """Whole numbers all the way: mean 0 and 1 / deviation 1 as the statistics, weights and gates of 1 and 2, so that every
+    term of the column sums is a whole number and every partial sum below 2^24 (2^8 for a gate's row in bf16): the formula's bits."""
+    from sharpnet_amd import normalization
+    w, rng = gpu_wrapper, np.random.default_rng(rows + dim)
+    u, dh, y, du = (rng.integers(1, 4, (rows, dim)).astype(np.float32) for _ in range(4))
+    sign = rng.choice([-1, 1], dim).astype(np.float32)
+    dh, du = dh * sign, du * sign
+    plain = np.tile(np.array([0, 1], np.float32), (rows, 1))
+    gs = tensor(w, plain)
+    weight = rng.choice([1, 2], dim).astype(np.float32)
+    vec = lambda: empty(w, (dim,))  # noqa: E731
+    # the norm ahead of the next block
+    dx, dw, db = empty(w, (rows, dim), stream), vec(), vec()
+    layer = normalization.BlockNorm(dim, "layer", "layer")
+    dy = empty(w, (rows, dim), block)
+    layer.BackwardPropagation(dx, tensor(w, u, stream), tensor(w, dh, block), y=tensor(w, y, block), dy=dy, postStatistics=gs, preStatistics=gs,
+                              dPreWeight=dw, dPreBias=db)
+    u64, dh64, y64, du64 = (a.astype(np.float64) for a in (u, dh, y, du))
+    assert np.array_equal(dw.ToNumpy(), (dh64 * u64).sum(0)) and np.array_equal(db.ToNumpy(), dh64.sum(0))
+    # the norm behind the block and its gate
+    gate = None if gate_rows is None else rng.choice([1, 2], dim if gate_rows == 0 else (-(-rows // gate_rows), dim)).astype(np.float32)
+    dpw, dpb, bias = vec(), vec(), np.ones(dim, np.float32)
+    dgate = None if gate is None else empty(w, gate.shape, block if gate_rows else "float32")
+    layer.BackwardPropagation(dx, None, None, du=tensor(w, du, stream), y=tensor(w, y, block), dy=dy, postStatistics=gs, postWeight=tensor(w, weight),
+                              postBias=tensor(w, bias), dPostWeight=dpw, dPostBias=dpb, dGate=dgate, gateRows=gate_rows or 0,
+                              gate=None if gate is None else tensor(w, gate, block if gate_rows else "float32"))
+    t = du64
+    if gate is not None:
+        each = du64 * (y64 * weight + bias)
+        if gate_rows == 0:
+            assert np.array_equal(dgate.ToNumpy(), each.sum(0))
+        else:
+            want = np.zeros(gate.shape)
+            np.add.at(want, np.arange(rows) // gate_rows, each)
+            assert np.array_equal(dgate.ToNumpy().reshape(gate.shape), ref.bf16(want) if block == "bfloat16" else want)
+        t = du64 * ref.gate_per_row(gate, gate_rows, rows, dim)
+    assert np.array_equal(dpw.ToNumpy(), (t * y64).sum(0)) and np.array_equal(dpb.ToNumpy(), t.sum(0))
+    assert np.array_equal(dx.ToNumpy().reshape(rows, dim), du)
+
+
+@pytest.mark.parametrize("rows,dim,stream,block", [(70, 20, "float32", "float32"), (70, 61, "bfloat16", "bfloat16"), (40, 100, "float32", "bfloat16"),
+                                                   (40, 127, "float32", "float32"), (20, 200, "bfloat16", "bfloat16"), (20, 510, "float32", "float32"),
+                                                   (600, 700, "float32", "bfloat16"), (9, 1001, "float32", "float32"), (600, 1500, "bfloat16", "bfloat16"),
+                                                   (5, 4096, "float32", "bfloat16"), (520, 5001, "float32", "float32"), (4, 8190, "bfloat16", "bfloat16")])
+def test_block_norm_rows_that_are_not_finite_spoil_no_others(gpu_wrapper, rows, dim, stream, block):
+    """NaN and infinities in a row, its gradients, statistics and gate: the other rows keep their bits."""
+    from sharpnet_amd import normalization
+    w, rng = gpu_wrapper, np.random.default_rng(dim)
+    c = norm_case(rng, rows, dim, "layer", "rms", 1, True, stream, block)
+    vectors = {k: tensor(w, v) for k, v in c["weights"].items()}
+    du, dh = rounded(rng.normal(0, 1, (rows, dim)), stream), rounded(rng.normal(0, 1, (rows, dim)), block)
+    layer = normalization.BlockNorm(dim, "layer", "rms", residualScale=0.7, gateActivation="tanh")
+    bad = sorted({1, rows // 2, rows - 2})
+
+    def results(spoil):
+        host = {"x": c["x"].copy(), "y": c["y"].copy(), "gate": c["gate"].copy(), "du": du.copy(), "dh": dh.copy()}
+        if spoil:
+            for i, r in enumerate(bad):
+                for k, name in enumerate(host):
+                    host[name][r, (7 * k + i) % dim] = (np.nan, np.inf, -np.inf)[(i + k) % 3]
+        x, y, gate, gdu, gdh = (tensor(w, host[k], stream if k in ("x", "du") else block) for k in host)
+        out = {"u": empty(w, (rows, dim), stream), "h": empty(w, (rows, dim), block), "dx": empty(w, (rows, dim), stream),
+               "dy": empty(w, (rows, dim), block), "dgate": empty(w, (rows, dim), block), "pre": empty(w, (rows, 2)), "post": empty(w, (rows, 2))}
+        layer.ForwardPropagation(x, out["h"], y=y, u=out["u"], gate=gate, gateRows=1, preWeight=vectors["pre_weight"], preBias=vectors["pre_bias"],
+                                 postWeight=vectors["post_weight"], postBias=vectors["post_bias"], preStatistics=out["pre"], postStatistics=out["post"])
+        layer.BackwardPropagation(out["dx"], out["u"], gdh, du=gdu, y=y, dy=out["dy"], gate=gate, dGate=out["dgate"], gateRows=1,
+                                  preWeight=vectors["pre_weight"], preStatistics=out["pre"], postWeight=vectors["post_weight"],
+                                  postBias=vectors["post_bias"], postStatistics=out["post"])
+        return {k: t.ToNumpy().reshape(rows, -1) for k, t in out.items()}
+    clean, spoiled = results(False), results(True)
+    others = np.setdiff1d(np.arange(rows), bad)
+    for k in clean:
+        assert np.all(np.isfinite(clean[k])), k
+        assert np.array_equal(clean[k][others], spoiled[k][others]), k
+        if k not in ("dgate", "post"):
+            assert not np.any(np.all(np.isfinite(spoiled[k][bad]), axis=1)), k
 
 
 def test_block_norm_rows_without_spread_and_missing_parts(gpu_wrapper):
@@ -807,6 +911,34 @@ def test_scratch_memory_that_has_grown_after_a_capture(gpu_wrapper):
             hip.hipGraphDestroy(graph)
         check_status(w.lib.snhip_stream_destroy(stream), "snhip_stream_destroy")
         layer.Dispose()
+
+
+def test_embedding_gradients_with_scratch_memory_on_two_handles_at_once(gpu_wrapper):
+    """Long batches of two handles on two streams in turn, one layer: whole numbers, so the formula's bits (one token lost or read
+    from the other batch would show)."""
+    from sharpnet_amd import GPUWrapper, embedding
+    from sharpnet_amd.hiplib import check_status
+    rng, vocabulary, dim = np.random.default_rng(15), 2000, 24
+    layer, jobs = embedding.WordEmbedding(vocabulary, dim, 2.0), []
+    for tokens in (50000, 8200):
+        w, stream = GPUWrapper(0), ctypes.c_void_p()
+        check_status(w.lib.snhip_stream_create(ctypes.byref(stream)))
+        x, dy = make_ids(rng, tokens, vocabulary, "int64"), rng.integers(-8, 9, (tokens, dim)).astype(np.float32)
+        jobs.append((w, stream, tensor(w, x, "int64"), tensor(w, dy), empty(w, (vocabulary, dim)), ref.embedding_backward(x, dy, vocabulary, 2.0)[0]))
+        w.synchronize()
+        check_status(w.lib.snhip_set_stream(w.handle, stream))
+    for _ in range(3):
+        for _ in range(10):
+            for w, _, x, dy, dW, _ in jobs:
+                layer.BackwardPropagation(dW, x, dy)
+        for w, _, _, _, dW, want in jobs:
+            assert np.array_equal(dW.ToNumpy(), want)
+            dW.SetValue(float("nan"))
+            w.synchronize()
+    for w, stream, *_ in jobs:
+        check_status(w.lib.snhip_set_stream(w.handle, None))
+        check_status(w.lib.snhip_stream_destroy(stream))
+    layer.Dispose()
 
 
 def test_one_layer_on_two_streams_of_a_handle(gpu_wrapper):

@@ -507,6 +507,68 @@ def test_scratch_memory_goes_by_stream(lib, handle):
     assert lib.snhip_get_stream(handle, ctypes.byref(p)) == 0 and not p.value
 
 
+def test_one_layers_scratch_memory_in_two_threads():
+    """Two threads, each with a handle of its own: gradients of one layer never get the other's scratch memory, whatever their sizes."""
+    import threading
+    import time
+    from sharpnet_amd import embedding, normalization
+    e, n, wrong = embedding.WordEmbedding(7, 6), normalization.BlockNorm(6, "rms"), []
+
+    class Wrapper:
+        device_id = 0
+
+        def __init__(self, number):
+            self.lib, self.handle, self.base, self.made = self, number, A * (1 + number), 0
+
+        def allocate(self, nbytes):
+            time.sleep(1e-4)
+            self.made += 1
+            return self.base + (self.made << 12)
+
+        def release(self, pointer, nbytes):
+            pass
+
+        def snhip_get_stream(self, handle, out):
+            time.sleep(1e-4)
+            out._obj.value = 0x1000 * handle
+            return 0
+
+        def size(self, desc, out):
+            time.sleep(1e-4)
+            out._obj.value = (desc._obj.tokens if isinstance(desc._obj, hiplib.EmbeddingDesc) else desc._obj.rows) * 4
+            return 0
+        snhip_embedding_backward_workspace_size = snhip_block_norm_backward_workspace_size = size
+
+        def check(self, rows, pointer, nbytes):
+            if not self.base <= pointer < self.base + A or nbytes < 4 * rows:
+                wrong.append((self.handle, rows, pointer, nbytes))
+            return 0
+
+        def snhip_embedding_backward(self, handle, desc, ids, dy, table, accumulate, workspace, nbytes):
+            return self.check(desc._obj.tokens, workspace, nbytes)
+
+        def snhip_block_norm_backward(self, handle, desc, workspace, nbytes):
+            return self.check(desc._obj.rows, workspace, nbytes)
+
+    def run(number):
+        w = Wrapper(number)
+
+        def on(shape, type_="float32"):
+            t = Stub(shape, type_)
+            t.Wrapper = t._lib = w
+            return t
+        for k in range(60):
+            rows = 3 + number + k
+            e.BackwardPropagation(on((7, 6)), on((rows,), "int32"), on((rows, 6)))
+            n.BackwardPropagation(on((rows, 6)), on((rows, 6)), on((rows, 6)), preStatistics=on((rows, 2)), dPreWeight=on((6,)))
+    threads = [threading.Thread(target=run, args=(number,)) for number in (1, 2, 3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 def test_adamw_clears_its_states_where_its_steps_go(bits):
     """Parameters of two wrappers of a device: the states are cleared by the one that the steps are issued by, and are clear
