@@ -28,8 +28,7 @@ struct BlockNormParams {
     float eps, scale, inv_dim;
     // backward: a workgroup takes a chunk of rows
     float* partial;            // [vector][chunk][dim]: column sums of pre weight, pre bias, post weight, post bias, gate
-    long long gate_groups;     // runs of rows with the same gate row (1 without a gate)
-    long long rows_per_group;
+    long long rows_per_group;  // rows with the same gate row (all without a gate)
     int flush;                 // 1: a chunk is `groups_per_chunk` whole groups; 0: one of `chunks_per_group` parts of a group
     int groups_per_chunk, chunks_per_group, rows_per_chunk, chunks;
     int slot[5];               // which vector of `partial` a column sum goes to, -1: not wanted

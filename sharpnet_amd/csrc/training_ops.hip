@@ -488,7 +488,7 @@ int snhip_block_norm_backward(void* handle, const snhip_block_norm_desc* desc, v
     if (!scope.ok()) return SNHIP_STATUS_NOT_INITIALIZED;
     BlockNormParams p = block_norm_params(desc);
     p.partial = static_cast<float*>(workspace);
-    p.gate_groups = b.groups, p.rows_per_group = b.rows_per_group, p.flush = b.flush;
+    p.rows_per_group = b.rows_per_group, p.flush = b.flush;
     p.groups_per_chunk = b.groups_per_chunk, p.chunks_per_group = b.chunks_per_group, p.rows_per_chunk = b.rows_per_chunk;
     p.chunks = b.chunks;
     for (int k = 0; k < 5; ++k) p.slot[k] = b.slots[k];
