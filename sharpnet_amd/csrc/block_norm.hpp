@@ -165,6 +165,12 @@ __device__ __forceinline__ float row_sum(float a, float (*lds)[2][TPR / 64 + 1],
 // The sigmoid from the hardware's exponential and reciprocal (1 ulp each; the exponent's rounding adds |g| 2^-24).
 // tanh x = (1 - e) / (1 + e) with e = exp(-2 |x|) from |x| = 1/4 on, where the difference keeps its digits (4 ulp), and its
 // Taylor series to x^9 below (the next term is under 2^-26 of x).
+// (r = 1 / (1 + e))
+__device__ __forceinline__ float tanh_from(float x, float e, float r) {
+    const float z = x * x, large = copysignf((1.0f - e) * r, x);
+    const float series = ((((62.0f / 2835.0f * z - 17.0f / 315.0f) * z + 2.0f / 15.0f) * z - 1.0f / 3.0f) * z) * x + x;
+    return fabsf(x) < 0.25f ? series : large;
+}
 __device__ __forceinline__ f32x4 gate_values(f32x4 g, int act) {
     if (act == GATE_SIGMOID) {
 #pragma unroll
@@ -172,35 +178,43 @@ __device__ __forceinline__ f32x4 gate_values(f32x4 g, int act) {
     } else if (act == GATE_TANH) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float x = g[j], a = fabsf(x), z = x * x;
-            const float e = __builtin_amdgcn_exp2f(a * -2.88539008177792681f);
-            const float large = copysignf((1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e), x);
-            const float series = ((((62.0f / 2835.0f * z - 17.0f / 315.0f) * z + 2.0f / 15.0f) * z - 1.0f / 3.0f) * z) * x + x;
-            g[j] = a < 0.25f ? series : large;
+            const float e = __builtin_amdgcn_exp2f(fabsf(g[j]) * -2.88539008177792681f);
+            g[j] = tanh_from(g[j], e, __builtin_amdgcn_rcpf(1.0f + e));
         }
     }
     return g;
 }
-// act(g) in place of g, and its slope: from e = exp(-|g|) or exp(-2 |g|), e / (1 + e)^2 and 4 e / (1 + e)^2.  (q - q q and 1 - q q of
-// the rounded q lose the digits of a gate near its limit: a sigmoid's slope off by 6 % at g = 16 and zero from 18 on.)
-__device__ __forceinline__ f32x4 gate_slopes(f32x4& g, int act) {
+// Backward through v * act(g): t becomes t * act(g), sum gets t * v * act'(g).  The slopes are q (1 - q) with 1 - q = e q, e = exp(-g),
+// and 4 e / (1 + e)^2 with e = exp(-2 |g|): q - q q and 1 - q q of the rounded q lose the digits of a gate near its limit (a
+// sigmoid's slope off by 6 % at g = 16 and zero from 18 on).
+// IN_BRANCH: all of it within the activation's branch, where no slopes are kept, for the kernels of long rows, which have no
+// register left (575 x 6240, fp32 stream, bf16 block, two norms with biases: 31 us, 45 us the other way); the others wait for v
+// later without it (33520 x 1001 bf16, a gate vector: 154 us, 168 us).
+template <bool IN_BRANCH>
+__device__ __forceinline__ void gate_gradient(f32x4& t, f32x4& sum, f32x4 v, f32x4 g, int act) {
     f32x4 slope = {1.0f, 1.0f, 1.0f, 1.0f};
+    auto put = [&](int j, float q, float s) {
+        if constexpr (IN_BRANCH)
+            sum[j] += t[j] * v[j] * s, t[j] *= q;
+        else
+            g[j] = q, slope[j] = s;
+    };
     if (act == GATE_SIGMOID) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const float e = __builtin_amdgcn_exp2f(fabsf(g[j]) * -1.44269504088896341f), r = __builtin_amdgcn_rcpf(1.0f + e), q = e * r;
-            slope[j] = q * r;
-            g[j] = g[j] < 0.0f ? q : r;
+            const float e = __builtin_amdgcn_exp2f(g[j] * -1.44269504088896341f), q = __builtin_amdgcn_rcpf(1.0f + e);
+            put(j, q, fminf(e, 0x1p+126f) * q * q);  // (beyond that q is zero)
         }
     } else if (act == GATE_TANH) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float e = __builtin_amdgcn_exp2f(fabsf(g[j]) * -2.88539008177792681f), r = __builtin_amdgcn_rcpf(1.0f + e);
-            slope[j] = 4.0f * e * r * r;
+            put(j, tanh_from(g[j], e, r), 4.0f * e * r * r);
         }
-        g = gate_values(g, act);
+    } else if constexpr (IN_BRANCH) {
+        sum += t * v, t *= g;
     }
-    return slope;
+    if constexpr (!IN_BRANCH) sum += t * v * slope, t *= g;
 }
 
 // which row of the workgroup's rows this thread works on: the same for a wavefront where a row takes one or more
@@ -454,9 +468,7 @@ __global__ void __launch_bounds__(TPR > 256 ? TPR : 256) block_norm_backward_ker
                         g = P::value(now.g[n], n, lane, dim);
                     else
                         g = P::vector(static_cast<const float*>(p.gate), n, lane, dim, 1.0f);
-                    const f32x4 slope = gate_slopes(g, p.act);  // (g: the gate's values from here on)
-                    acc_g[n] += t[n] * v * slope;
-                    t[n] *= g;
+                    gate_gradient<(TPR > 256)>(t[n], acc_g[n], v, g, p.act);
                 }
                 if constexpr (MODE == 2) {
                     acc_pw[n] += t[n] * hat[n];

@@ -38,6 +38,11 @@ class BlockNorm:
         self._workspace = LayerWorkspace()
         self._mine = threading.local()  # a descriptor for each thread and direction; a call fills in what is not the layer's kind
 
+    def __setattr__(self, name, value):
+        object.__setattr__(self, name, value)
+        if name in ("EmbeddingDim", "PreNorm", "PostNorm", "GateActivation"):
+            object.__setattr__(self, "_kind", object())  # what a thread has laid out for calls of the layer as it was is over
+
     def _rows(self, w, t, name, shape, type_):
         """The address of t, which is None or has rows like those of shape, in the given type, on the wrapper's device."""
         if t is None:
@@ -72,10 +77,9 @@ class BlockNorm:
         if gateRows < 0:
             raise ValueError("gateRows is %d" % gateRows)
         rows, mine = math.prod(stream.Shape) // dim, self._mine.__dict__
-        kind = self.PreNorm, self.PostNorm, self.GateActivation, dim
-        if mine.get("kind") != kind:  # (the first call, or the layer has been changed)
+        if mine.get("kind") is not self._kind:  # (the first call, or the layer has been changed)
             mine.clear()
-            mine["kind"], self._vectorShape = kind, [dim]
+            mine["kind"], self._vectorShape = self._kind, [dim]
         d = mine.get(direction)
         if d is None:
             d = mine[direction] = BlockNormDesc(pre_norm=self.PreNorm, post_norm=self.PostNorm, gate_activation=self.GateActivation, dim=dim)
@@ -99,8 +103,8 @@ class BlockNorm:
         shape, w, stream_type = x.Shape, self.Wrapper or x.Wrapper, x.Type
         block = h if h is not None else y if y is not None else x
         block_type = block.Type
-        if (u is not None and y is None) or (self.PreNorm == NORM_NONE and (h is not None or preStatistics is not None)) or \
-                (self.PostNorm == NORM_NONE and postStatistics is not None):
+        if (y is None and u is not None) or (not self.PreNorm and (h is not None or preStatistics is not None)) or \
+                (postStatistics is not None and not self.PostNorm):
             raise ValueError("there is no u without y, and neither h nor statistics without their norm")
         d = self._desc("forward", x, block, gate, gateRows, preWeight, preBias, postWeight, postBias, preStatistics, postStatistics)
         d.x, d.u = pointer_on(w, x), self._rows(w, u, "u", shape, stream_type)

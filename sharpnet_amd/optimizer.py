@@ -86,10 +86,11 @@ class AdamW:
         if learningRate is not None:
             self.LearningRate = learningRate
         if self._plan is not None:
-            if self.StepCount + 1 > 0x7FFFFFFF:
-                raise ValueError("step %d" % (self.StepCount + 1))
+            step = self.StepCount + 1
+            if step > 0x7FFFFFFF:
+                raise ValueError("step %d" % step)
             d = AdamwStepDesc()
-            d.step, d.learning_rate, d.beta1, d.beta2 = self.StepCount + 1, self.LearningRate, self.Beta1, self.Beta2
+            d.step, d.learning_rate, d.beta1, d.beta2 = step, self.LearningRate, self.Beta1, self.Beta2
             d.epsilon, d.gradient_scale, d.seed = self.Epsilon, gradientScale, self.Seed
             check_status(self._lib.snhip_adamw_step(self._wrapper.handle, self._plan, ctypes.byref(d)), "snhip_adamw_step")
         self.StepCount += 1
