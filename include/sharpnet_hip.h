@@ -59,7 +59,8 @@ int snhip_reserve_workspace(void* handle, size_t bytes);
 int snhip_get_workspace_size(void* handle, size_t* bytes);
 /* No counterpart is bound by the reference (it never calls cublasSetStream, so
  * GEMMs run on the legacy default stream); offered for callers with their own
- * hipStream_t.  stream == NULL selects the null stream again. */
+ * hipStream_t.  stream == NULL selects the null stream again.  The handle's scratch buffer (above) is one for all its streams:
+ * calls that use it have to have finished on the stream before. */
 int snhip_set_stream(void* handle, void* stream);
 /* The stream that snhip_set_stream selected (NULL: the null stream), for callers whose scratch memory goes by it: calls before
  * and after a change of streams are not ordered. */

@@ -115,7 +115,8 @@ class BlockNorm:
                             preStatistics=None, dPreWeight=None, dPreBias=None, postWeight=None, postBias=None, postStatistics=None,
                             dPostWeight=None, dPostBias=None, accumulate=False, workspace=None):
         """dx and dy from dh and du (either may be None), with the forward pass's u, y, gate and statistics (y also where its values
-        do not matter: without it there is no block and no dy); gradients that are None are skipped, ``accumulate`` adds to those of the vectors.  Without a ``workspace`` the layer keeps one of its
+        do not matter: without it there is no block and no dy); gradients that are None are skipped, ``accumulate`` adds to those of
+        the vectors.  Without a ``workspace`` the layer keeps one of its
         own (see WordEmbedding.BackwardPropagation)."""
         shape, w, lib, stream_type = dx.Shape, self.Wrapper or dx.Wrapper, dx._lib, dx.Type
         block = dh if dh is not None else y if y is not None else dy if dy is not None else dx
